@@ -374,6 +374,51 @@ int buda_prestride(const void *src, int elem_bytes, const uint32_t shape[4], con
 int buda_i8_gemm(const void *A, int64_t M, int64_t K, int64_t lda, const void *W_tiles, int64_t N, const float *scale,
                  int64_t scale_len, float zero_point, int out_mode, void *C, int64_t ldc, void *stream);
 
+/* ------------------------------------------------------------------ a few rows against block-float weights
+ * Products of 1..64 rows (the tokens of a decoding step) with weights stored as block-float queue images, each weight read
+ * once.  Images are those of buda_bfp8b_gemm, for Bfp8_b, Bfp4_b and Bfp2_b alike: geometry grid 1x1, ublock 1x1, order R,
+ * no tile header, default byte layout, 16-byte aligned; sizes that fill no tile are padded to whole tiles (with zeros, as
+ * the pack writes them).  Every stored weight counts at its exact value, sums are binary32.  Results do not depend on
+ * what else runs: the same call gives the same bits.  K, N, H, I <= 2^24. */
+#define BUDA_MAX_FEW_ROWS 64
+
+/* Y[M,N] (BUDA_DF_Float16_b or BUDA_DF_Float32, row stride ldy elements) = A[M,K] (bfloat16, row stride lda elements) @ W,
+ * W a [K,N] tensor as an image of format w_df: ceil(K/32) * ceil(N/32) tile records.  Any K, N >= 1 and 0 <= M <= 64;
+ * Y must not overlap A.  The few-row counterpart of buda_bfp8b_gemm (pybuda/pybuda/op/eval/pybuda/matmul.py:20-33; weight
+ * formats pybuda/csrc/passes/amp.cpp:457-500). */
+int buda_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, const void *W_tiles, int64_t N, int w_df, void *Y, int64_t ldy,
+                    int y_df, void *stream);
+
+/* The router of a mixture of experts: scores X[T,H] (bfloat16) @ W_router[E,H]^T (bfloat16 or binary32, one row for each
+ * expert), their softmax over the experts, and for each token the `top` experts of the largest scores in descending order,
+ * the lowest index first among equal ones; a NaN score ranks below every number.  weights[T,top] (binary32) are the softmax
+ * values, divided by their sum over the chosen experts when `renormalize` is not 0; ids[T,top] (int32) the experts.
+ * T <= 64, E <= 256, top <= 16 and <= E. */
+#define BUDA_MAX_EXPERTS 256
+#define BUDA_MAX_TOP 16
+int buda_moe_route(const void *X, int64_t T, int64_t H, int64_t ldx, const void *W_router, int router_df, int64_t ldw, int64_t E,
+                   int top, int renormalize, float *weights, int32_t *ids, void *stream);
+
+#define BUDA_ACT_SILU 0   /* v / (1 + exp(-v))           */
+#define BUDA_ACT_GELU 1   /* v / 2 * (1 + erf(v / sqrt 2)) */
+
+/* The experts' products for routed tokens:
+ *   Y[t] (bfloat16) = sum_s weights[t,s] * (act(X[t] @ gate_e) * (X[t] @ up_e)) @ down_e,  e = ids[t,s]
+ * gate, up: images of [H,I] matrices, down: of [I,H] matrices, the E experts of one kind one after another (what packing a
+ * [1,E,H,I] tensor gives); up == NULL: experts without a gate, act(X[t] @ gate_e) alone.  A slot whose id is outside
+ * [0, E) counts nothing (a dropped or padded slot); a token without a slot gets zeros; an expert named twice by a token
+ * counts with the sum of its weights.  Y may be X.  workspace: buda_moe_workspace_bytes(T, top, I) bytes, 16-byte
+ * aligned, for this call alone until it has run (two captured graphs that replay at the same time need one each). */
+int64_t buda_moe_workspace_bytes(int64_t T, int top, int64_t I);
+int buda_moe_experts(const void *X, int64_t T, int64_t H, int64_t ldx, const float *weights, const int32_t *ids, int top,
+                     const void *gate, const void *up, const void *down, int64_t E, int64_t I, int w_df, int act, void *Y,
+                     int64_t ldy, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* The whole layer: buda_moe_route into weights / ids, then buda_moe_experts with them, the launches overlapping. */
+int buda_moe_layer(const void *X, int64_t T, int64_t H, int64_t ldx, const void *W_router, int router_df, int64_t ldw, int top,
+                   int renormalize, const void *gate, const void *up, const void *down, int64_t E, int64_t I, int w_df, int act,
+                   float *weights, int32_t *ids, void *Y, int64_t ldy, void *workspace, uint64_t workspace_bytes, void *stream);
+
 /* Inter-process handles for device memory from buda_malloc, so that one process per GPU can hand its
  * output matrix to its peers.  export: 64-byte handle of an allocation's base pointer.  open: maps a
  * peer's allocation into this process (peer access is enabled on demand).  close: unmaps it. */
@@ -398,7 +443,8 @@ enum {
     BUDA_DEVSTAT_UNPACK_FULL_WAIT = 3,
     BUDA_DEVSTAT_UNPACK_EMPTY_WAIT = 4,
     BUDA_DEVSTAT_GEMM_WAIT = 5,
-    BUDA_DEVSTAT_SELFTEST_WAIT = 6     /* buda_selftest_bounded_wait (buda_cuda_testing.h): the wait that nothing completes ran out */
+    BUDA_DEVSTAT_SELFTEST_WAIT = 6,    /* buda_selftest_bounded_wait (buda_cuda_testing.h): the wait that nothing completes ran out */
+    BUDA_DEVSTAT_FEW_ROWS_WAIT = 7     /* few-row products: a warp waited too long for its weights */
 };
 
 /* Number of kernels this library has launched in this process (for launch accounting). */

@@ -1,0 +1,398 @@
+"""GPU tests of the few-row operators on block-float weights (bfp_matvec, moe_route, moe_experts, moe_layer) against plain
+64-bit implementations on the oracle-decoded weights.
+
+Tolerances, derived: a product of two stored operands (8 bits each) is exact in binary32.  Adding n of them in any order,
+each addition off by at most one last place of a partial sum that no sum of magnitudes exceeds, is off by at most
+n 2^-23 sum |products|.  Rounding the result to bfloat16 adds 2^-8 of it, to binary32 2^-24.  The experts' intermediate
+is carried in two bfloat16 pieces, off by at most 2^-16 of it; the slope of silu and gelu stays below 1.13, and their
+binary32 evaluation is off by a few units of 2^-24, for which 2^-19 of the value is allowed."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ["Bfp8_b", "Bfp4_b", "Bfp2_b"]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.fail("these tests need a CUDA device; there is no CPU fallback to test")
+    from pybuda import cuda_ops
+
+    return cuda_ops
+
+
+def _pad32(n):
+    return -(-n // 32) * 32
+
+
+def _store(oracle, w, df):
+    """(queue image as CUDA bytes, float64 values it stands for) of a [K,N] matrix, zero-padded to tiles."""
+    k, n = w.shape
+    p = np.zeros((1, 1, _pad32(k), _pad32(n)), np.float32)
+    p[0, 0, :k, :n] = w
+    code = getattr(oracle, df)
+    img = oracle.tilize_pack(p, code)
+    return torch.from_numpy(img).cuda(), oracle.unpack_untilize(img, code, p.shape)[0, 0, :k, :n].astype(np.float64)
+
+
+def _rand(shape, seed, scale=1.0):
+    return (np.random.default_rng(seed).standard_normal(shape) * scale).astype(np.float32)
+
+
+def _bf16(x):
+    return torch.from_numpy(np.ascontiguousarray(x)).bfloat16()
+
+
+def _check_sum(got, a, w, dtype):
+    """got = a @ w for exact operands a, w (float64 numpy)."""
+    ref, mag = a @ w, np.abs(a) @ np.abs(w)
+    tol = (a.shape[1] + 16) * 2.0 ** -23 * mag + np.abs(ref) * (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24) + 2.0 ** -133
+    err = np.abs(got.double().cpu().numpy() - ref)
+    assert got.dtype == dtype and (err <= tol).all(), f"worst {np.max(err / tol)} of the tolerance at {np.unravel_index(np.argmax(err / tol), err.shape)}"
+
+
+# ------------------------------------------------------------------------------------------------ matvec
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("m,k,n", [(1, 32, 32), (1, 1, 1), (2, 17, 33), (3, 64, 128), (8, 100, 130), (9, 256, 96), (16, 544, 288), (17, 96, 160),
+                                   (33, 320, 64), (64, 70, 40), (1, 4096, 256), (5, 2080, 1100)])
+def test_matvec_shapes(ops, oracle, df, m, k, n):
+    img, w = _store(oracle, _rand((k, n), m + k + n, 0.05), df)
+    a = _bf16(_rand((m, k), 1))
+    for dtype in (torch.bfloat16, torch.float32):
+        got = ops.bfp_matvec(a.cuda(), img, n, getattr(ops.DF, df), out_dtype=dtype)
+        _check_sum(got, a.double().numpy(), w, dtype)
+    rc, st = ops._cabi.device_status()
+    assert rc == 0 and st == 0
+
+
+@pytest.mark.parametrize("df", FORMATS)
+def test_matvec_one_hot_rows_copy_the_stored_values(ops, oracle, df):
+    k, n = 96, 160
+    img, w = _store(oracle, _rand((k, n), 3), df)      # magnitudes on both sides of 2: shared exponents on both sides of 128
+    a = torch.eye(k)[:64].bfloat16()
+    got = ops.bfp_matvec(a.cuda(), img, n, getattr(ops.DF, df), out_dtype=torch.float32).cpu().numpy()
+    assert np.array_equal(got, w[:64].astype(np.float32))
+    got = ops.bfp_matvec(torch.eye(k)[32:].bfloat16().cuda(), img, n, getattr(ops.DF, df)).cpu()
+    assert torch.equal(got.float(), torch.from_numpy(w[32:].astype(np.float32)))
+
+
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("exponent", [1, 2, 7, 64, 126, 127, 128, 129, 190, 253])
+def test_matvec_shared_exponents_of_the_whole_range(ops, oracle, df, exponent):
+    """Images of one shared exponent and all data patterns; the activation brings the product back to the middle."""
+    code, m = getattr(ops.DF, df), {"Bfp8_b": 7, "Bfp4_b": 3, "Bfp2_b": 1}[df]
+    rec = {"Bfp8_b": 1088, "Bfp4_b": 576, "Bfp2_b": 320}[df]
+    raw = np.random.default_rng(exponent).integers(0, 256, rec, dtype=np.uint8)
+    raw[:64] = exponent
+    w = oracle.unpack_untilize(raw, getattr(oracle, df), (1, 1, 32, 32))[0, 0].astype(np.float64)
+    back = 2.0 ** min(127, max(-120, 127 - exponent))
+    a = torch.eye(32).mul(back).bfloat16()
+    got = ops.bfp_matvec(a.cuda(), torch.from_numpy(raw).cuda(), 32, code, out_dtype=torch.float32).cpu().numpy()
+    assert np.array_equal(got.astype(np.float64), w * back)
+    assert np.abs(w).max() >= 2.0 ** (exponent - 127) * (1 if m > 1 else 0.5)
+
+
+def test_matvec_not_finite_activations_stay_in_their_row(ops, oracle):
+    k, n = 64, 96
+    img, w = _store(oracle, _rand((k, n), 5) + 0.1, "Bfp4_b")
+    a = _bf16(_rand((4, k), 6))
+    a[1, 7], a[2, 63], a[2, 0] = float("nan"), float("inf"), float("-inf")
+    got = ops.bfp_matvec(a.cuda(), img, n, ops.DF.Bfp4_b, out_dtype=torch.float32).cpu()
+    assert torch.isnan(got[1]).all() and not torch.isfinite(got[2]).any()
+    _check_sum(got[[0, 3]], a.double().numpy()[[0, 3]], w, torch.float32)
+
+
+def test_matvec_strides_alignment_and_neighbours(ops, oracle):
+    k, n = 75, 70
+    img, w = _store(oracle, _rand((k, n), 8, 0.1), "Bfp8_b")
+    for offset, pitch in ((0, 75), (1, 76), (1, 81), (2, 128), (3, 77)):
+        big = _bf16(_rand((5, 256), offset)).reshape(-1).cuda()
+        a = big[offset:offset + 4 * pitch + k].as_strided((5, k), (pitch, 1))
+        wide = torch.full((9, n + 5), 7.0, dtype=torch.bfloat16, device="cuda")
+        ops.bfp_matvec(a, img, n, ops.DF.Bfp8_b, out=wide[2:7, 3:3 + n])
+        _check_sum(wide[2:7, 3:3 + n], a.double().cpu().numpy(), w, torch.bfloat16)
+        wide[2:7, 3:3 + n] = 7.0
+        assert torch.all(wide == 7.0)       # rows behind the last one and columns beside them keep what they held
+    same = a[:1].expand(6, k)               # a row stride of zero
+    got = ops.bfp_matvec(same, img, n, ops.DF.Bfp8_b)
+    assert torch.equal(got, got[:1].expand_as(got))
+    assert ops.bfp_matvec(a[:0], img, n, ops.DF.Bfp8_b).shape == (0, n)
+
+
+def test_matvec_rows_do_not_depend_on_their_company(ops, oracle):
+    k, n = 512, 256
+    img, _ = _store(oracle, _rand((k, n), 9, 0.1), "Bfp4_b")
+    a = _bf16(_rand((8, k), 2)).cuda()
+    all8 = ops.bfp_matvec(a, img, n, ops.DF.Bfp4_b, out_dtype=torch.float32)
+    for i in (0, 5):
+        assert torch.equal(all8[i], ops.bfp_matvec(a[i:i + 1], img, n, ops.DF.Bfp4_b, out_dtype=torch.float32)[0])
+    for _ in range(20):
+        assert torch.equal(all8, ops.bfp_matvec(a, img, n, ops.DF.Bfp4_b, out_dtype=torch.float32))
+
+
+# ------------------------------------------------------------------------------------------------ router
+def _route_ref(x, w, top, renorm):
+    l = x.double().numpy() @ w.double().numpy().T
+    ids = np.argsort(-l, axis=1, kind="stable")[:, :top]
+    p = np.exp(l - l.max(1, keepdims=True))
+    c = np.take_along_axis(p, ids, 1)
+    return c / (c.sum(1, keepdims=True) if renorm else p.sum(1, keepdims=True)), ids
+
+
+@pytest.mark.parametrize("router", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t,h,e,top", [(1, 1, 1, 1), (1, 8, 2, 2), (2, 33, 5, 3), (3, 1024, 8, 2), (17, 100, 7, 7), (19, 257, 64, 8), (37, 512, 65, 16),
+                                       (64, 96, 256, 16), (40, 2048, 128, 1)])
+def test_route_shapes(ops, router, t, h, e, top):
+    g = torch.Generator().manual_seed(t + h + e)
+    x, w = torch.randn(t, h, generator=g).bfloat16(), (torch.randn(e, h, generator=g) * 2 * h ** -0.5).to(router)
+    for renorm in (True, False):
+        weights, ids = ops.moe_route(x.cuda(), w.cuda(), top, renorm)
+        ref, rid = _route_ref(x, w, top, renorm)
+        assert ids.dtype == torch.int32 and np.array_equal(ids.cpu().numpy(), rid)
+        # scores below 16 in magnitude, exponentials and the sum in binary32: a few units of 2^-24 each, h / 8 group sums exact to 2^-24
+        assert np.abs(weights.double().cpu().numpy() - ref).max() <= 2.0 ** -18 * ref.max()
+
+
+def test_route_ties_go_to_the_lowest_index(ops):
+    x = torch.ones(3, 64).bfloat16().cuda()
+    w = torch.zeros(40, 64, device="cuda")
+    w[[7, 9, 33], 0] = 2.0
+    w[3, 0] = -0.0
+    weights, ids = ops.moe_route(x, w, 6, True)
+    assert ids.cpu().tolist() == [[7, 9, 33, 0, 1, 2]] * 3
+    w.zero_()
+    weights, ids = ops.moe_route(x, w, 5, False)
+    assert ids.cpu().tolist() == [[0, 1, 2, 3, 4]] * 3
+    assert torch.equal(weights.cpu(), torch.full((3, 5), 1 / 40))
+
+
+def test_route_scores_that_are_not_numbers(ops):
+    x = torch.ones(2, 16).bfloat16().cuda()
+    w = torch.arange(6, device="cuda").float().view(6, 1).expand(6, 16).contiguous()
+    w[4, 3] = float("nan")
+    w[5, 3] = -float("inf")
+    weights, ids = ops.moe_route(x, w, 6, True)
+    assert ids.cpu().tolist() == [[3, 2, 1, 0, 5, 4]] * 2       # a NaN score behind every number
+    assert torch.isnan(weights).all()
+    weights, ids = ops.moe_route(x, w, 4, True)
+    assert ids.cpu().tolist() == [[3, 2, 1, 0]] * 2 and torch.allclose(weights.sum(1), torch.ones(2, device="cuda"))
+    w[:] = float("nan")
+    _, ids = ops.moe_route(x, w, 3, False)
+    assert ids.cpu().tolist() == [[0, 1, 2]] * 2                # distinct experts whatever the scores are
+
+
+def test_route_strides_and_alignment(ops):
+    g = torch.Generator().manual_seed(4)
+    buf, wbuf = torch.randn(4000, generator=g).bfloat16().cuda(), torch.randn(9000, generator=g).cuda()
+    for off, h, pitch in ((1, 120, 128), (0, 121, 121), (8, 64, 72), (3, 99, 130)):
+        x = buf[off:].as_strided((6, h), (pitch, 1), off)
+        w = wbuf.as_strided((24, h), (pitch + 4, 1), off)
+        _, ids = ops.moe_route(x, w, 4, True)
+        assert np.array_equal(ids.cpu().numpy(), _route_ref(x.cpu(), w.cpu(), 4, True)[1])
+
+
+# ------------------------------------------------------------------------------------------------ experts
+def _make_experts(oracle, e, h, i, df, seed, gated=True):
+    out = []
+    for which, (r, c) in enumerate(((h, i), (h, i), (i, h))):
+        if which == 1 and not gated:
+            out.append((None, None))
+            continue
+        pairs = [_store(oracle, _rand((r, c), seed + 10 * which + 100 * k, r ** -0.5), df) for k in range(e)]
+        out.append((torch.stack([p[0] for p in pairs]), np.stack([p[1] for p in pairs])))
+    return [o[0] for o in out], [o[1] for o in out]
+
+
+def _experts_ref(x, weights, ids, vals, act):
+    """(reference, tolerance) in float64."""
+    gate, up, down = vals
+    x, weights, ids = x.double().numpy(), weights.double().cpu().numpy(), ids.cpu().numpy()
+    y, tol = np.zeros(x.shape), np.zeros(x.shape)
+    erf = lambda v: torch.erf(torch.from_numpy(v)).numpy()
+    h_n, i_n = gate.shape[1], gate.shape[2]
+    for t in range(x.shape[0]):
+        for s in range(ids.shape[1]):
+            e = ids[t, s]
+            if e < 0 or e >= gate.shape[0]:
+                continue
+            w = weights[t, s]
+            gt, dg = x[t] @ gate[e], (h_n + 16) * 2.0 ** -23 * (np.abs(x[t]) @ np.abs(gate[e]))
+            a = gt / (1 + np.exp(-gt)) if act == "silu" else 0.5 * gt * (1 + erf(gt / np.sqrt(2)))
+            da = 1.13 * dg + 2.0 ** -19 * np.abs(a) + 2.0 ** -100
+            u, du = (1.0, 0.0) if up is None else (x[t] @ up[e], (h_n + 16) * 2.0 ** -23 * (np.abs(x[t]) @ np.abs(up[e])))
+            h = a * u
+            dh = da * (np.abs(u) + du) + np.abs(a) * du
+            dh += 2.0 ** -16 * (np.abs(h) + dh)
+            y[t] += w * (h @ down[e])
+            tol[t] += abs(w) * ((dh + (2 * i_n * ids.shape[1] + 16) * 2.0 ** -23 * (np.abs(h) + dh)) @ np.abs(down[e]))
+    return y, tol + 2.0 ** -8 * (np.abs(y) + tol)
+
+
+def _check_experts(got, x, weights, ids, vals, act):
+    ref, tol = _experts_ref(x, weights, ids, vals, act)
+    err = np.abs(got.double().cpu().numpy() - ref)
+    assert (err <= tol).all(), f"worst {np.max(err / np.maximum(tol, 1e-300))} of the tolerance"
+
+
+def _routing(t, e, top, seed, drop=0.0):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.rand(t, e, generator=g).argsort(1)[:, :top].int()
+    weights = torch.rand(t, top, generator=g)
+    if drop:
+        ids[torch.rand(t, top, generator=g) < drop] = -1
+    return weights, ids
+
+
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("t,h,i,e,top,act,gated", [(1, 32, 32, 1, 1, "silu", True), (1, 64, 96, 4, 2, "gelu", True), (3, 100, 50, 5, 3, "silu", True),
+                                                  (8, 128, 160, 3, 2, "gelu", False), (9, 96, 64, 6, 2, "silu", True), (20, 70, 33, 2, 1, "gelu", True),
+                                                  (40, 64, 40, 3, 3, "silu", False), (64, 33, 65, 20, 4, "gelu", True), (2, 300, 700, 2, 2, "silu", True)])
+def test_experts_shapes(ops, oracle, df, t, h, i, e, top, act, gated):
+    images, vals = _make_experts(oracle, e, h, i, df, t + h, gated)
+    x = _bf16(_rand((t, h), 7))
+    weights, ids = _routing(t, e, top, t, drop=0.2 if top > 2 else 0.0)
+    got = ops.moe_experts(x.cuda(), weights.cuda(), ids.cuda(), *images, i, getattr(ops.DF, df), act)
+    assert got.dtype == torch.bfloat16 and got.shape == (t, h)
+    _check_experts(got, x, weights, ids, vals, act)
+    rc, st = ops._cabi.device_status()
+    assert rc == 0 and st == 0
+
+
+def test_experts_dropped_repeated_and_foreign_slots(ops, oracle):
+    e, h, i, t = 5, 96, 80, 6
+    images, vals = _make_experts(oracle, e, h, i, "Bfp4_b", 11)
+    x = _bf16(_rand((t, h), 12))
+    weights = torch.rand(t, 4, generator=torch.Generator().manual_seed(5))
+    ids = torch.tensor([[0, 1, 2, 3], [4, 4, 4, 4], [-1, -1, -1, -1], [2, -1, 2, 0], [5, 1000000, -7, 3], [1, 1, -1, 0]], dtype=torch.int32)
+    got = ops.moe_experts(x.cuda(), weights.cuda(), ids.cuda(), *images, i)
+    _check_experts(got, x, weights, ids, vals, "silu")
+    assert torch.all(got[2] == 0)
+    none = ops.moe_experts(x.cuda(), weights.cuda(), torch.full_like(ids, -1).cuda(), *images, i)
+    assert torch.all(none == 0)
+
+
+def test_experts_many_experts_one_token_each(ops, oracle):
+    e, h, i, t = 256, 32, 32, 64
+    images, vals = _make_experts(oracle, e, h, i, "Bfp2_b", 13)
+    x = _bf16(_rand((t, h), 14))
+    ids = torch.arange(256, dtype=torch.int32).view(64, 4).flip(0).contiguous()
+    weights = torch.rand(t, 4, generator=torch.Generator().manual_seed(6))
+    got = ops.moe_experts(x.cuda(), weights.cuda(), ids.cuda(), *images, i, ops.DF.Bfp2_b)
+    _check_experts(got, x, weights, ids, vals, "silu")
+    one = torch.full((t, 1), 255, dtype=torch.int32)            # all tokens to the last expert
+    got = ops.moe_experts(x.cuda(), weights[:, :1].contiguous().cuda(), one.cuda(), *images, i, ops.DF.Bfp2_b, "gelu")
+    _check_experts(got, x, weights[:, :1], one, vals, "gelu")
+
+
+def test_experts_strides_neighbours_and_in_place(ops, oracle):
+    e, h, i, t = 3, 70, 40, 5
+    images, vals = _make_experts(oracle, e, h, i, "Bfp8_b", 15)
+    big = _bf16(_rand((8, 91), 16)).cuda()
+    x = big[1:6, 3:3 + h]
+    weights, ids = _routing(t, e, 2, 3)
+    wide = torch.full((7, 90), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.moe_experts(x, weights.cuda(), ids.cuda(), *images, i, ops.DF.Bfp8_b, out=wide[1:6, 5:5 + h])
+    _check_experts(wide[1:6, 5:5 + h], x.cpu(), weights, ids, vals, "silu")
+    want = wide[1:6, 5:5 + h].clone()
+    wide[1:6, 5:5 + h] = 7.0
+    assert torch.all(wide == 7.0)
+    before = big.clone()
+    ops.moe_experts(x, weights.cuda(), ids.cuda(), *images, i, ops.DF.Bfp8_b, out=x)
+    assert torch.equal(x, want)
+    big[1:6, 3:3 + h] = before[1:6, 3:3 + h]
+    assert torch.equal(big, before)
+
+
+# ------------------------------------------------------------------------------------------------ the layer, and the operators together
+@pytest.mark.parametrize("t,h,i,e,top,df,router", [(1, 64, 96, 8, 2, "Bfp4_b", torch.float32), (7, 100, 40, 12, 3, "Bfp8_b", torch.bfloat16),
+                                                   (33, 64, 64, 40, 4, "Bfp2_b", torch.float32)])
+def test_layer_is_route_then_experts(ops, oracle, t, h, i, e, top, df, router):
+    images, vals = _make_experts(oracle, e, h, i, df, 17)
+    g = torch.Generator().manual_seed(18)
+    x, wr = torch.randn(t, h, generator=g).bfloat16(), (torch.randn(e, h, generator=g) * 2 * h ** -0.5).to(router)
+    for renorm in (True, False):
+        weights, ids = ops.moe_route(x.cuda(), wr.cuda(), top, renorm)
+        two = ops.moe_experts(x.cuda(), weights, ids, *images, i, getattr(ops.DF, df), "gelu")
+        for _ in range(5):
+            assert torch.equal(two, ops.moe_layer(x.cuda(), wr.cuda(), top, *images, i, getattr(ops.DF, df), "gelu", renorm))
+        rw, rid = _route_ref(x, wr, top, renorm)
+        _check_experts(two, x, torch.from_numpy(rw), torch.from_numpy(rid), vals, "gelu")
+
+
+def _block(ops, x, proj, wr, images, i):
+    """A decoding step's use: a projection, the layer on its result, a projection of the sum back to binary32."""
+    a = ops.bfp_matvec(x, proj, x.shape[1], ops.DF.Bfp4_b)
+    y = ops.moe_layer(a, wr, 2, *images, i)
+    return ops.bfp_matvec(a + y, proj, x.shape[1], ops.DF.Bfp4_b, out_dtype=torch.float32), y
+
+
+def test_operators_together_eager_captured_and_on_side_streams(ops, oracle):
+    h, i, e = 128, 96, 8
+    images, _ = _make_experts(oracle, e, h, i, "Bfp4_b", 19)
+    proj, pv = _store(oracle, _rand((h, h), 20, h ** -0.5), "Bfp4_b")
+    wr = torch.randn(e, h, generator=torch.Generator().manual_seed(21)).cuda() * 0.2
+    xs = [_bf16(_rand((3, h), 30 + k)).cuda() for k in range(6)]
+    want = [_block(ops, x, proj, wr, images, i) for x in xs]
+    a = ops.bfp_matvec(xs[0], proj, h, ops.DF.Bfp4_b)
+    _check_sum(a, xs[0].double().cpu().numpy(), pv, torch.bfloat16)
+    # two graphs, replayed at the same time on two streams
+    graphs, bufs, outs, streams = [], [], [], [torch.cuda.Stream() for _ in range(2)]
+    for k in range(2):
+        buf = xs[k].clone()
+        gr = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(gr):
+            out = _block(ops, buf, proj, wr, images, i)
+        graphs.append(gr), bufs.append(buf), outs.append(out)
+    for r in range(3):
+        for k in range(2):
+            bufs[k].copy_(xs[2 * r + k])
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for k in range(2):
+                with torch.cuda.stream(streams[k]):
+                    graphs[k].replay()
+        torch.cuda.synchronize()
+        for k in range(2):
+            assert torch.equal(outs[k][0], want[2 * r + k][0]) and torch.equal(outs[k][1], want[2 * r + k][1])
+    # eager calls on two streams at once
+    got = [[], []]
+    for r in range(20):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(_block(ops, xs[k], proj, wr, images, i))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(o[0], want[k][0]) and torch.equal(o[1], want[k][1]) for o in got[k])
+    rc, st = ops._cabi.device_status()
+    assert rc == 0 and st == 0
+
+
+def test_images_from_the_pack_of_a_stacked_tensor(ops, oracle):
+    """The documented way to the images: tilize_pack of [1,E,H,I], one row of bytes for each expert."""
+    e, h, i = 3, 64, 96
+    w = _rand((1, e, h, i), 22, 0.1)
+    img = ops.tilize_pack(torch.from_numpy(w).cuda(), ops.DF.Bfp4_b).view(e, -1)
+    for k in range(e):
+        assert torch.equal(img[k], _store(oracle, w[0, k], "Bfp4_b")[0])
+
+
+def test_image_past_4_gib(ops):
+    """Records whose offsets pass 32 bits: 512 experts' worth of bytes in a 256-expert set, only the ends filled."""
+    e, h, i = 256, 4096, 4096
+    per = (h // 32) * (i // 32) * 1088
+    images = torch.zeros(e, per, dtype=torch.uint8, device="cuda")
+    assert images.numel() > 1 << 32
+    g = torch.Generator().manual_seed(23)
+    x = torch.randn(2, h, generator=g).bfloat16().cuda()
+    small = torch.randn(1, 1, h, i, generator=g) * h ** -0.5
+    img = ops.tilize_pack(small.cuda(), ops.DF.Bfp8_b)
+    images[255] = img
+    images[3] = img
+    weights = torch.ones(2, 1, device="cuda")
+    last = ops.moe_experts(x, weights, torch.tensor([[255], [255]], dtype=torch.int32, device="cuda"), images, images, images, i, ops.DF.Bfp8_b)
+    low = ops.moe_experts(x, weights, torch.tensor([[3], [3]], dtype=torch.int32, device="cuda"), images, images, images, i, ops.DF.Bfp8_b)
+    assert torch.equal(last, low) and last.float().abs().max() > 0.01

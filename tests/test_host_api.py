@@ -337,3 +337,28 @@ def test_cpp_twins_of_the_torch_device_descriptor_helpers():
         B.to_pytorch_tensor_desc(t.data_ptr(), 4, DF.Float32, [1, 2, 3, 4, 5], [1, 1, 1, 1, 1])
     with pytest.raises(ValueError):
         B.buda_padded_shape([1, 2, 3, 4, 5])
+
+
+def test_few_row_operators_refuse_bad_arguments():
+    """Refusals that need no device: the Python checks, and the C checks that run before any launch."""
+    import ctypes
+
+    import torch
+    from pybuda import _cabi, cuda_ops as ops
+
+    x, img = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(4 * 576, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.bfp_matvec(x, img, 64)
+    with pytest.raises(RuntimeError, match="bfloat16 matrix"):
+        ops.bfp_matvec(x.float(), img, 64)
+    with pytest.raises(RuntimeError, match="bfloat16 matrix"):
+        ops.bfp_matvec(x.t(), img, 64)
+    with pytest.raises(RuntimeError, match="Bfp8_b, Bfp4_b or Bfp2_b"):
+        ops.bfp_matvec(x, img, 64, ops.DF.Float16_b)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.moe_route(x, torch.zeros(4, 64), 2)
+    with pytest.raises(RuntimeError, match="activation"):
+        ops.moe_experts(x, torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int32), img.view(1, -1), None, img.view(1, -1), 64, activation="relu")
+    assert _cabi.lib.buda_moe_workspace_bytes(3, 2, 33) == 3 * 2 * 2 * 64 * 2
+    for bad in ((65, 2, 32), (-1, 2, 32), (1, 0, 32), (1, 17, 32), (1, 1, 0), (1, 1, 1 << 25)):
+        assert _cabi.lib.buda_moe_workspace_bytes(*bad) == -1, bad

@@ -1,0 +1,624 @@
+// K9: products of a few rows (tokens) with block-float weights, for serving.
+//
+//   matvec      Y[m, n]  = sum_k A[m, k] W[k, n]
+//   experts     h[s, i]  = w_s act((x_t G_e)[i]) (x_t U_e)[i]            (launch 1, "in")
+//               y[t, n]  = sum over the slots s of token t of sum_i h[s, i] D_e[i, n]   (launch 2, "out")
+//
+// W, G, U, D are queue images in the default byte layout: tile records of 64 shared exponents and four 16x16 faces, a
+// stored datum of m magnitude bits standing for (-1)^s q 2^(E - 126 - m).
+//
+// Bound: bytes of the images (1.0625 / 0.5625 / 0.3125 a weight) -- every weight meets only a few rows.  What decides is
+// how many copies are in flight and how few instructions decode a weight:
+//   * A warp owns 128 output columns (4 tile columns) and walks tile rows.  One bulk copy brings the 4 adjacent records
+//     of a tile row into the warp's own ring in shared memory; no warp waits for another until the sums are joined.
+//   * Decode: a datum's sign and magnitude bits are moved to bit 15 and to the top of the 7 mantissa bits of a
+//     bfloat16, which makes the subnormal number (-1)^s q 2^(-126 - m); a packed multiply by 2^E finishes it, exactly.
+//     One byte permute puts the same byte of two weight rows into both halves of a register in both places, so a pair
+//     costs one AND (plus a shift for all but one datum of a byte) and the multiply.
+//   * The products go through mma.sync m16n8k16 with the WEIGHTS as the 16-row operand and the tokens as the 8 columns:
+//     a lane's fragment is two weight columns at four weight rows, which is what its 64-bit piece of a face holds, so
+//     decoded weights never leave the registers.  (tcgen05 reads its operands from shared or tensor memory: the decoded
+//     weights would be written and read once more there for a product whose tensor work is a few per cent of its time.)
+//   * The tile rows are split over the 8 warps of a CTA and over a cluster of up to 8 CTAs; sums are joined through
+//     shared and distributed shared memory in a fixed order: no workspace, no atomics, the same bits every time.
+// Sums are held in binary32 throughout.  h is carried between the two launches as two bfloat16 pieces (the rounded value and
+// the rounded rest, together within 2^-16 of h), so nothing is lost against a binary32 h at twice the tensor work.
+#include <cuda_bf16.h>
+#include <cstdio>
+
+#include "few_rows.cuh"
+
+namespace buda {
+namespace few {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kGroupTiles = 4;          // tile columns of one warp
+constexpr int kPitch = 132;             // floats per token of a warp's sums: 8-byte stores of 4 x 4 lanes meet no bank twice
+
+enum { kMatvec = 0, kExpertsIn = 1, kExpertsOut = 2 };
+
+template <int MB>
+struct Fmt {
+    static constexpr int kRow = 2 * (MB + 1);               // bytes of one face row
+    static constexpr int kFace = 16 * kRow;
+    static constexpr int kRec = 64 + 4 * kFace;
+    static constexpr int kStage = kGroupTiles * kRec;
+    static constexpr int kStages = MB == 7 ? 3 : MB == 3 ? 5 : 8;
+};
+
+struct Args {
+    const __nv_bfloat16 *x;      // [rows, K], row stride ldx; experts-out: h
+    int64_t ldx;
+    int rows, K, Kt, N, Nt;
+    const uint8_t *w0, *w1;      // w1: the up matrix of gated experts
+    void *out;
+    int64_t ldo;
+    int out_f32;
+    const int *ids;
+    const float *wts;
+    int top, E, act;
+    __nv_bfloat16 *h;            // [rows * top][2][32 * tile rows of the down matrix]
+    int hpad;
+    int cluster;
+    unsigned int *status;
+};
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b)
+{
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr)
+{
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+// The raw data of one lane: face rows 2t, 2t+1 (p = 0) and 2t+8, 2t+9 (p = 1) of one face.
+template <int MB>
+struct Raw {
+    uint32_t w[2][2][(MB + 1) / 2];   // [p][row][32-bit word]
+};
+
+// 8-bit data: the two 16-byte rows are fetched in opposite order by the lanes of odd g, which keeps the 8 lanes of a
+// 128-bit access in distinct banks; the byte permutes undo it.
+template <int MB>
+__device__ __forceinline__ void load_raw(Raw<MB> &r, const uint8_t *face, int t, int odd)
+{
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+        const uint8_t *at = face + (2 * t + 8 * p) * Fmt<MB>::kRow;
+        if constexpr (MB == 7) {
+            const uint4 a = *reinterpret_cast<const uint4 *>(at + 16 * odd), b = *reinterpret_cast<const uint4 *>(at + 16 * (odd ^ 1));
+            r.w[p][0][0] = a.x; r.w[p][0][1] = a.y; r.w[p][0][2] = a.z; r.w[p][0][3] = a.w;
+            r.w[p][1][0] = b.x; r.w[p][1][1] = b.y; r.w[p][1][2] = b.z; r.w[p][1][3] = b.w;
+        } else if constexpr (MB == 3) {
+            const uint4 a = *reinterpret_cast<const uint4 *>(at);
+            r.w[p][0][0] = a.x; r.w[p][0][1] = a.y;
+            r.w[p][1][0] = a.z; r.w[p][1][1] = a.w;
+        } else {
+            const uint2 a = *reinterpret_cast<const uint2 *>(at);
+            r.w[p][0][0] = a.x;
+            r.w[p][1][0] = a.y;
+        }
+    }
+}
+
+// Weight columns 2j and 2j+1 of the pair of rows p as subnormal bfloat16 pairs (low half: the even row).
+template <int MB>
+__device__ __forceinline__ void pair_of(const Raw<MB> &r, int p, int j, uint32_t sel_flip, uint32_t &even, uint32_t &odd)
+{
+    constexpr uint32_t keep = 0x80008000u | (((0x7fu << (7 - MB)) & 0x7fu) * 0x00010001u);
+    if constexpr (MB == 7) {
+        const int w = j >> 1, b = (j & 1) * 2;
+        even = __byte_perm(r.w[p][0][w], r.w[p][1][w], (0x4400u + 0x1111u * b) ^ sel_flip) & keep;
+        odd = __byte_perm(r.w[p][0][w], r.w[p][1][w], (0x4400u + 0x1111u * (b + 1)) ^ sel_flip) & keep;
+    } else if constexpr (MB == 3) {
+        const uint32_t d = __byte_perm(r.w[p][0][j >> 2], r.w[p][1][j >> 2], 0x4400u + 0x1111u * (j & 3));
+        even = (d << 4) & keep;
+        odd = d & keep;
+    } else {
+        const uint32_t d = __byte_perm(r.w[p][0][0], r.w[p][1][0], 0x4400u + 0x1111u * (j >> 1));
+        even = (j & 1) ? (d << 2) & keep : (d << 6) & keep;
+        odd = (j & 1) ? d & keep : (d << 4) & keep;
+    }
+}
+
+// 2^a and 2^b (0 <= a, b <= 127) as a bfloat16 pair
+__device__ __forceinline__ uint32_t pow2_pair(uint32_t a, uint32_t b) { return ((a + 127u) << 7) | ((b + 127u) << 23); }
+
+// One 16-row step: BIG where a shared exponent is above 127 (2^E is no bfloat16 then: up to three factors).
+template <int MB, int NT, int PIECES, bool BIG>
+__device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw, const uint32_t (&e)[2], uint32_t sel_flip,
+                                     const uint32_t (&x)[PIECES][NT][2])
+{
+    uint32_t s[2], s2[2], s3[2];
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+        const uint32_t a = e[p] & 0xffu, b = e[p] >> 8;
+        if constexpr (BIG) {
+            s[p] = pow2_pair(min(a, 127u), min(b, 127u));
+            s2[p] = pow2_pair(min(max(a, 127u) - 127u, 127u), min(max(b, 127u) - 127u, 127u));
+            s3[p] = pow2_pair(max(a, 254u) - 254u, max(b, 254u) - 254u);
+        } else {
+            s[p] = pow2_pair(a, b);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        uint32_t a[4];
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            pair_of<MB>(raw, p, j, sel_flip, a[2 * p], a[2 * p + 1]);
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                uint32_t v = mul_bf16x2(a[2 * p + c], s[p]);
+                if constexpr (BIG) v = mul_bf16x2(mul_bf16x2(v, s2[p]), s3[p]);
+                a[2 * p + c] = v;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < PIECES; q++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) mma16816(acc[j][nt], a, x[q][nt][0], x[q][nt][1]);
+    }
+}
+
+// Elements k, k+1 of a row (k even), zero past K.
+__device__ __forceinline__ uint32_t load_pair(const __nv_bfloat16 *row, int k, int K, bool vec)
+{
+    if (row == nullptr || k >= K) return 0u;
+    if (vec && k + 1 < K) return *reinterpret_cast<const uint32_t *>(row + k);
+    const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
+    return (uint32_t)p[k] | (k + 1 < K ? (uint32_t)p[k + 1] << 16 : 0u);
+}
+
+__device__ __forceinline__ float activate(float v, int act)
+{
+    if (act == BUDA_ACT_SILU) return v / (1.0f + expf(-v));
+    return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+}
+
+// Shared memory: [ring of every warp | the warps' sums, over the ring][the CTA's sums][barriers][tables]
+template <int MB, int NT>
+struct Lay {
+    static constexpr int kTok = 8 * NT;
+    static constexpr int kRing = kWarps * Fmt<MB>::kStages * Fmt<MB>::kStage;
+    static constexpr int kSums = kWarps * kTok * kPitch * 4;
+    static constexpr int kFirst = kRing > kSums ? kRing : kSums;
+    static constexpr int kPart = kFirst;                                  // [kTok][128] floats
+    static constexpr int kBars = kPart + kTok * 128 * 4;
+    static constexpr int kTables = kBars + kWarps * Fmt<MB>::kStages * 8;
+    static constexpr int kMap = kTables;                                  // 8 words: bit e set where expert e has a token
+    static constexpr int kCtl = kMap + kMaxExperts / 8;                   // 4 words
+    static constexpr int kList = kCtl + 16;                               // in: tokens (row, slot, weight); out: experts
+    static constexpr int kRows = kList + 4 * kMaxExperts;                 // out: slot of (expert, token)
+    static constexpr int kBytesIn = kRows;
+    static constexpr int kBytesOut = kRows + 2 * kMaxExperts * kTok;
+};
+
+template <int MB, int NT, int MODE>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) few_rows_kernel(const Args A)
+{
+    using F = Fmt<MB>;
+    using L = Lay<MB, NT>;
+    constexpr int S = F::kStages;
+    constexpr int PIECES = MODE == kExpertsOut ? 2 : 1;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int c = A.cluster;
+    const int rank = c > 1 ? (int)cluster_rank() : 0;
+    const int group = blockIdx.x / c;
+    uint8_t *ring = smem + warp * S * F::kStage;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars) + warp * S;
+    uint32_t *map = reinterpret_cast<uint32_t *>(smem + L::kMap);
+    volatile int *ctl = reinterpret_cast<volatile int *>(smem + L::kCtl);   // [0] abort flag, [1] count
+    int *list = reinterpret_cast<int *>(smem + L::kList);
+    int16_t *rows = reinterpret_cast<int16_t *>(smem + L::kRows);
+
+    if (lane == 0) {
+        for (int i = 0; i < S; i++) mbar_init(bars + i, 1);
+        mbar_fence_init();
+    }
+    if (tid == 0) ctl[0] = 0;
+    if (MODE != kMatvec && tid < kMaxExperts / 32) map[tid] = 0;
+
+    // ---- which tokens and which matrices
+    int n_tok = 0, units = A.Kt, tok0 = 0;
+    int64_t w_off = 0;
+    const int64_t image = (int64_t)A.Kt * A.Nt * F::kRec;
+    if (MODE == kMatvec) {
+        __syncthreads();
+        tok0 = blockIdx.y * L::kTok;
+        n_tok = min(A.rows - tok0, L::kTok);
+    } else {
+        if (MODE == kExpertsIn) griddep_wait();
+        __syncthreads();
+        tok0 = MODE == kExpertsOut ? blockIdx.y * L::kTok : 0;
+        const int t_end = MODE == kExpertsOut ? min(A.rows, tok0 + L::kTok) : A.rows;
+        for (int i = tok0 * A.top + tid; i < t_end * A.top; i += kThreads) {
+            const int e = __ldcg(A.ids + i);
+            if (e >= 0 && e < A.E) atomicOr(&map[e >> 5], 1u << (e & 31));
+        }
+        __syncthreads();
+        int count = 0;
+        for (int w = 0; w < kMaxExperts / 32; w++) count += __popc(map[w]);
+        if (MODE == kExpertsIn) {
+            griddep_launch();
+            if ((int)blockIdx.y >= count) return;      // the whole cluster: it shares blockIdx.y
+            int e = 0, left = blockIdx.y;
+            for (int w = 0; w < kMaxExperts / 32; w++) {
+                const int here = __popc(map[w]);
+                if (left >= 0 && left < here) e = 32 * w + (int)__fns(map[w], 0, left + 1);
+                left -= here;
+            }
+            w_off = e * image;
+            if (warp == 0) {                           // the tokens of this expert, in order; a repeated slot adds its weight
+                int found = 0;
+                for (int base = 0; base < A.rows; base += 32) {
+                    const int tk = base + lane;
+                    int first = -1;
+                    float w = 0.0f;
+                    if (tk < A.rows)
+                        for (int s = 0; s < A.top; s++)
+                            if (__ldcg(A.ids + tk * A.top + s) == e) {
+                                w += __ldcg(A.wts + tk * A.top + s);
+                                if (first < 0) first = s;
+                            }
+                    const uint32_t m = __ballot_sync(0xffffffffu, first >= 0);
+                    if (first >= 0) {
+                        const int at = found + __popc(m & ((1u << lane) - 1u));
+                        list[2 * at] = tk * A.top + first;
+                        list[2 * at + 1] = __float_as_int(w);
+                    }
+                    found += __popc(m);
+                }
+                if (lane == 0) ctl[1] = found;
+            }
+            __syncthreads();
+            tok0 = blockIdx.z * L::kTok;
+            n_tok = min(ctl[1] - tok0, L::kTok);
+            if (n_tok <= 0) return;                    // the whole cluster here too
+        } else {
+            n_tok = t_end - tok0;
+            if (tid < kMaxExperts) {                   // expert e is number (set bits below e)
+                if (map[tid >> 5] >> (tid & 31) & 1u) {
+                    int at = __popc(map[tid >> 5] & ((1u << (tid & 31)) - 1u));
+                    for (int w = 0; w < (tid >> 5); w++) at += __popc(map[w]);
+                    list[at] = tid;
+                }
+            }
+            for (int i = tid; i < count * L::kTok; i += kThreads) rows[i] = -1;
+            __syncthreads();
+            if (tid < n_tok)
+                for (int s = A.top - 1; s >= 0; s--) {
+                    const int e = __ldcg(A.ids + (tok0 + tid) * A.top + s);
+                    if (e < 0 || e >= A.E) continue;
+                    int at = __popc(map[e >> 5] & ((1u << (e & 31)) - 1u));
+                    for (int w = 0; w < (e >> 5); w++) at += __popc(map[w]);
+                    rows[at * L::kTok + tid] = (int16_t)((tok0 + tid) * A.top + s);
+                }
+            __syncthreads();
+            units = count * A.Kt;
+        }
+    }
+
+    // ---- this warp's share of the tile rows, and the copies of one of them
+    const int workers = c * kWarps, me = rank * kWarps + warp;
+    const int u0 = (int)((int64_t)units * me / workers), n = (int)((int64_t)units * (me + 1) / workers) - u0;
+    const bool gated = MODE == kExpertsIn && A.w1 != nullptr;
+    const int span = gated ? kGroupTiles / 2 : kGroupTiles;
+    const int nt0 = group * span;
+    const uint32_t bytes = (uint32_t)min(span, A.Nt - nt0) * F::kRec;
+    auto issue = [&](int i) {
+        const int u = u0 + i;
+        int kt = u;
+        int64_t off = w_off;
+        if (MODE == kExpertsOut) {
+            const int s = u / A.Kt;
+            kt = u - s * A.Kt;
+            off = list[s] * image;
+        }
+        off += ((int64_t)kt * A.Nt + nt0) * F::kRec;
+        uint8_t *dst = ring + (i % S) * F::kStage;
+        uint64_t *bar = bars + i % S;
+        mbar_arrive_expect_tx(bar, gated ? 2 * bytes : bytes);
+        bulk_g2s(dst, A.w0 + off, bytes, bar);
+        if (gated) bulk_g2s(dst + F::kStage / 2, A.w1 + off, bytes, bar);
+    };
+    __syncwarp();
+    if (lane == 0)
+        for (int i = 0; i < min(S, n); i++) issue(i);
+    if (MODE == kExpertsOut) griddep_wait();           // h is complete; the weights were asked for before it was
+
+    // ---- the tokens' values of one tile row: lane (g, t) holds token g, k = 2t, 2t+1, 2t+8, 2t+9 of both face rows
+    const __nv_bfloat16 *xrow[NT];
+    bool vec = true;
+    auto row_of = [&](int nt, int u) -> const __nv_bfloat16 * {
+        const int tk = nt * 8 + g;
+        if (tk >= n_tok) return nullptr;
+        if (MODE == kMatvec) return A.x + (int64_t)(tok0 + tk) * A.ldx;
+        if (MODE == kExpertsIn) return A.x + (int64_t)(list[2 * (tok0 + tk)] / A.top) * A.ldx;
+        const int r = rows[(u / A.Kt) * L::kTok + tk];
+        return r < 0 ? nullptr : A.h + (int64_t)r * 2 * A.hpad;
+    };
+    if (MODE != kExpertsOut) {
+        vec = ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 3) == 0;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) xrow[nt] = row_of(nt, 0);
+    }
+    uint32_t xb[2][PIECES][NT][2], ahead[2][PIECES][NT][2];   // this tile row's, and the next one's on their way
+    auto load_x = [&](uint32_t (&xb)[2][PIECES][NT][2], int i) {
+        const int u = u0 + i;
+        const int kt = MODE == kExpertsOut ? u % A.Kt : u;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            if (MODE == kExpertsOut) xrow[nt] = row_of(nt, u);
+#pragma unroll
+            for (int q = 0; q < PIECES; q++)
+#pragma unroll
+                for (int f = 0; f < 2; f++)
+#pragma unroll
+                    for (int p = 0; p < 2; p++) {
+                        const int k = kt * 32 + f * 16 + p * 8 + 2 * t;
+                        if (MODE == kExpertsOut)
+                            xb[f][q][nt][p] = xrow[nt] ? __ldcg(reinterpret_cast<const uint32_t *>(xrow[nt] + q * A.hpad + k)) : 0u;
+                        else
+                            xb[f][q][nt][p] = load_pair(xrow[nt], k, A.K, vec);
+                    }
+        }
+    };
+
+    float acc[8][NT][4];
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) acc[j][nt][v] = 0.0f;
+
+    // lane group g reads face column (g >> 1) & 1 of tile (g & 1) + 2 * (g >> 2): neighbours in g are records apart, which
+    // puts the 8 lanes of a 128-bit access in distinct banks
+    const int tile = (g & 1) | ((g >> 2) << 1), fc = (g >> 1) & 1, odd = g & 1;
+    const uint32_t sel_flip = MB == 7 && odd ? 0x4444u : 0u;
+    bool ok = true;
+    int done = 0;
+    if (n > 0) load_x(ahead, 0);
+    for (; done < n; done++) {
+#pragma unroll
+        for (int v = 0; v < 4 * PIECES * NT; v++) (&xb[0][0][0][0])[v] = (&ahead[0][0][0][0])[v];
+        if (done + 1 < n) load_x(ahead, done + 1);
+        ok = mbar_wait_bounded(bars + done % S, (done / S) & 1, const_cast<int *>(&ctl[0]), A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint8_t *rec = ring + (done % S) * F::kStage + tile * F::kRec;
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+            const int face = 2 * f + fc;
+            Raw<MB> raw;
+            load_raw<MB>(raw, rec + 64 + face * F::kFace, t, odd);
+            uint32_t e[2];
+            e[0] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t);
+            e[1] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t + 8);
+            if (__any_sync(0xffffffffu, ((e[0] | e[1]) & 0x8080u) != 0))
+                step<MB, NT, PIECES, true>(acc, raw, e, sel_flip, xb[f]);
+            else
+                step<MB, NT, PIECES, false>(acc, raw, e, sel_flip, xb[f]);
+        }
+        __syncwarp();
+        if (lane == 0 && done + S < n) issue(done + S);
+    }
+    if (!ok)   // a copy that did not arrive in time: let those in flight land before the memory is given up (again bounded)
+        for (int i = done; i < min(n, done + S); i++) {
+            int own = 0;
+            (void)mbar_wait_bounded(bars + i % S, (i / S) & 1, &own, A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
+        }
+
+    // ---- join the warps: sums[warp][token][j][g][2]
+    __syncthreads();
+    float *sums = reinterpret_cast<float *>(smem);
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int v = 0; v < 2; v++)
+                *reinterpret_cast<float2 *>(sums + (warp * L::kTok + nt * 8 + 2 * t + v) * kPitch + j * 16 + g * 2) =
+                    make_float2(acc[j][nt][v], acc[j][nt][2 + v]);
+    __syncthreads();
+    float *part = reinterpret_cast<float *>(smem + L::kPart);
+    for (int i = tid; i < n_tok * 64; i += kThreads) {
+        const int tk = i >> 6, q = i & 63;
+        float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const float2 v = *reinterpret_cast<const float2 *>(sums + (w * L::kTok + tk) * kPitch + 2 * q);
+            s.x += v.x;
+            s.y += v.y;
+        }
+        *reinterpret_cast<float2 *>(part + tk * 128 + 2 * q) = s;
+    }
+    if (c > 1) cluster_sync(); else __syncthreads();
+
+    // ---- join the CTAs of the cluster (each finishes its share of the outputs) and write
+    auto total = [&](int tk, int q) {
+        float2 s = make_float2(0.0f, 0.0f);
+        if (c == 1) return *reinterpret_cast<const float2 *>(part + tk * 128 + 2 * q);
+        const uint32_t at = smem_u32(part + tk * 128 + 2 * q);
+        for (int r = 0; r < c; r++) {
+            const float2 v = ld_cluster_f2(map_rank(at, r));
+            s.x += v.x;
+            s.y += v.y;
+        }
+        return s;
+    };
+    const int per_tok = gated ? 32 : 64, items = n_tok * per_tok;
+    for (int i = rank * kThreads + tid; i < items; i += c * kThreads) {
+        const int tk = i / per_tok, r = i % per_tok;
+        const int j = gated ? r >> 2 : r >> 3, gg = gated ? r & 3 : r & 7, q = j * 8 + gg;
+        const int col = nt0 * 32 + ((gg & 1) | ((gg >> 2) << 1)) * 32 + ((gg >> 1) & 1) * 16 + 2 * j;
+        float2 v = total(tk, q);
+        if (MODE == kExpertsIn) {
+            float2 up = make_float2(1.0f, 1.0f);
+            if (gated) up = total(tk, q + 4);
+            const float w = __int_as_float(list[2 * (tok0 + tk) + 1]);
+            float r2[2] = {activate(v.x, A.act) * up.x * w, activate(v.y, A.act) * up.y * w};
+            __nv_bfloat16 *h = A.h + (int64_t)list[2 * (tok0 + tk)] * 2 * A.hpad;
+            if (col < A.hpad) {
+                uint32_t hi = 0, lo = 0;
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    if (col + b >= A.N) continue;      // tile padding stays zero
+                    const __nv_bfloat16 a = __float2bfloat16_rn(r2[b]);
+                    // infinities and NaN are carried by the first piece alone
+                    const float rest = r2[b] - __bfloat162float(a);
+                    const __nv_bfloat16 d = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);
+                    hi |= (uint32_t)__bfloat16_as_ushort(a) << (16 * b);
+                    lo |= (uint32_t)__bfloat16_as_ushort(d) << (16 * b);
+                }
+                *reinterpret_cast<uint32_t *>(h + col) = hi;
+                *reinterpret_cast<uint32_t *>(h + A.hpad + col) = lo;
+            }
+        } else {
+            const int64_t at = (int64_t)(tok0 + tk) * A.ldo + col;
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+                if (col + b < A.N) {
+                    const float f = b ? v.y : v.x;
+                    if (A.out_f32) reinterpret_cast<float *>(A.out)[at + b] = f;
+                    else reinterpret_cast<__nv_bfloat16 *>(A.out)[at + b] = __float2bfloat16_rn(f);
+                }
+        }
+    }
+    if (c > 1) cluster_sync();       // no CTA leaves while another reads its sums
+}
+
+template <int MB, int NT, int MODE>
+cudaError_t launch_one(const Args &a, dim3 grid, bool dependent, cudaStream_t stream)
+{
+    using L = Lay<MB, NT>;
+    const int bytes = MODE == kExpertsOut ? L::kBytesOut : L::kBytesIn;
+    cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<MB, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (a.cluster > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = a.cluster;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        n++;
+    }
+    if (dependent) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n].val.programmaticStreamSerializationAllowed = 1;
+        n++;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, few_rows_kernel<MB, NT, MODE>, a);
+}
+
+template <int MODE>
+cudaError_t dispatch(int mant_bits, int tokens, const Args &a, dim3 grid, bool dependent, cudaStream_t stream)
+{
+#define BUDA_FEW(MB)                                                                                    \
+    return tokens <= 8 ? launch_one<MB, 1, MODE>(a, grid, dependent, stream)                            \
+                       : launch_one<MB, 2, MODE>(a, grid, dependent, stream)
+    switch (mant_bits) {
+        case 7: BUDA_FEW(7);
+        case 3: BUDA_FEW(3);
+        default: BUDA_FEW(1);
+    }
+#undef BUDA_FEW
+}
+
+// How many CTAs share the tile rows of one column group: doubled while the launch does not fill the device's resident
+// CTAs and every warp keeps a tile row.
+int split_of(int64_t groups, int64_t tile_rows, int sm_count, int per_sm)
+{
+    int c = 1;
+    while (c < 8 && groups * c * 2 <= (int64_t)sm_count * per_sm && tile_rows >= (int64_t)c * 2 * kWarps) c *= 2;
+    return c;
+}
+
+int tokens_per_pass(int rows) { return rows <= 8 ? 8 : 16; }
+
+}  // namespace few
+
+using namespace few;
+
+cudaError_t launch_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, const void *W, int64_t N, int mant_bits, void *Y, int64_t ldy,
+                              int out_f32, int sm_count, cudaStream_t stream, unsigned int *status)
+{
+    Args a = {};
+    a.x = (const __nv_bfloat16 *)A; a.ldx = lda;
+    a.rows = (int)M; a.K = (int)K; a.Kt = (int)((K + 31) / 32); a.N = (int)N; a.Nt = (int)((N + 31) / 32);
+    a.w0 = (const uint8_t *)W;
+    a.out = Y; a.ldo = ldy; a.out_f32 = out_f32;
+    a.status = status;
+    const int tok = tokens_per_pass(a.rows), groups = (a.Nt + kGroupTiles - 1) / kGroupTiles, passes = (a.rows + tok - 1) / tok;
+    a.cluster = split_of((int64_t)groups * passes, a.Kt, sm_count, tok == 8 ? 2 : 1);
+    return dispatch<kMatvec>(mant_bits, a.rows, a, dim3(groups * a.cluster, passes), false, stream);
+}
+
+cudaError_t launch_moe_experts(const MoeArgs &m, bool dependent, int sm_count, cudaStream_t stream, unsigned int *status)
+{
+    const int tok = tokens_per_pass(m.T), passes = (m.T + tok - 1) / tok;
+    const int Ht = (m.H + 31) / 32, It = (m.I + 31) / 32;
+    const int most = m.E < m.T * m.top ? m.E : m.T * m.top;
+    Args a = {};
+    a.x = (const __nv_bfloat16 *)m.x; a.ldx = m.ldx;
+    a.rows = m.T; a.K = m.H; a.Kt = Ht; a.N = m.I; a.Nt = It;
+    a.w0 = (const uint8_t *)m.gate; a.w1 = (const uint8_t *)m.up;
+    a.ids = m.ids; a.wts = m.weights; a.top = m.top; a.E = m.E; a.act = m.act;
+    a.h = (__nv_bfloat16 *)m.h; a.hpad = 32 * It;
+    a.status = status;
+    const int span = m.up ? kGroupTiles / 2 : kGroupTiles, groups = (It + span - 1) / span;
+    a.cluster = split_of((int64_t)groups * most, Ht, sm_count, tok == 8 ? 2 : 1);
+    cudaError_t e = dispatch<kExpertsIn>(m.mant_bits, m.T, a, dim3(groups * a.cluster, most, passes), dependent, stream);
+    if (e != cudaSuccess) return e;
+    a.K = m.I; a.Kt = It; a.N = m.H; a.Nt = Ht;
+    a.w0 = (const uint8_t *)m.down; a.w1 = nullptr;
+    a.out = m.y; a.ldo = m.ldy; a.out_f32 = 0;
+    const int groups2 = (Ht + kGroupTiles - 1) / kGroupTiles;
+    a.cluster = split_of((int64_t)groups2 * passes, (int64_t)It, sm_count, tok == 8 ? 2 : 1);
+    return dispatch<kExpertsOut>(m.mant_bits, m.T, a, dim3(groups2 * a.cluster, passes), true, stream);
+}
+
+}  // namespace buda

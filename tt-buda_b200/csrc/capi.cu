@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "buda_common.cuh"
+#include "few_rows.cuh"
 
 namespace buda {
 cudaError_t launch_tilize(const TileJob &job, const PtrTable &ptrs, int batch, int mant_bits, int es, int a_format, int path,
@@ -40,6 +41,11 @@ cudaError_t launch_prestride(const void *src, int elem_bytes, const uint32_t sha
 cudaError_t launch_i8_gemm(const void *A, int64_t M, int64_t K, int64_t lda, const void *W, int64_t N, const float *scale,
                            int64_t scale_len, float zero_point, int out_mode, void *C, int64_t ldc, int sm_count, cudaStream_t stream,
                            unsigned int *status, char *err, size_t err_len);
+cudaError_t launch_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, const void *W, int64_t N, int mant_bits, void *Y, int64_t ldy,
+                              int out_f32, int sm_count, cudaStream_t stream, unsigned int *status);
+cudaError_t launch_moe_route(const void *x, int64_t ldx, int T, int H, const void *w, int w_f32, int64_t ldw, int E, int top, int renorm,
+                             float *weights, int *ids, int sm_count, cudaStream_t stream);
+cudaError_t launch_moe_experts(const MoeArgs &m, bool dependent, int sm_count, cudaStream_t stream, unsigned int *status);
 
 // One CTA, one thread waiting: the barrier expects one arrival that never comes.  The other 31 lanes only take part in
 // the final warp convergence.  The wait is the product kernels' own mbar_wait_bounded with a caller-given limit.
@@ -1333,6 +1339,148 @@ int buda_i8_gemm(const void *A, int64_t M, int64_t K, int64_t lda, const void *W
     if (e != cudaSuccess) return msg[0] ? fail(BUDA_RUNTIME_ERROR, "%s", msg) : cuda_fail(e, "int8 gemm launch failed");
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return BUDA_SUCCESS;
+}
+
+static_assert(kMaxFewRows == BUDA_MAX_FEW_ROWS && kMaxExperts == BUDA_MAX_EXPERTS && kMaxTop == BUDA_MAX_TOP, "limits of the header");
+
+static bool misaligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+
+// The checks that the few-row operators share: what the images are stored as, and how they have to be read.
+static int check_few_rows(const char *what, int64_t rows, const void *x, int64_t ldx, int64_t a, int64_t b, int w_df)
+{
+    constexpr int64_t kMost = 1 << 24;
+    if (rows < 0 || rows > kMaxFewRows) return fail(BUDA_RUNTIME_ERROR, "%s: %lld rows, 0 to %d are supported", what, (long long)rows, kMaxFewRows);
+    if (a < 1 || b < 1 || a > kMost || b > kMost)
+        return fail(BUDA_RUNTIME_ERROR, "%s: sizes %lld and %lld are not in 1..%lld", what, (long long)a, (long long)b, (long long)kMost);
+    if (ldx < 0) return fail(BUDA_RUNTIME_ERROR, "%s: negative row stride", what);
+    if (!is_bfp_b(w_df)) return fail(BUDA_RUNTIME_ERROR, "%s: weights must be Bfp8_b, Bfp4_b or Bfp2_b, got data format %d", what, w_df);
+    if (rows && !x) return fail(BUDA_RUNTIME_ERROR, "%s: null matrix pointer", what);
+    if (misaligned(x, 2)) return fail(BUDA_RUNTIME_ERROR, "%s: activations must be 2-byte aligned", what);
+    BfpPolicy layout = current_policy();
+    layout.rmode = layout.bump = 0;   // rounding and overflow do not change how bytes are read back
+    if (!policy_is_default(layout))
+        return fail(BUDA_RUNTIME_ERROR, "%s reads weight images in the default byte layout; the current block-float policy changes it", what);
+    return BUDA_SUCCESS;
+}
+
+int buda_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, const void *W_tiles, int64_t N, int w_df, void *Y, int64_t ldy,
+                    int y_df, void *stream)
+{
+    DevCtx *ctx;
+    if (int rc = get_ctx(&ctx)) return rc;
+    if (int rc = check_few_rows("bfp_matvec", M, A, lda, K, N, w_df)) return rc;
+    if (y_df != BUDA_DF_Float16_b && y_df != BUDA_DF_Float32)
+        return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: the output must be Float16_b or Float32, got data format %d", y_df);
+    if (M > 1 && ldy < N) return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: output rows of %lld values overlap at a stride of %lld", (long long)N, (long long)ldy);
+    if (M == 0) return BUDA_SUCCESS;
+    if (!W_tiles || !Y) return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: null matrix pointer");
+    if (misaligned(W_tiles, 16)) return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: weight images must be 16-byte aligned");
+    if (misaligned(Y, y_df == BUDA_DF_Float32 ? 4 : 2)) return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: misaligned output");
+    cudaError_t e = launch_bfp_matvec(A, M, K, lda, W_tiles, N, bfp_mant_bits(w_df), Y, ldy, y_df == BUDA_DF_Float32, ctx->sm_count,
+                                      (cudaStream_t)stream, ctx->status);
+    if (e != cudaSuccess) return cuda_fail(e, "bfp_matvec launch failed");
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return BUDA_SUCCESS;
+}
+
+static int check_route(int64_t T, const void *X, int64_t H, int64_t ldx, const void *W, int router_df, int64_t ldw, int64_t E, int top,
+                       const float *weights, const int32_t *ids)
+{
+    if (T < 0 || T > kMaxFewRows) return fail(BUDA_RUNTIME_ERROR, "moe_route: %lld tokens, 0 to %d are supported", (long long)T, kMaxFewRows);
+    if (H < 1 || H > (1 << 24)) return fail(BUDA_RUNTIME_ERROR, "moe_route: hidden size %lld is not in 1..2^24", (long long)H);
+    if (E < 1 || E > kMaxExperts) return fail(BUDA_RUNTIME_ERROR, "moe_route: %lld experts, 1 to %d are supported", (long long)E, kMaxExperts);
+    if (top < 1 || top > kMaxTop || top > E)
+        return fail(BUDA_RUNTIME_ERROR, "moe_route: %d experts for a token, 1 to %d and at most the %lld there are", top, kMaxTop, (long long)E);
+    if (router_df != BUDA_DF_Float32 && router_df != BUDA_DF_Float16_b)
+        return fail(BUDA_RUNTIME_ERROR, "moe_route: router weights must be Float32 or Float16_b, got data format %d", router_df);
+    if (ldx < 0 || ldw < 0) return fail(BUDA_RUNTIME_ERROR, "moe_route: negative row stride");
+    if (!W || (T && (!X || !weights || !ids))) return fail(BUDA_RUNTIME_ERROR, "moe_route: null pointer");
+    if (misaligned(X, 2) || misaligned(W, router_df == BUDA_DF_Float32 ? 4 : 2) || misaligned(weights, 4) || misaligned(ids, 4))
+        return fail(BUDA_RUNTIME_ERROR, "moe_route: misaligned pointer");
+    return BUDA_SUCCESS;
+}
+
+int buda_moe_route(const void *X, int64_t T, int64_t H, int64_t ldx, const void *W_router, int router_df, int64_t ldw, int64_t E,
+                   int top, int renormalize, float *weights, int32_t *ids, void *stream)
+{
+    DevCtx *ctx;
+    if (int rc = get_ctx(&ctx)) return rc;
+    if (int rc = check_route(T, X, H, ldx, W_router, router_df, ldw, E, top, weights, ids)) return rc;
+    if (T == 0) return BUDA_SUCCESS;
+    cudaError_t e = launch_moe_route(X, ldx, (int)T, (int)H, W_router, router_df == BUDA_DF_Float32, ldw, (int)E, top, renormalize != 0,
+                                     weights, ids, ctx->sm_count, (cudaStream_t)stream);
+    if (e != cudaSuccess) return cuda_fail(e, "moe_route launch failed");
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return BUDA_SUCCESS;
+}
+
+int64_t buda_moe_workspace_bytes(int64_t T, int top, int64_t I)
+{
+    if (T < 0 || T > kMaxFewRows || top < 1 || top > kMaxTop || I < 1 || I > (1 << 24)) {
+        fail(BUDA_RUNTIME_ERROR, "moe workspace: %lld tokens, %d experts each, intermediate size %lld", (long long)T, top, (long long)I);
+        return -1;
+    }
+    return moe_h_bytes(T, top, I);
+}
+
+static int check_experts(const void *X, int64_t T, int64_t H, int64_t ldx, const float *weights, const int32_t *ids, int top,
+                         const void *gate, const void *up, const void *down, int64_t E, int64_t I, int w_df, int act, const void *Y,
+                         int64_t ldy, const void *workspace, uint64_t workspace_bytes)
+{
+    if (int rc = check_few_rows("moe_experts", T, X, ldx, H, I, w_df)) return rc;
+    if (E < 1 || E > kMaxExperts) return fail(BUDA_RUNTIME_ERROR, "moe_experts: %lld experts, 1 to %d are supported", (long long)E, kMaxExperts);
+    if (top < 1 || top > kMaxTop) return fail(BUDA_RUNTIME_ERROR, "moe_experts: %d experts for a token, 1 to %d are supported", top, kMaxTop);
+    if (act != BUDA_ACT_SILU && act != BUDA_ACT_GELU) return fail(BUDA_RUNTIME_ERROR, "moe_experts: unknown activation %d", act);
+    if (T > 1 && ldy < H) return fail(BUDA_RUNTIME_ERROR, "moe_experts: output rows of %lld values overlap at a stride of %lld", (long long)H, (long long)ldy);
+    if (!gate || !down || (T && (!weights || !ids || !Y || !workspace))) return fail(BUDA_RUNTIME_ERROR, "moe_experts: null pointer");
+    if (misaligned(gate, 16) || misaligned(up, 16) || misaligned(down, 16) || misaligned(workspace, 16))
+        return fail(BUDA_RUNTIME_ERROR, "moe_experts: weight images and the workspace must be 16-byte aligned");
+    if (misaligned(weights, 4) || misaligned(ids, 4) || misaligned(Y, 2)) return fail(BUDA_RUNTIME_ERROR, "moe_experts: misaligned pointer");
+    if ((uint64_t)moe_h_bytes(T, top, I) > workspace_bytes)
+        return fail(BUDA_RUNTIME_ERROR, "moe_experts: workspace of %llu bytes, %lld are needed", (unsigned long long)workspace_bytes,
+                    (long long)moe_h_bytes(T, top, I));
+    return BUDA_SUCCESS;
+}
+
+static int run_experts(DevCtx *ctx, const void *X, int64_t T, int64_t H, int64_t ldx, const float *weights, const int32_t *ids, int top,
+                       const void *gate, const void *up, const void *down, int64_t E, int64_t I, int w_df, int act, void *Y, int64_t ldy,
+                       void *workspace, bool after_route, void *stream)
+{
+    MoeArgs m;
+    m.x = X; m.ldx = ldx;
+    m.T = (int)T; m.H = (int)H; m.I = (int)I; m.E = (int)E; m.top = top;
+    m.mant_bits = bfp_mant_bits(w_df); m.act = act;
+    m.weights = weights; m.ids = ids;
+    m.gate = gate; m.up = up; m.down = down;
+    m.y = Y; m.ldy = ldy; m.h = workspace;
+    cudaError_t e = launch_moe_experts(m, after_route, ctx->sm_count, (cudaStream_t)stream, ctx->status);
+    if (e != cudaSuccess) return cuda_fail(e, "moe_experts launch failed");
+    g_launches.fetch_add(2, std::memory_order_relaxed);
+    return BUDA_SUCCESS;
+}
+
+int buda_moe_experts(const void *X, int64_t T, int64_t H, int64_t ldx, const float *weights, const int32_t *ids, int top,
+                     const void *gate, const void *up, const void *down, int64_t E, int64_t I, int w_df, int act, void *Y,
+                     int64_t ldy, void *workspace, uint64_t workspace_bytes, void *stream)
+{
+    DevCtx *ctx;
+    if (int rc = get_ctx(&ctx)) return rc;
+    if (int rc = check_experts(X, T, H, ldx, weights, ids, top, gate, up, down, E, I, w_df, act, Y, ldy, workspace, workspace_bytes)) return rc;
+    if (T == 0) return BUDA_SUCCESS;
+    return run_experts(ctx, X, T, H, ldx, weights, ids, top, gate, up, down, E, I, w_df, act, Y, ldy, workspace, false, stream);
+}
+
+int buda_moe_layer(const void *X, int64_t T, int64_t H, int64_t ldx, const void *W_router, int router_df, int64_t ldw, int top,
+                   int renormalize, const void *gate, const void *up, const void *down, int64_t E, int64_t I, int w_df, int act,
+                   float *weights, int32_t *ids, void *Y, int64_t ldy, void *workspace, uint64_t workspace_bytes, void *stream)
+{
+    DevCtx *ctx;
+    if (int rc = get_ctx(&ctx)) return rc;
+    if (int rc = check_route(T, X, H, ldx, W_router, router_df, ldw, E, top, weights, ids)) return rc;
+    if (int rc = check_experts(X, T, H, ldx, weights, ids, top, gate, up, down, E, I, w_df, act, Y, ldy, workspace, workspace_bytes)) return rc;
+    if (T == 0) return BUDA_SUCCESS;
+    if (int rc = buda_moe_route(X, T, H, ldx, W_router, router_df, ldw, E, top, renormalize, weights, ids, stream)) return rc;
+    return run_experts(ctx, X, T, H, ldx, weights, ids, top, gate, up, down, E, I, w_df, act, Y, ldy, workspace, true, stream);
 }
 
 int buda_prestride(const void *src, int elem_bytes, const uint32_t shape[4], const uint64_t strides_bytes[4], int stride,

@@ -1,0 +1,213 @@
+// K10: the router of a mixture of experts for a few tokens, one launch.
+//
+//   l[t, e] = sum_h x[t, h] w[e, h],  p = softmax(l[t, :]),  the `top` largest l of a token in descending order (of equal
+//   ones the lowest index first),  weight = p, or p over the sum of the chosen ones
+//
+// Bound: for a few tokens the latency of one pass over w (E * H values that every cluster reads once, from L2 after the
+// first).  A cluster of 8 CTAs takes a block of tokens; its CTAs share the experts, the warps of a CTA share an expert's
+// row when there are fewer experts than warps, so that all of w is asked for at once.  The scores meet in distributed
+// shared memory; the warp of token i chooses in CTA i % 8.
+// Scores decide which experts run, so they are summed more exactly than a binary32 chain would: 8 products at a time in
+// binary32, the groups in binary64, kept in binary64 until the largest has been taken off.
+#include <cuda_bf16.h>
+
+#include "few_rows.cuh"
+
+namespace buda {
+namespace route {
+
+constexpr int kCluster = 8;
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kPerCta = kMaxExperts / kCluster;
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ double ld_cluster_f64(const double *p, uint32_t rank)
+{
+    uint32_t a;
+    double v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// Eight consecutive values of a row as binary32; `vec`: 16-byte loads are allowed.  Zero past H.
+__device__ __forceinline__ void load8(float (&v)[8], const __nv_bfloat16 *row, int h, int H, bool vec)
+{
+    if (vec && h + 8 <= H) {
+        const uint4 r = *reinterpret_cast<const uint4 *>(row + h);
+        const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = __uint_as_float(u[i] << 16);
+            v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = h + i < H ? __bfloat162float(row[h + i]) : 0.0f;
+    }
+}
+__device__ __forceinline__ void load8(float (&v)[8], const float *row, int h, int H, bool vec)
+{
+    if (vec && h + 8 <= H) {
+        const float4 a = *reinterpret_cast<const float4 *>(row + h), b = *reinterpret_cast<const float4 *>(row + h + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = h + i < H ? row[h + i] : 0.0f;
+    }
+}
+
+// Binary64 in an order that unsigned integers have: NaN below every number, 0 for "already chosen".
+__device__ __forceinline__ uint64_t order_of(double l)
+{
+    if (isnan(l)) return 1ull;
+    const uint64_t b = (uint64_t)__double_as_longlong(l + 0.0);
+    return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+
+template <typename TW, int TB>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
+    route_kernel(const __nv_bfloat16 *x, int64_t ldx, int T, int H, const TW *w, int64_t ldw, int E, int top, int renorm, int split,
+                 float *weights, int *ids)
+{
+    __shared__ double part[kPerCta * TB * kWarps];      // [expert of this CTA][token][piece of the row]
+    __shared__ double score[kPerCta * TB];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const int t0 = (blockIdx.x / kCluster) * TB, nt = min(T - t0, TB);
+    const int mine = E > (int)rank ? (E - (int)rank + kCluster - 1) / kCluster : 0;   // experts rank, rank + 8, ...
+    const bool xvec = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * 2)) & 15) == 0;
+    const bool wvec = ((reinterpret_cast<uintptr_t>(w) | (uintptr_t)(ldw * sizeof(TW))) & 15) == 0;
+    const int octets = (H + 7) / 8;
+    for (int task = warp; task < mine * split; task += kWarps) {
+        const int el = task / split, piece = task % split;
+        const TW *row = w + (int64_t)(rank + el * kCluster) * ldw;
+        const int o1 = (int)((int64_t)octets * (piece + 1) / split);
+        double s[TB];
+#pragma unroll
+        for (int i = 0; i < TB; i++) s[i] = 0.0;
+#pragma unroll 4
+        for (int o = (int)((int64_t)octets * piece / split) + lane; o < o1; o += 32) {
+            float a[8];
+            load8(a, row, o * 8, H, wvec);
+#pragma unroll
+            for (int i = 0; i < TB; i++) {
+                if (i >= nt) break;
+                float b[8];
+                load8(b, x + (int64_t)(t0 + i) * ldx, o * 8, H, xvec);
+                float p = 0.0f;
+#pragma unroll
+                for (int v = 0; v < 8; v++) p = fmaf(a[v], b[v], p);
+                s[i] += (double)p;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < TB; i++) {
+#pragma unroll
+            for (int d = 16; d; d >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
+            if (lane == 0) part[(el * TB + i) * split + piece] = s[i];
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < mine * TB; i += kThreads) {
+        double v = 0.0;
+        for (int p = 0; p < split; p++) v += part[i * split + p];
+        score[i] = v;
+    }
+    cluster_sync();
+    // warp `warp` of CTA `rank` chooses for token 8 * warp + rank of the block
+    const int i = warp * kCluster + (int)rank;
+    if (i < nt) {
+        double l[kMaxExperts / 32];
+        uint64_t key[kMaxExperts / 32];
+#pragma unroll
+        for (int q = 0; q < kMaxExperts / 32; q++) {
+            const int e = q * 32 + lane;
+            l[q] = e < E ? ld_cluster_f64(&score[(e / kCluster) * TB + i], e % kCluster) : 0.0;
+            key[q] = e < E ? order_of(l[q]) : 0ull;
+        }
+        int my_id = 0;              // lane s keeps the s-th choice
+        double my_l = 0.0, most = 0.0;
+        for (int s = 0; s < top; s++) {
+            uint64_t best = 0;
+            int at = 0;
+            double bl = 0.0;
+#pragma unroll
+            for (int q = 0; q < kMaxExperts / 32; q++)
+                if (key[q] > best) {
+                    best = key[q];
+                    at = q * 32 + lane;
+                    bl = l[q];
+                }
+            const uint32_t hi = (uint32_t)(best >> 32), mhi = __reduce_max_sync(0xffffffffu, hi);
+            const uint32_t lo = hi == mhi ? (uint32_t)best : 0u, mlo = __reduce_max_sync(0xffffffffu, lo);
+            const bool in = hi == mhi && (uint32_t)best == mlo;
+            const uint32_t id = __reduce_min_sync(0xffffffffu, in ? (uint32_t)at : 0xffffffffu);
+            const double v = __shfl_sync(0xffffffffu, bl, id & 31);
+#pragma unroll
+            for (int q = 0; q < kMaxExperts / 32; q++)
+                if (q * 32 + lane == (int)id) key[q] = 0;
+            if (s == 0) most = v;
+            if (lane == s) {
+                my_id = (int)id;
+                my_l = v;
+            }
+        }
+        float sum = 0.0f;
+        if (renorm) {
+            sum = lane < top ? expf((float)(my_l - most)) : 0.0f;
+        } else {
+#pragma unroll
+            for (int q = 0; q < kMaxExperts / 32; q++)
+                if (q * 32 + lane < E) sum += expf((float)(l[q] - most));
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane < top) {
+            const int64_t o = (int64_t)(t0 + i) * top + lane;
+            ids[o] = my_id;
+            weights[o] = expf((float)(my_l - most)) / sum;
+        }
+    }
+    cluster_sync();      // no CTA leaves while another reads its scores
+}
+
+template <typename TW>
+cudaError_t launch_tw(const void *x, int64_t ldx, int T, int H, const void *w, int64_t ldw, int E, int top, int renorm, float *weights,
+                      int *ids, int sm_count, cudaStream_t stream)
+{
+    // enough tokens to a cluster that all clusters are resident at once
+    const int clusters = sm_count / kCluster > 0 ? sm_count / kCluster : 1;
+    const int tb = T <= clusters ? 1 : T <= 2 * clusters ? 2 : 4;
+    const int most = (E + kCluster - 1) / kCluster;
+    int split = 1;
+    while (split < kWarps && split * 2 * most <= kWarps) split *= 2;
+    const dim3 grid((unsigned)((T + tb - 1) / tb * kCluster));
+#define BUDA_ROUTE(TB)                                                                                                        \
+    route_kernel<TW, TB><<<grid, kThreads, 0, stream>>>((const __nv_bfloat16 *)x, ldx, T, H, (const TW *)w, ldw, E, top, renorm, \
+                                                        split, weights, ids)
+    if (tb == 1) BUDA_ROUTE(1);
+    else if (tb == 2) BUDA_ROUTE(2);
+    else BUDA_ROUTE(4);
+#undef BUDA_ROUTE
+    return cudaGetLastError();
+}
+
+}  // namespace route
+
+cudaError_t launch_moe_route(const void *x, int64_t ldx, int T, int H, const void *w, int w_f32, int64_t ldw, int E, int top, int renorm,
+                             float *weights, int *ids, int sm_count, cudaStream_t stream)
+{
+    return w_f32 ? route::launch_tw<float>(x, ldx, T, H, w, ldw, E, top, renorm, weights, ids, sm_count, stream)
+                 : route::launch_tw<__nv_bfloat16>(x, ldx, T, H, w, ldw, E, top, renorm, weights, ids, sm_count, stream);
+}
+
+}  // namespace buda

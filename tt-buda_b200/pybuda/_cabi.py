@@ -123,6 +123,12 @@ _SIGS = {
     "buda_bfp8b_gemm_multicast": (_i, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
     "buda_prestride": (_i, [_vp, _i, _u32p, _u64p, _i, ctypes.POINTER(ctypes.c_int), _i, _vp, _u32, _u32, _vp]),
     "buda_i8_gemm": (_i, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _f, _i, _vp, _i64, _vp]),
+    "buda_bfp_matvec": (_i, [_vp, _i64, _i64, _i64, _vp, _i64, _i, _vp, _i64, _i, _vp]),
+    "buda_moe_route": (_i, [_vp, _i64, _i64, _i64, _vp, _i, _i64, _i64, _i, _i, _vp, _vp, _vp]),
+    "buda_moe_workspace_bytes": (_i64, [_i64, _i, _i64]),
+    "buda_moe_experts": (_i, [_vp, _i64, _i64, _i64, _vp, _vp, _i, _vp, _vp, _vp, _i64, _i64, _i, _i, _vp, _i64, _vp, _u64, _vp]),
+    "buda_moe_layer": (_i, [_vp, _i64, _i64, _i64, _vp, _i, _i64, _i, _i, _vp, _vp, _vp, _i64, _i64, _i, _i, _vp, _vp, _vp, _i64, _vp,
+                            _u64, _vp]),
     "buda_gemm_select_kernel": (_i, [_i]),
     "buda_selftest_bounded_wait": (_i, [_u32, _vp]),
     "buda_ipc_export": (_i, [_vp, ctypes.c_char_p]),
