@@ -95,6 +95,41 @@ def test_matvec_shared_exponents_of_the_whole_range(ops, oracle, df, exponent):
     assert np.abs(w).max() >= 2.0 ** (exponent - 127) * (1 if m > 1 else 0.5)
 
 
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("exponent", [1, 2, 7, 64, 126, 127, 128, 129, 190, 253])
+def test_matvec_one_row_over_the_whole_range(ops, oracle, df, exponent):
+    """The same for a single row, whose activations are scaled in place of the weights: each of the 32 rows on its own, with
+    activations from the smallest normal number to the largest that keeps the product finite."""
+    code, m = getattr(ops.DF, df), {"Bfp8_b": 7, "Bfp4_b": 3, "Bfp2_b": 1}[df]
+    rec = {"Bfp8_b": 1088, "Bfp4_b": 576, "Bfp2_b": 320}[df]
+    raw = np.random.default_rng(exponent).integers(0, 256, rec, dtype=np.uint8)
+    raw[:64] = exponent
+    w = oracle.unpack_untilize(raw, getattr(oracle, df), (1, 1, 32, 32))[0, 0].astype(np.float64)
+    img = torch.from_numpy(raw).cuda()
+    for power in (-126, -100, -30, 0, 30, 100, 127):
+        if not -110 <= exponent - 127 + power <= 126:
+            continue                        # the product leaves binary32, or is small enough to be rounded at 2^-125
+        for k in (0, 5, 14, 31):
+            a = torch.zeros(1, 32)
+            a[0, k] = -(2.0 ** power)
+            got = ops.bfp_matvec(a.bfloat16().cuda(), img, 32, code, out_dtype=torch.float32).cpu().numpy()
+            assert np.array_equal(got[0].astype(np.float64), -w[k] * 2.0 ** power), (power, k)
+
+
+@pytest.mark.parametrize("df", FORMATS)
+def test_matvec_one_row_of_mixed_magnitudes(ops, oracle, df):
+    """Blocks of very unlike shared exponents in one matrix against activations that undo them: every step takes the wide path."""
+    k, n = 160, 200
+    rng = np.random.default_rng(2)
+    power = rng.integers(-60, 61, (k, 1))
+    w0 = rng.standard_normal((k, n)) * 2.0 ** power * np.repeat(2.0 ** rng.integers(-8, 9, (k, -(-n // 16))), 16, 1)[:, :n]
+    img, w = _store(oracle, w0.astype(np.float32), df)
+    for rows in (1, 3):
+        a = torch.from_numpy(rng.standard_normal((rows, k)) * 2.0 ** (-power[:, 0] + 20)).bfloat16()
+        got = ops.bfp_matvec(a.cuda(), img, n, getattr(ops.DF, df), out_dtype=torch.float32)
+        _check_sum(got, a.double().numpy(), w, torch.float32)
+
+
 def test_matvec_not_finite_activations_stay_in_their_row(ops, oracle):
     k, n = 64, 96
     img, w = _store(oracle, _rand((k, n), 5) + 0.1, "Bfp4_b")
@@ -103,6 +138,8 @@ def test_matvec_not_finite_activations_stay_in_their_row(ops, oracle):
     got = ops.bfp_matvec(a.cuda(), img, n, ops.DF.Bfp4_b, out_dtype=torch.float32).cpu()
     assert torch.isnan(got[1]).all() and not torch.isfinite(got[2]).any()
     _check_sum(got[[0, 3]], a.double().numpy()[[0, 3]], w, torch.float32)
+    assert torch.isnan(ops.bfp_matvec(a[1:2].cuda(), img, n, ops.DF.Bfp4_b)).all()
+    assert not torch.isfinite(ops.bfp_matvec(a[2:3].cuda(), img, n, ops.DF.Bfp4_b)).any()
 
 
 def test_matvec_strides_alignment_and_neighbours(ops, oracle):

@@ -24,7 +24,8 @@
 // Sums are held in binary32 throughout.  h is carried between the two launches as two bfloat16 pieces (the rounded value and
 // the rounded rest, together within 2^-16 of h), so nothing is lost against a binary32 h at twice the tensor work.
 #include <cuda_bf16.h>
-#include <cstdio>
+
+#include <atomic>
 
 #include "few_rows.cuh"
 
@@ -35,8 +36,12 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kGroupTiles = 4;          // tile columns of one warp
 constexpr int kPitch = 132;             // floats per token of a warp's sums: 8-byte stores of 4 x 4 lanes meet no bank twice
+constexpr int kDown = 24;               // single-token sums are held times 2^-24 (see single_step)
 
 enum { kMatvec = 0, kExpertsIn = 1, kExpertsOut = 2 };
+
+// CTAs that an SM holds, by registers: 80 suffice for one token (but for the two pieces of experts-out), 128 for up to 16 tokens
+__host__ __device__ constexpr int ctas_per_sm(int nt, int mode) { return nt == 0 && mode != kExpertsOut ? 3 : nt <= 2 ? 2 : 1; }
 
 template <int MB>
 struct Fmt {
@@ -44,7 +49,7 @@ struct Fmt {
     static constexpr int kFace = 16 * kRow;
     static constexpr int kRec = 64 + 4 * kFace;
     static constexpr int kStage = kGroupTiles * kRec;
-    static constexpr int kStages = MB == 7 ? 3 : MB == 3 ? 5 : 8;
+    static constexpr int kStages = MB == 7 ? 2 : MB == 3 ? 4 : 7;   // about 72 KB of rings: three CTAs fit an SM
 };
 
 struct Args {
@@ -155,10 +160,19 @@ __device__ __forceinline__ void pair_of(const Raw<MB> &r, int p, int j, uint32_t
     }
 }
 
-// 2^a and 2^b (0 <= a, b <= 127) as a bfloat16 pair
-__device__ __forceinline__ uint32_t pow2_pair(uint32_t a, uint32_t b) { return ((a + 127u) << 7) | ((b + 127u) << 23); }
+// 2^a and 2^b (-127 < a, b <= 127) as a bfloat16 pair
+__device__ __forceinline__ uint32_t pow2_pair(int a, int b) { return ((uint32_t)(a + 127) << 7) | ((uint32_t)(b + 127) << 23); }
 
-// One 16-row step: BIG where a shared exponent is above 127 (2^E is no bfloat16 then: up to three factors).
+// the two shared exponents of a row pair, moved by `by`, as a pair of powers of two (0 < exponent + by + 127 < 255)
+__device__ __forceinline__ uint32_t scale_pair(uint32_t e, int by)
+{
+    return (__byte_perm(e, 0u, 0x4140u) + (uint32_t)(by + 127) * 0x00010001u) << 7;
+}
+
+__device__ __forceinline__ bool not_finite_pair(uint32_t v) { return (((v & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0; }
+
+// One 16-row step for up to 8 * NT tokens: the weights are scaled.  BIG where a shared exponent is above 127 (2^E is no
+// bfloat16 then: up to three factors).
 template <int MB, int NT, int PIECES, bool BIG>
 __device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw, const uint32_t (&e)[2], uint32_t sel_flip,
                                      const uint32_t (&x)[PIECES][NT][2])
@@ -166,13 +180,13 @@ __device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw,
     uint32_t s[2], s2[2], s3[2];
 #pragma unroll
     for (int p = 0; p < 2; p++) {
-        const uint32_t a = e[p] & 0xffu, b = e[p] >> 8;
         if constexpr (BIG) {
-            s[p] = pow2_pair(min(a, 127u), min(b, 127u));
-            s2[p] = pow2_pair(min(max(a, 127u) - 127u, 127u), min(max(b, 127u) - 127u, 127u));
-            s3[p] = pow2_pair(max(a, 254u) - 254u, max(b, 254u) - 254u);
+            const int a = e[p] & 0xff, b = e[p] >> 8;
+            s[p] = pow2_pair(min(a, 127), min(b, 127));
+            s2[p] = pow2_pair(min(max(a - 127, 0), 127), min(max(b - 127, 0), 127));
+            s3[p] = pow2_pair(max(a - 254, 0), max(b - 254, 0));
         } else {
-            s[p] = pow2_pair(a, b);
+            s[p] = scale_pair(e[p], 0);
         }
     }
 #pragma unroll
@@ -195,6 +209,57 @@ __device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw,
     }
 }
 
+// The same for ONE token: the 8 columns of the product are free, so column g carries the token's values scaled by the
+// shared exponents of lane group g's own face, and the weights stay the unscaled subnormals -- 2 multiplies instead of 32.
+// Only the diagonal (row group g, column g) counts.  The columns are held times 2^-24, which keeps x 2^E inside bfloat16
+// up to |x| max|w| = 2^24 (a product below 2^-102 is then rounded at 2^-125).
+template <int MB, int PIECES>
+__device__ __forceinline__ void single_step(float (&acc)[8][1][4], const Raw<MB> &raw, uint32_t sel_flip, const uint32_t (&b)[PIECES][2])
+{
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        uint32_t a[4];
+        pair_of<MB>(raw, 0, j, sel_flip, a[0], a[1]);
+        pair_of<MB>(raw, 1, j, sel_flip, a[2], a[3]);
+#pragma unroll
+        for (int q = 0; q < PIECES; q++) mma16816(acc[j][0], a, b[q][0], b[q][1]);
+    }
+}
+
+// One token where some x 2^(E - 24) is no finite bfloat16: what is too much for the column goes to the weights.
+template <int MB, int PIECES>
+__device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Raw<MB> &raw, const uint32_t (&e)[2], uint32_t sel_flip,
+                                              const uint32_t (&x)[PIECES][2])
+{
+#pragma unroll
+    for (int q = 0; q < PIECES; q++) {
+        uint32_t b[2], s1[2], s2[2], s3[2];
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            int d[2], v[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int E = (e[p] >> (8 * h)) & 0xff, ex = (x[q][p] >> (7 + 16 * h)) & 0xff;
+                d[h] = E == 255 ? 255 : max(ex + E - kDown - 254, 0);   // a weight of 2^128 and above stays an infinity
+                v[h] = E - kDown - d[h];
+            }
+            b[p] = mul_bf16x2(mul_bf16x2(x[q][p], pow2_pair(min(v[0], 127), min(v[1], 127))), pow2_pair(max(v[0] - 127, 0), max(v[1] - 127, 0)));
+            s1[p] = pow2_pair(min(d[0], 127), min(d[1], 127));
+            s2[p] = pow2_pair(min(max(d[0] - 127, 0), 127), min(max(d[1] - 127, 0), 127));
+            s3[p] = pow2_pair(max(d[0] - 254, 0), max(d[1] - 254, 0));
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            uint32_t a[4];
+            pair_of<MB>(raw, 0, j, sel_flip, a[0], a[1]);
+            pair_of<MB>(raw, 1, j, sel_flip, a[2], a[3]);
+#pragma unroll
+            for (int c = 0; c < 4; c++) a[c] = mul_bf16x2(mul_bf16x2(mul_bf16x2(a[c], s1[c >> 1]), s2[c >> 1]), s3[c >> 1]);
+            mma16816(acc[j][0], a, b[0], b[1]);
+        }
+    }
+}
+
 // Elements k, k+1 of a row (k even), zero past K.
 __device__ __forceinline__ uint32_t load_pair(const __nv_bfloat16 *row, int k, int K, bool vec)
 {
@@ -213,7 +278,7 @@ __device__ __forceinline__ float activate(float v, int act)
 // Shared memory: [ring of every warp | the warps' sums, over the ring][the CTA's sums][barriers][tables]
 template <int MB, int NT>
 struct Lay {
-    static constexpr int kTok = 8 * NT;
+    static constexpr int kTok = NT ? 8 * NT : 1;
     static constexpr int kRing = kWarps * Fmt<MB>::kStages * Fmt<MB>::kStage;
     static constexpr int kSums = kWarps * kTok * kPitch * 4;
     static constexpr int kFirst = kRing > kSums ? kRing : kSums;
@@ -222,52 +287,250 @@ struct Lay {
     static constexpr int kTables = kBars + kWarps * Fmt<MB>::kStages * 8;
     static constexpr int kMap = kTables;                                  // 8 words: bit e set where expert e has a token
     static constexpr int kCtl = kMap + kMaxExperts / 8;                   // 4 words
-    static constexpr int kList = kCtl + 16;                               // in: tokens (row, slot, weight); out: experts
+    static constexpr int kList = kCtl + 16;                               // in: (slot, weight) of the tokens; out: experts
     static constexpr int kRows = kList + 4 * kMaxExperts;                 // out: slot of (expert, token)
-    static constexpr int kBytesIn = kRows;
-    static constexpr int kBytesOut = kRows + 2 * kMaxExperts * kTok;
+    static constexpr int kBytes(int mode) { return mode == kMatvec ? kList : mode == kExpertsIn ? kRows : kRows + 2 * kMaxExperts * kTok; }
 };
 
+// What a warp works on: `units` tile rows of (expert, tile row) pairs, its own share of them, and its ring.
+struct Work {
+    int n_tok, tok0;             // tokens of this CTA; the first one
+    int units;
+    int64_t w_off;               // experts-in: where this expert's images begin
+    const int *list;
+    const int16_t *rows;
+};
+
+// The sums of this warp's share of the tile rows, left in sums[warp][token][j][g][2].  SINGLE: one token (NT = 1 then).
+template <int MB, int NT, int MODE, bool SINGLE>
+__device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *smem, uint64_t *bars, volatile int *abort_flag, int group, int me,
+                                         int workers, int tok_pitch)
+{
+    using F = Fmt<MB>;
+    constexpr int S = F::kStages;
+    constexpr int PIECES = MODE == kExpertsOut ? 2 : 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint8_t *ring = smem + warp * S * F::kStage;
+    const int64_t image = (int64_t)A.Kt * A.Nt * F::kRec;
+    const int u0 = (int)((int64_t)W.units * me / workers), n = (int)((int64_t)W.units * (me + 1) / workers) - u0;
+    const bool gated = MODE == kExpertsIn && A.w1 != nullptr;
+    const int span = gated ? kGroupTiles / 2 : kGroupTiles;
+    const int nt0 = group * span;
+    const uint32_t bytes = (uint32_t)min(span, A.Nt - nt0) * F::kRec;
+
+    // the copies of the warp's next tile row: (i_s, i_kt) and the ring stage advance with every call
+    int i_s = MODE == kExpertsOut ? u0 / A.Kt : 0, i_kt = MODE == kExpertsOut ? u0 % A.Kt : u0, i_st = 0;
+    auto issue = [&]() {
+        const int64_t off = (MODE == kExpertsOut ? W.list[i_s] * image : W.w_off) + ((int64_t)i_kt * A.Nt + nt0) * F::kRec;
+        uint8_t *dst = ring + i_st * F::kStage;
+        uint64_t *bar = bars + i_st;
+        mbar_arrive_expect_tx(bar, gated ? 2 * bytes : bytes);
+        bulk_g2s(dst, A.w0 + off, bytes, bar);
+        if (gated) bulk_g2s(dst + F::kStage / 2, A.w1 + off, bytes, bar);
+        i_st = i_st + 1 == S ? 0 : i_st + 1;
+        i_kt++;
+        if (MODE == kExpertsOut && i_kt == A.Kt) {
+            i_kt = 0;
+            i_s++;
+        }
+    };
+    __syncwarp();
+    if (lane == 0)
+        for (int i = 0; i < min(S, n); i++) issue();
+    // The weights were asked for before what the launch in front of this one computes is waited for: it writes activations, never
+    // weights, and what was in front of that one was complete before it let this launch begin.
+    if (MODE != kExpertsIn) griddep_wait();
+    if (MODE == kMatvec) griddep_launch();
+
+    // The tokens' values of one tile row: lane (g, t) holds token g, k = 2t, 2t+1, 2t+8, 2t+9 of both face rows.  Lanes past the
+    // last token read the first one's row: their columns of the product are dropped.
+    const __nv_bfloat16 *xp[NT];
+    uint32_t present[NT];                 // experts-out: all ones where the token has this expert
+    const bool vec = MODE == kExpertsOut || ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 3) == 0;
+    int x_s = i_s, x_kt = 0;
+    auto rows_of = [&]() {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            int tk = SINGLE ? 0 : nt * 8 + g;
+            if (tk >= W.n_tok) tk = 0;
+            present[nt] = ~0u;
+            if (MODE == kMatvec) {
+                xp[nt] = A.x + (int64_t)(W.tok0 + tk) * A.ldx + 2 * t;
+            } else if (MODE == kExpertsIn) {
+                xp[nt] = A.x + (int64_t)(W.list[2 * (W.tok0 + tk)] / A.top) * A.ldx + 2 * t;
+            } else {
+                const int r = W.rows[x_s * tok_pitch + tk];
+                if (r < 0) present[nt] = 0u;
+                xp[nt] = A.h + (int64_t)max(r, 0) * 2 * A.hpad + 2 * t;
+            }
+        }
+    };
+    uint32_t xb[2][PIECES][NT][2], ahead[2][PIECES][NT][2];   // this tile row's, and the next one's on their way
+    auto load_x = [&]() {
+        if (MODE == kExpertsOut && x_kt == A.Kt) {
+            x_kt = 0;
+            x_s++;
+            rows_of();
+        }
+        const int k0 = x_kt * 32;
+        if (MODE == kExpertsOut || (vec && k0 + 32 <= A.K)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int q = 0; q < PIECES; q++) {
+                    const uint32_t *at = reinterpret_cast<const uint32_t *>(xp[nt] + q * A.hpad + k0);
+#pragma unroll
+                    for (int f = 0; f < 2; f++)
+#pragma unroll
+                        for (int p = 0; p < 2; p++) {
+                            if (MODE == kExpertsOut) ahead[f][q][nt][p] = __ldcg(at + f * 8 + p * 4);
+                            else ahead[f][q][nt][p] = at[f * 8 + p * 4];
+                            if (MODE == kExpertsOut && !SINGLE) ahead[f][q][nt][p] &= present[nt];
+                        }
+                }
+        } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) ahead[v >> 1][0][nt][v & 1] = load_pair(xp[nt] - 2 * t, k0 + v * 8 + 2 * t, A.K, vec);
+        }
+        x_kt++;
+    };
+
+    float acc[8][NT][4];
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) acc[j][nt][v] = 0.0f;
+
+    // lane group g reads face column (g >> 1) & 1 of tile (g & 1) + 2 * (g >> 2): neighbours in g are records apart, which
+    // puts the 8 lanes of a 128-bit access in distinct banks
+    const int tile = (g & 1) | ((g >> 2) << 1), fc = (g >> 1) & 1, odd = g & 1;
+    const uint32_t sel_flip = MB == 7 && odd ? 0x4444u : 0u;
+    bool ok = true;
+    int done = 0, st = 0, phase = 0;
+    if (n > 0) {
+        x_kt = MODE == kExpertsOut ? u0 % A.Kt : u0;
+        x_s = MODE == kExpertsOut ? u0 / A.Kt : 0;
+        rows_of();
+        load_x();
+    }
+    for (; done < n; done++) {
+#pragma unroll
+        for (int v = 0; v < 4 * PIECES * NT; v++) (&xb[0][0][0][0])[v] = (&ahead[0][0][0][0])[v];
+        if (done + 1 < n) load_x();
+        ok = mbar_wait_bounded(bars + st, phase, const_cast<int *>(abort_flag), A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint8_t *rec = ring + st * F::kStage + tile * F::kRec;
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+            const int face = 2 * f + fc;
+            Raw<MB> raw;
+            load_raw<MB>(raw, rec + 64 + face * F::kFace, t, odd);
+            uint32_t e[2];
+            e[0] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t);
+            e[1] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t + 8);
+            bool wide = ((e[0] | e[1]) & 0x8080u) != 0;
+            if constexpr (SINGLE) {
+                uint32_t b[PIECES][2], x[PIECES][2];
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    const uint32_t s = scale_pair(e[p], -kDown);
+#pragma unroll
+                    for (int q = 0; q < PIECES; q++) {
+                        x[q][p] = xb[f][q][0][p];
+                        b[q][p] = mul_bf16x2(x[q][p], s);
+                        wide |= not_finite_pair(b[q][p]);
+                    }
+                }
+                if (__any_sync(0xffffffffu, wide)) single_step_wide<MB, PIECES>(acc, raw, e, sel_flip, x);
+                else single_step<MB, PIECES>(acc, raw, sel_flip, b);
+            } else {
+                if (__any_sync(0xffffffffu, wide)) step<MB, NT, PIECES, true>(acc, raw, e, sel_flip, xb[f]);
+                else step<MB, NT, PIECES, false>(acc, raw, e, sel_flip, xb[f]);
+            }
+        }
+        __syncwarp();
+        if (lane == 0 && done + S < n) issue();
+        if (++st == S) {
+            st = 0;
+            phase ^= 1;
+        }
+    }
+    if (!ok)   // a copy that did not arrive in time: let those in flight land before the memory is given up (again bounded)
+        for (int i = done; i < min(n, done + S); i++) {
+            int own = 0;
+            (void)mbar_wait_bounded(bars + i % S, (i / S) & 1, &own, A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
+        }
+    __syncthreads();                      // every warp is done with its ring: the sums take its place
+    float *sums = reinterpret_cast<float *>(smem);
+    if constexpr (SINGLE) {
+        if (t == (g >> 1))
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                *reinterpret_cast<float2 *>(sums + warp * tok_pitch * kPitch + j * 16 + g * 2) =
+                    make_float2(((g & 1) ? acc[j][0][1] : acc[j][0][0]) * (float)(1 << kDown),
+                                ((g & 1) ? acc[j][0][3] : acc[j][0][2]) * (float)(1 << kDown));
+    } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int v = 0; v < 2; v++)
+                if (nt * 8 + 2 * t + v < W.n_tok)
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        *reinterpret_cast<float2 *>(sums + (warp * tok_pitch + nt * 8 + 2 * t + v) * kPitch + j * 16 + g * 2) =
+                            make_float2(acc[j][nt][v], acc[j][nt][2 + v]);
+    }
+    __syncthreads();
+}
+
+// NT: groups of 8 tokens in one pass; 0: one token.
 template <int MB, int NT, int MODE>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) few_rows_kernel(const Args A)
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT, MODE)) few_rows_kernel(const Args A)
 {
     using F = Fmt<MB>;
     using L = Lay<MB, NT>;
-    constexpr int S = F::kStages;
-    constexpr int PIECES = MODE == kExpertsOut ? 2 : 1;
     extern __shared__ __align__(128) uint8_t smem[];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int c = A.cluster;
     const int rank = c > 1 ? (int)cluster_rank() : 0;
     const int group = blockIdx.x / c;
-    uint8_t *ring = smem + warp * S * F::kStage;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars) + warp * S;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars) + warp * F::kStages;
     uint32_t *map = reinterpret_cast<uint32_t *>(smem + L::kMap);
     volatile int *ctl = reinterpret_cast<volatile int *>(smem + L::kCtl);   // [0] abort flag, [1] count
     int *list = reinterpret_cast<int *>(smem + L::kList);
     int16_t *rows = reinterpret_cast<int16_t *>(smem + L::kRows);
 
     if (lane == 0) {
-        for (int i = 0; i < S; i++) mbar_init(bars + i, 1);
+        for (int i = 0; i < F::kStages; i++) mbar_init(bars + i, 1);
         mbar_fence_init();
     }
     if (tid == 0) ctl[0] = 0;
     if (MODE != kMatvec && tid < kMaxExperts / 32) map[tid] = 0;
 
     // ---- which tokens and which matrices
-    int n_tok = 0, units = A.Kt, tok0 = 0;
-    int64_t w_off = 0;
-    const int64_t image = (int64_t)A.Kt * A.Nt * F::kRec;
+    Work W;
+    W.list = list;
+    W.rows = rows;
+    W.units = A.Kt;
+    W.w_off = 0;
+    W.tok0 = blockIdx.y * L::kTok;
     if (MODE == kMatvec) {
         __syncthreads();
-        tok0 = blockIdx.y * L::kTok;
-        n_tok = min(A.rows - tok0, L::kTok);
+        W.n_tok = min(A.rows - W.tok0, L::kTok);
     } else {
-        if (MODE == kExpertsIn) griddep_wait();
+        if (MODE == kExpertsIn) {
+            griddep_wait();
+            griddep_launch();
+            W.tok0 = 0;
+        }
         __syncthreads();
-        tok0 = MODE == kExpertsOut ? blockIdx.y * L::kTok : 0;
-        const int t_end = MODE == kExpertsOut ? min(A.rows, tok0 + L::kTok) : A.rows;
-        for (int i = tok0 * A.top + tid; i < t_end * A.top; i += kThreads) {
+        const int t_end = MODE == kExpertsOut ? min(A.rows, W.tok0 + L::kTok) : A.rows;
+        for (int i = W.tok0 * A.top + tid; i < t_end * A.top; i += kThreads) {
             const int e = __ldcg(A.ids + i);
             if (e >= 0 && e < A.E) atomicOr(&map[e >> 5], 1u << (e & 31));
         }
@@ -275,7 +538,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) few_rows_kernel(con
         int count = 0;
         for (int w = 0; w < kMaxExperts / 32; w++) count += __popc(map[w]);
         if (MODE == kExpertsIn) {
-            griddep_launch();
             if ((int)blockIdx.y >= count) return;      // the whole cluster: it shares blockIdx.y
             int e = 0, left = blockIdx.y;
             for (int w = 0; w < kMaxExperts / 32; w++) {
@@ -283,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) few_rows_kernel(con
                 if (left >= 0 && left < here) e = 32 * w + (int)__fns(map[w], 0, left + 1);
                 left -= here;
             }
-            w_off = e * image;
+            W.w_off = e * ((int64_t)A.Kt * A.Nt * F::kRec);
             if (warp == 0) {                           // the tokens of this expert, in order; a repeated slot adds its weight
                 int found = 0;
                 for (int base = 0; base < A.rows; base += 32) {
@@ -307,11 +569,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) few_rows_kernel(con
                 if (lane == 0) ctl[1] = found;
             }
             __syncthreads();
-            tok0 = blockIdx.z * L::kTok;
-            n_tok = min(ctl[1] - tok0, L::kTok);
-            if (n_tok <= 0) return;                    // the whole cluster here too
+            W.tok0 = blockIdx.z * L::kTok;
+            W.n_tok = min(ctl[1] - W.tok0, L::kTok);
+            if (W.n_tok <= 0) return;                  // the whole cluster here too
         } else {
-            n_tok = t_end - tok0;
+            W.n_tok = t_end - W.tok0;
             if (tid < kMaxExperts) {                   // expert e is number (set bits below e)
                 if (map[tid >> 5] >> (tid & 31) & 1u) {
                     int at = __popc(map[tid >> 5] & ((1u << (tid & 31)) - 1u));
@@ -321,144 +583,33 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) few_rows_kernel(con
             }
             for (int i = tid; i < count * L::kTok; i += kThreads) rows[i] = -1;
             __syncthreads();
-            if (tid < n_tok)
+            if (tid < W.n_tok)
                 for (int s = A.top - 1; s >= 0; s--) {
-                    const int e = __ldcg(A.ids + (tok0 + tid) * A.top + s);
+                    const int e = __ldcg(A.ids + (W.tok0 + tid) * A.top + s);
                     if (e < 0 || e >= A.E) continue;
                     int at = __popc(map[e >> 5] & ((1u << (e & 31)) - 1u));
                     for (int w = 0; w < (e >> 5); w++) at += __popc(map[w]);
-                    rows[at * L::kTok + tid] = (int16_t)((tok0 + tid) * A.top + s);
+                    rows[at * L::kTok + tid] = (int16_t)((W.tok0 + tid) * A.top + s);
                 }
             __syncthreads();
-            units = count * A.Kt;
+            W.units = count * A.Kt;
         }
     }
 
-    // ---- this warp's share of the tile rows, and the copies of one of them
     const int workers = c * kWarps, me = rank * kWarps + warp;
-    const int u0 = (int)((int64_t)units * me / workers), n = (int)((int64_t)units * (me + 1) / workers) - u0;
-    const bool gated = MODE == kExpertsIn && A.w1 != nullptr;
-    const int span = gated ? kGroupTiles / 2 : kGroupTiles;
-    const int nt0 = group * span;
-    const uint32_t bytes = (uint32_t)min(span, A.Nt - nt0) * F::kRec;
-    auto issue = [&](int i) {
-        const int u = u0 + i;
-        int kt = u;
-        int64_t off = w_off;
-        if (MODE == kExpertsOut) {
-            const int s = u / A.Kt;
-            kt = u - s * A.Kt;
-            off = list[s] * image;
-        }
-        off += ((int64_t)kt * A.Nt + nt0) * F::kRec;
-        uint8_t *dst = ring + (i % S) * F::kStage;
-        uint64_t *bar = bars + i % S;
-        mbar_arrive_expect_tx(bar, gated ? 2 * bytes : bytes);
-        bulk_g2s(dst, A.w0 + off, bytes, bar);
-        if (gated) bulk_g2s(dst + F::kStage / 2, A.w1 + off, bytes, bar);
-    };
-    __syncwarp();
-    if (lane == 0)
-        for (int i = 0; i < min(S, n); i++) issue(i);
-    if (MODE == kExpertsOut) griddep_wait();           // h is complete; the weights were asked for before it was
-
-    // ---- the tokens' values of one tile row: lane (g, t) holds token g, k = 2t, 2t+1, 2t+8, 2t+9 of both face rows
-    const __nv_bfloat16 *xrow[NT];
-    bool vec = true;
-    auto row_of = [&](int nt, int u) -> const __nv_bfloat16 * {
-        const int tk = nt * 8 + g;
-        if (tk >= n_tok) return nullptr;
-        if (MODE == kMatvec) return A.x + (int64_t)(tok0 + tk) * A.ldx;
-        if (MODE == kExpertsIn) return A.x + (int64_t)(list[2 * (tok0 + tk)] / A.top) * A.ldx;
-        const int r = rows[(u / A.Kt) * L::kTok + tk];
-        return r < 0 ? nullptr : A.h + (int64_t)r * 2 * A.hpad;
-    };
-    if (MODE != kExpertsOut) {
-        vec = ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 3) == 0;
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) xrow[nt] = row_of(nt, 0);
+    if constexpr (NT == 0) {
+        products<MB, 1, MODE, true>(A, W, smem, bars, &ctl[0], group, me, workers, 1);
+    } else if constexpr (MODE == kExpertsIn) {
+        if (W.n_tok == 1) products<MB, 1, MODE, true>(A, W, smem, bars, &ctl[0], group, me, workers, L::kTok);
+        else products<MB, NT, MODE, false>(A, W, smem, bars, &ctl[0], group, me, workers, L::kTok);
+    } else {
+        products<MB, NT, MODE, false>(A, W, smem, bars, &ctl[0], group, me, workers, L::kTok);
     }
-    uint32_t xb[2][PIECES][NT][2], ahead[2][PIECES][NT][2];   // this tile row's, and the next one's on their way
-    auto load_x = [&](uint32_t (&xb)[2][PIECES][NT][2], int i) {
-        const int u = u0 + i;
-        const int kt = MODE == kExpertsOut ? u % A.Kt : u;
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            if (MODE == kExpertsOut) xrow[nt] = row_of(nt, u);
-#pragma unroll
-            for (int q = 0; q < PIECES; q++)
-#pragma unroll
-                for (int f = 0; f < 2; f++)
-#pragma unroll
-                    for (int p = 0; p < 2; p++) {
-                        const int k = kt * 32 + f * 16 + p * 8 + 2 * t;
-                        if (MODE == kExpertsOut)
-                            xb[f][q][nt][p] = xrow[nt] ? __ldcg(reinterpret_cast<const uint32_t *>(xrow[nt] + q * A.hpad + k)) : 0u;
-                        else
-                            xb[f][q][nt][p] = load_pair(xrow[nt], k, A.K, vec);
-                    }
-        }
-    };
 
-    float acc[8][NT][4];
-#pragma unroll
-    for (int j = 0; j < 8; j++)
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int v = 0; v < 4; v++) acc[j][nt][v] = 0.0f;
-
-    // lane group g reads face column (g >> 1) & 1 of tile (g & 1) + 2 * (g >> 2): neighbours in g are records apart, which
-    // puts the 8 lanes of a 128-bit access in distinct banks
-    const int tile = (g & 1) | ((g >> 2) << 1), fc = (g >> 1) & 1, odd = g & 1;
-    const uint32_t sel_flip = MB == 7 && odd ? 0x4444u : 0u;
-    bool ok = true;
-    int done = 0;
-    if (n > 0) load_x(ahead, 0);
-    for (; done < n; done++) {
-#pragma unroll
-        for (int v = 0; v < 4 * PIECES * NT; v++) (&xb[0][0][0][0])[v] = (&ahead[0][0][0][0])[v];
-        if (done + 1 < n) load_x(ahead, done + 1);
-        ok = mbar_wait_bounded(bars + done % S, (done / S) & 1, const_cast<int *>(&ctl[0]), A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint8_t *rec = ring + (done % S) * F::kStage + tile * F::kRec;
-#pragma unroll
-        for (int f = 0; f < 2; f++) {
-            const int face = 2 * f + fc;
-            Raw<MB> raw;
-            load_raw<MB>(raw, rec + 64 + face * F::kFace, t, odd);
-            uint32_t e[2];
-            e[0] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t);
-            e[1] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t + 8);
-            if (__any_sync(0xffffffffu, ((e[0] | e[1]) & 0x8080u) != 0))
-                step<MB, NT, PIECES, true>(acc, raw, e, sel_flip, xb[f]);
-            else
-                step<MB, NT, PIECES, false>(acc, raw, e, sel_flip, xb[f]);
-        }
-        __syncwarp();
-        if (lane == 0 && done + S < n) issue(done + S);
-    }
-    if (!ok)   // a copy that did not arrive in time: let those in flight land before the memory is given up (again bounded)
-        for (int i = done; i < min(n, done + S); i++) {
-            int own = 0;
-            (void)mbar_wait_bounded(bars + i % S, (i / S) & 1, &own, A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
-        }
-
-    // ---- join the warps: sums[warp][token][j][g][2]
-    __syncthreads();
-    float *sums = reinterpret_cast<float *>(smem);
-#pragma unroll
-    for (int j = 0; j < 8; j++)
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int v = 0; v < 2; v++)
-                *reinterpret_cast<float2 *>(sums + (warp * L::kTok + nt * 8 + 2 * t + v) * kPitch + j * 16 + g * 2) =
-                    make_float2(acc[j][nt][v], acc[j][nt][2 + v]);
-    __syncthreads();
+    // ---- join the warps
+    const float *sums = reinterpret_cast<const float *>(smem);
     float *part = reinterpret_cast<float *>(smem + L::kPart);
-    for (int i = tid; i < n_tok * 64; i += kThreads) {
+    for (int i = tid; i < W.n_tok * 64; i += kThreads) {
         const int tk = i >> 6, q = i & 63;
         float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -483,18 +634,20 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) few_rows_kernel(con
         }
         return s;
     };
-    const int per_tok = gated ? 32 : 64, items = n_tok * per_tok;
+    const bool gated = MODE == kExpertsIn && A.w1 != nullptr;
+    const int col0 = group * (gated ? kGroupTiles / 2 : kGroupTiles) * 32;
+    const int per_tok = gated ? 32 : 64, items = W.n_tok * per_tok;
     for (int i = rank * kThreads + tid; i < items; i += c * kThreads) {
-        const int tk = i / per_tok, r = i % per_tok;
+        const int tk = gated ? i >> 5 : i >> 6, r = i & (per_tok - 1);
         const int j = gated ? r >> 2 : r >> 3, gg = gated ? r & 3 : r & 7, q = j * 8 + gg;
-        const int col = nt0 * 32 + ((gg & 1) | ((gg >> 2) << 1)) * 32 + ((gg >> 1) & 1) * 16 + 2 * j;
+        const int col = col0 + ((gg & 1) | ((gg >> 2) << 1)) * 32 + ((gg >> 1) & 1) * 16 + 2 * j;
         float2 v = total(tk, q);
         if (MODE == kExpertsIn) {
             float2 up = make_float2(1.0f, 1.0f);
             if (gated) up = total(tk, q + 4);
-            const float w = __int_as_float(list[2 * (tok0 + tk) + 1]);
+            const float w = __int_as_float(list[2 * (W.tok0 + tk) + 1]);
             float r2[2] = {activate(v.x, A.act) * up.x * w, activate(v.y, A.act) * up.y * w};
-            __nv_bfloat16 *h = A.h + (int64_t)list[2 * (tok0 + tk)] * 2 * A.hpad;
+            __nv_bfloat16 *h = A.h + (int64_t)list[2 * (W.tok0 + tk)] * 2 * A.hpad;
             if (col < A.hpad) {
                 uint32_t hi = 0, lo = 0;
 #pragma unroll
@@ -511,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) few_rows_kernel(con
                 *reinterpret_cast<uint32_t *>(h + A.hpad + col) = lo;
             }
         } else {
-            const int64_t at = (int64_t)(tok0 + tk) * A.ldo + col;
+            const int64_t at = (int64_t)(W.tok0 + tk) * A.ldo + col;
 #pragma unroll
             for (int b = 0; b < 2; b++)
                 if (col + b < A.N) {
@@ -524,42 +677,50 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) few_rows_kernel(con
     if (c > 1) cluster_sync();       // no CTA leaves while another reads its sums
 }
 
+// Every launch may begin before the one in front of it is done (it waits for that one before it reads activations or ids, and
+// before it writes).  Only launches that say so let it: those of this file and of the router.
 template <int MB, int NT, int MODE>
-cudaError_t launch_one(const Args &a, dim3 grid, bool dependent, cudaStream_t stream)
+cudaError_t launch_one(const Args &a, dim3 grid, cudaStream_t stream)
 {
-    using L = Lay<MB, NT>;
-    const int bytes = MODE == kExpertsOut ? L::kBytesOut : L::kBytesIn;
-    cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<MB, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    constexpr int bytes = Lay<MB, NT>::kBytes(MODE);
+    static std::atomic<uint64_t> ready{0};      // devices whose kernel may take this much shared memory
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
+        e = cudaFuncSetAttribute(few_rows_kernel<MB, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = stream;
     cudaLaunchAttribute at[2];
-    int n = 0;
-    if (a.cluster > 1) {
-        at[n].id = cudaLaunchAttributeClusterDimension;
-        at[n].val.clusterDim.x = a.cluster;
-        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
-        n++;
-    }
-    if (dependent) {
-        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[n].val.programmaticStreamSerializationAllowed = 1;
-        n++;
-    }
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = a.cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = n;
+    cfg.numAttrs = a.cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, few_rows_kernel<MB, NT, MODE>, a);
 }
 
+int passes_of(int rows) { return rows <= 32 ? 1 : (rows + 31) / 32; }
+int groups_of_8(int rows) { return rows == 1 ? 0 : rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+
 template <int MODE>
-cudaError_t dispatch(int mant_bits, int tokens, const Args &a, dim3 grid, bool dependent, cudaStream_t stream)
+cudaError_t dispatch(int mant_bits, int nt, const Args &a, dim3 grid, cudaStream_t stream)
 {
-#define BUDA_FEW(MB)                                                                                    \
-    return tokens <= 8 ? launch_one<MB, 1, MODE>(a, grid, dependent, stream)                            \
-                       : launch_one<MB, 2, MODE>(a, grid, dependent, stream)
+#define BUDA_FEW(MB)                                              \
+    switch (nt) {                                                 \
+        case 0: return launch_one<MB, 0, MODE>(a, grid, stream);  \
+        case 1: return launch_one<MB, 1, MODE>(a, grid, stream);  \
+        case 2: return launch_one<MB, 2, MODE>(a, grid, stream);  \
+        default: return launch_one<MB, 4, MODE>(a, grid, stream); \
+    }
     switch (mant_bits) {
         case 7: BUDA_FEW(7);
         case 3: BUDA_FEW(3);
@@ -577,8 +738,6 @@ int split_of(int64_t groups, int64_t tile_rows, int sm_count, int per_sm)
     return c;
 }
 
-int tokens_per_pass(int rows) { return rows <= 8 ? 8 : 16; }
-
 }  // namespace few
 
 using namespace few;
@@ -592,16 +751,16 @@ cudaError_t launch_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, 
     a.w0 = (const uint8_t *)W;
     a.out = Y; a.ldo = ldy; a.out_f32 = out_f32;
     a.status = status;
-    const int tok = tokens_per_pass(a.rows), groups = (a.Nt + kGroupTiles - 1) / kGroupTiles, passes = (a.rows + tok - 1) / tok;
-    a.cluster = split_of((int64_t)groups * passes, a.Kt, sm_count, tok == 8 ? 2 : 1);
-    return dispatch<kMatvec>(mant_bits, a.rows, a, dim3(groups * a.cluster, passes), false, stream);
+    const int nt = groups_of_8(a.rows), groups = (a.Nt + kGroupTiles - 1) / kGroupTiles, passes = passes_of(a.rows);
+    a.cluster = split_of((int64_t)groups * passes, a.Kt, sm_count, ctas_per_sm(nt, kMatvec));
+    return dispatch<kMatvec>(mant_bits, nt, a, dim3(groups * a.cluster, passes), stream);
 }
 
-cudaError_t launch_moe_experts(const MoeArgs &m, bool dependent, int sm_count, cudaStream_t stream, unsigned int *status)
+cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stream, unsigned int *status)
 {
-    const int tok = tokens_per_pass(m.T), passes = (m.T + tok - 1) / tok;
+    const int nt = groups_of_8(m.T), passes = passes_of(m.T);
     const int Ht = (m.H + 31) / 32, It = (m.I + 31) / 32;
-    const int most = m.E < m.T * m.top ? m.E : m.T * m.top;
+    const int slots = m.T * m.top, most = m.E < slots ? m.E : slots;
     Args a = {};
     a.x = (const __nv_bfloat16 *)m.x; a.ldx = m.ldx;
     a.rows = m.T; a.K = m.H; a.Kt = Ht; a.N = m.I; a.Nt = It;
@@ -610,15 +769,15 @@ cudaError_t launch_moe_experts(const MoeArgs &m, bool dependent, int sm_count, c
     a.h = (__nv_bfloat16 *)m.h; a.hpad = 32 * It;
     a.status = status;
     const int span = m.up ? kGroupTiles / 2 : kGroupTiles, groups = (It + span - 1) / span;
-    a.cluster = split_of((int64_t)groups * most, Ht, sm_count, tok == 8 ? 2 : 1);
-    cudaError_t e = dispatch<kExpertsIn>(m.mant_bits, m.T, a, dim3(groups * a.cluster, most, passes), dependent, stream);
+    a.cluster = split_of((int64_t)groups * most, Ht, sm_count, ctas_per_sm(nt, kExpertsIn));
+    cudaError_t e = dispatch<kExpertsIn>(m.mant_bits, nt, a, dim3(groups * a.cluster, most, passes), stream);
     if (e != cudaSuccess) return e;
     a.K = m.I; a.Kt = It; a.N = m.H; a.Nt = Ht;
     a.w0 = (const uint8_t *)m.down; a.w1 = nullptr;
     a.out = m.y; a.ldo = m.ldy; a.out_f32 = 0;
     const int groups2 = (Ht + kGroupTiles - 1) / kGroupTiles;
-    a.cluster = split_of((int64_t)groups2 * passes, (int64_t)It, sm_count, tok == 8 ? 2 : 1);
-    return dispatch<kExpertsOut>(m.mant_bits, m.T, a, dim3(groups2 * a.cluster, passes), true, stream);
+    a.cluster = split_of((int64_t)groups2 * passes, (int64_t)It * most, sm_count, ctas_per_sm(nt, kExpertsOut));
+    return dispatch<kExpertsOut>(m.mant_bits, nt, a, dim3(groups2 * a.cluster, passes), stream);
 }
 
 }  // namespace buda

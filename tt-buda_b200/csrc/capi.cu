@@ -45,7 +45,7 @@ cudaError_t launch_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, 
                               int out_f32, int sm_count, cudaStream_t stream, unsigned int *status);
 cudaError_t launch_moe_route(const void *x, int64_t ldx, int T, int H, const void *w, int w_f32, int64_t ldw, int E, int top, int renorm,
                              float *weights, int *ids, int sm_count, cudaStream_t stream);
-cudaError_t launch_moe_experts(const MoeArgs &m, bool dependent, int sm_count, cudaStream_t stream, unsigned int *status);
+cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stream, unsigned int *status);
 
 // One CTA, one thread waiting: the barrier expects one arrival that never comes.  The other 31 lanes only take part in
 // the final warp convergence.  The wait is the product kernels' own mbar_wait_bounded with a caller-given limit.
@@ -1444,7 +1444,7 @@ static int check_experts(const void *X, int64_t T, int64_t H, int64_t ldx, const
 
 static int run_experts(DevCtx *ctx, const void *X, int64_t T, int64_t H, int64_t ldx, const float *weights, const int32_t *ids, int top,
                        const void *gate, const void *up, const void *down, int64_t E, int64_t I, int w_df, int act, void *Y, int64_t ldy,
-                       void *workspace, bool after_route, void *stream)
+                       void *workspace, void *stream)
 {
     MoeArgs m;
     m.x = X; m.ldx = ldx;
@@ -1453,7 +1453,7 @@ static int run_experts(DevCtx *ctx, const void *X, int64_t T, int64_t H, int64_t
     m.weights = weights; m.ids = ids;
     m.gate = gate; m.up = up; m.down = down;
     m.y = Y; m.ldy = ldy; m.h = workspace;
-    cudaError_t e = launch_moe_experts(m, after_route, ctx->sm_count, (cudaStream_t)stream, ctx->status);
+    cudaError_t e = launch_moe_experts(m, ctx->sm_count, (cudaStream_t)stream, ctx->status);
     if (e != cudaSuccess) return cuda_fail(e, "moe_experts launch failed");
     g_launches.fetch_add(2, std::memory_order_relaxed);
     return BUDA_SUCCESS;
@@ -1467,7 +1467,7 @@ int buda_moe_experts(const void *X, int64_t T, int64_t H, int64_t ldx, const flo
     if (int rc = get_ctx(&ctx)) return rc;
     if (int rc = check_experts(X, T, H, ldx, weights, ids, top, gate, up, down, E, I, w_df, act, Y, ldy, workspace, workspace_bytes)) return rc;
     if (T == 0) return BUDA_SUCCESS;
-    return run_experts(ctx, X, T, H, ldx, weights, ids, top, gate, up, down, E, I, w_df, act, Y, ldy, workspace, false, stream);
+    return run_experts(ctx, X, T, H, ldx, weights, ids, top, gate, up, down, E, I, w_df, act, Y, ldy, workspace, stream);
 }
 
 int buda_moe_layer(const void *X, int64_t T, int64_t H, int64_t ldx, const void *W_router, int router_df, int64_t ldw, int top,
@@ -1480,7 +1480,7 @@ int buda_moe_layer(const void *X, int64_t T, int64_t H, int64_t ldx, const void 
     if (int rc = check_experts(X, T, H, ldx, weights, ids, top, gate, up, down, E, I, w_df, act, Y, ldy, workspace, workspace_bytes)) return rc;
     if (T == 0) return BUDA_SUCCESS;
     if (int rc = buda_moe_route(X, T, H, ldx, W_router, router_df, ldw, E, top, renormalize, weights, ids, stream)) return rc;
-    return run_experts(ctx, X, T, H, ldx, weights, ids, top, gate, up, down, E, I, w_df, act, Y, ldy, workspace, true, stream);
+    return run_experts(ctx, X, T, H, ldx, weights, ids, top, gate, up, down, E, I, w_df, act, Y, ldy, workspace, stream);
 }
 
 int buda_prestride(const void *src, int elem_bytes, const uint32_t shape[4], const uint64_t strides_bytes[4], int stride,

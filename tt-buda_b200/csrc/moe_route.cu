@@ -17,7 +17,7 @@ namespace buda {
 namespace route {
 
 constexpr int kCluster = 8;
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kPerCta = kMaxExperts / kCluster;
 
@@ -35,33 +35,57 @@ __device__ __forceinline__ double ld_cluster_f64(const double *p, uint32_t rank)
     return v;
 }
 
-// Eight consecutive values of a row as binary32; `vec`: 16-byte loads are allowed.  Zero past H.
-__device__ __forceinline__ void load8(float (&v)[8], const __nv_bfloat16 *row, int h, int H, bool vec)
-{
-    if (vec && h + 8 <= H) {
-        const uint4 r = *reinterpret_cast<const uint4 *>(row + h);
+// Eight consecutive values of a row, fetched (16-byte loads where `vec`, zero past H) and turned into binary32 later, so that
+// many rows' loads are under way before the first is used.
+template <typename T>
+struct Octet;
+template <>
+struct Octet<__nv_bfloat16> {
+    uint4 r;
+    __device__ __forceinline__ void load(const __nv_bfloat16 *row, int h, int H, bool vec)
+    {
+        if (vec && h + 8 <= H) {
+            r = *reinterpret_cast<const uint4 *>(row + h);
+            return;
+        }
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
+        uint32_t u[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) u[i] = h + i < H ? p[h + i] : 0u;
+        r = make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const
+    {
         const uint32_t u[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             v[2 * i] = __uint_as_float(u[i] << 16);
             v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = h + i < H ? __bfloat162float(row[h + i]) : 0.0f;
     }
-}
-__device__ __forceinline__ void load8(float (&v)[8], const float *row, int h, int H, bool vec)
-{
-    if (vec && h + 8 <= H) {
-        const float4 a = *reinterpret_cast<const float4 *>(row + h), b = *reinterpret_cast<const float4 *>(row + h + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
+};
+template <>
+struct Octet<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float *row, int h, int H, bool vec)
+    {
+        if (vec && h + 8 <= H) {
+            a = *reinterpret_cast<const float4 *>(row + h);
+            b = *reinterpret_cast<const float4 *>(row + h + 4);
+            return;
+        }
+        float v[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = h + i < H ? row[h + i] : 0.0f;
+        a = make_float4(v[0], v[1], v[2], v[3]);
+        b = make_float4(v[4], v[5], v[6], v[7]);
     }
-}
+    __device__ __forceinline__ void get(float (&v)[8]) const
+    {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+};
 
 // Binary64 in an order that unsigned integers have: NaN below every number, 0 for "already chosen".
 __device__ __forceinline__ uint64_t order_of(double l)
@@ -72,12 +96,13 @@ __device__ __forceinline__ uint64_t order_of(double l)
 }
 
 template <typename TW, int TB>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1)
     route_kernel(const __nv_bfloat16 *x, int64_t ldx, int T, int H, const TW *w, int64_t ldw, int E, int top, int renorm, int split,
                  float *weights, int *ids)
 {
     __shared__ double part[kPerCta * TB * kWarps];      // [expert of this CTA][token][piece of the row]
     __shared__ double score[kPerCta * TB];
+    asm volatile("griddepcontrol.wait;" ::: "memory");                // x may come from the launch in front of this one
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t rank;
@@ -94,19 +119,29 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
         double s[TB];
 #pragma unroll
         for (int i = 0; i < TB; i++) s[i] = 0.0;
-#pragma unroll 4
-        for (int o = (int)((int64_t)octets * piece / split) + lane; o < o1; o += 32) {
-            float a[8];
-            load8(a, row, o * 8, H, wvec);
+        constexpr int kBatch = 4;       // octets of a row on their way at once
+        for (int o = (int)((int64_t)octets * piece / split) + lane; o < o1; o += 32 * kBatch) {
+            Octet<TW> a[kBatch];
+            Octet<__nv_bfloat16> b[kBatch][TB];
 #pragma unroll
-            for (int i = 0; i < TB; i++) {
-                if (i >= nt) break;
-                float b[8];
-                load8(b, x + (int64_t)(t0 + i) * ldx, o * 8, H, xvec);
-                float p = 0.0f;
+            for (int u = 0; u < kBatch; u++) {
+                const int h = o + 32 * u < o1 ? (o + 32 * u) * 8 : H;
+                a[u].load(row, h, H, wvec);
 #pragma unroll
-                for (int v = 0; v < 8; v++) p = fmaf(a[v], b[v], p);
-                s[i] += (double)p;
+                for (int i = 0; i < TB; i++) b[u][i].load(x + (int64_t)(t0 + min(i, nt - 1)) * ldx, h, H, xvec);
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; u++) {
+                float av[8];
+                a[u].get(av);
+#pragma unroll
+                for (int i = 0; i < TB; i++) {
+                    float bv[8], p = 0.0f;
+                    b[u][i].get(bv);
+#pragma unroll
+                    for (int v = 0; v < 8; v++) p = fmaf(av[v], bv[v], p);
+                    s[i] += (double)p;
+                }
             }
         }
 #pragma unroll
@@ -190,15 +225,17 @@ cudaError_t launch_tw(const void *x, int64_t ldx, int T, int H, const void *w, i
     const int most = (E + kCluster - 1) / kCluster;
     int split = 1;
     while (split < kWarps && split * 2 * most <= kWarps) split *= 2;
-    const dim3 grid((unsigned)((T + tb - 1) / tb * kCluster));
-#define BUDA_ROUTE(TB)                                                                                                        \
-    route_kernel<TW, TB><<<grid, kThreads, 0, stream>>>((const __nv_bfloat16 *)x, ldx, T, H, (const TW *)w, ldw, E, top, renorm, \
-                                                        split, weights, ids)
-    if (tb == 1) BUDA_ROUTE(1);
-    else if (tb == 2) BUDA_ROUTE(2);
-    else BUDA_ROUTE(4);
-#undef BUDA_ROUTE
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((T + tb - 1) / tb * kCluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;     // begins while the launch in front of it ends, if that one lets it
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    auto kernel = tb == 1 ? route_kernel<TW, 1> : tb == 2 ? route_kernel<TW, 2> : route_kernel<TW, 4>;
+    return cudaLaunchKernelEx(&cfg, kernel, (const __nv_bfloat16 *)x, ldx, T, H, (const TW *)w, ldw, E, top, renorm, split, weights, ids);
 }
 
 }  // namespace route

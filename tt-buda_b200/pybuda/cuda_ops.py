@@ -4,7 +4,6 @@ torch is used for device memory and streams only; every byte of arithmetic happe
 libbuda_cuda.so (hand-written sm_100a kernels) reached through its C ABI.  Functions raise if
 the tensor is not on a CUDA device: there is no CPU path here.
 """
-import contextlib
 import ctypes
 import enum
 
@@ -240,11 +239,17 @@ def _output(what, out, x, rows, cols, dtype):
     return out
 
 
-def _on(device):
-    """The current stream of the tensors' device as an address, and what makes that device current for the call."""
-    i = device.index
-    guard = contextlib.nullcontext() if i == torch.cuda.current_device() else torch.cuda.device(i)
-    return torch.cuda.current_stream(device).cuda_stream, guard
+def _launch(device, entry, *args):
+    """One C call on the current stream of `device`, whichever device is current.  (torch.cuda.current_stream() builds a Stream
+    object: 4 us, half of what a few-row call costs on the host.)"""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if device.index == torch.cuda.current_device():
+        rc = entry(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args, stream)
+    if rc:
+        check(rc)
 
 
 def bfp_matvec(a, w_image, n, w_df=DF.Bfp4_b, out=None, out_dtype=torch.bfloat16):
@@ -261,10 +266,8 @@ def bfp_matvec(a, w_image, n, w_df=DF.Bfp4_b, out=None, out_dtype=torch.bfloat16
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise RuntimeError("bfp_matvec: the output is bfloat16 or float32")
     out = _output("bfp_matvec", out, a, m, n, out_dtype)
-    stream, guard = _on(a.device)
-    with guard:
-        check(_cabi.lib.buda_bfp_matvec(a.data_ptr(), m, k, a.stride(0), w_image.data_ptr(), n, w_df, out.data_ptr(), out.stride(0),
-                                        5 if out_dtype == torch.bfloat16 else 0, stream))
+    _launch(a.device, _cabi.lib.buda_bfp_matvec, a.data_ptr(), m, k, a.stride(0), w_image.data_ptr(), n, w_df, out.data_ptr(),
+            out.stride(0), 5 if out_dtype == torch.bfloat16 else 0)
     return out
 
 
@@ -287,11 +290,8 @@ def moe_route(x, w_router, top, renormalize=True):
     t, e = x.shape[0], w_router.shape[0]
     weights = torch.empty((t, max(int(top), 0)), dtype=torch.float32, device=x.device)
     ids = torch.empty(weights.shape, dtype=torch.int32, device=x.device)
-    stream, guard = _on(x.device)
-    with guard:
-        check(_cabi.lib.buda_moe_route(x.data_ptr(), t, x.shape[1], x.stride(0), w_router.data_ptr(),
-                                       5 if w_router.dtype == torch.bfloat16 else 0, w_router.stride(0), e, top, renormalize,
-                                       weights.data_ptr(), ids.data_ptr(), stream))
+    _launch(x.device, _cabi.lib.buda_moe_route, x.data_ptr(), t, x.shape[1], x.stride(0), w_router.data_ptr(),
+            5 if w_router.dtype == torch.bfloat16 else 0, w_router.stride(0), e, top, renormalize, weights.data_ptr(), ids.data_ptr())
     return weights, ids
 
 
@@ -309,11 +309,11 @@ def _experts_check(x, gate, up, down, inter, w_df, activation):
     return experts
 
 
-def _workspace(x, top, inter):
+def _workspace(x, top, inter, more=0):
     nbytes = _cabi.lib.buda_moe_workspace_bytes(x.shape[0], top, inter)
     if nbytes < 0:
         raise _cabi.BudaError(_cabi.RUNTIME_ERROR, _cabi.last_error())
-    return torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    return torch.empty(nbytes + more, dtype=torch.uint8, device=x.device)
 
 
 def moe_experts(x, weights, ids, gate, up, down, inter, w_df=DF.Bfp4_b, activation="silu", out=None):
@@ -332,12 +332,10 @@ def moe_experts(x, weights, ids, gate, up, down, inter, w_df=DF.Bfp4_b, activati
         raise RuntimeError(f"moe_experts: ids (int32) and weights (float32) are contiguous [{t}, top] tensors on {x.device}")
     top = ids.shape[1]
     out = _output("moe_experts", out, x, t, hidden, torch.bfloat16)
-    stream, guard = _on(x.device)
-    with guard:
-        ws = _workspace(x, top, inter)
-        check(_cabi.lib.buda_moe_experts(x.data_ptr(), t, hidden, x.stride(0), weights.data_ptr(), ids.data_ptr(), top, gate.data_ptr(),
-                                         None if up is None else up.data_ptr(), down.data_ptr(), experts, inter, w_df,
-                                         _ACTIVATIONS[activation], out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(), stream))
+    ws = _workspace(x, top, inter)
+    _launch(x.device, _cabi.lib.buda_moe_experts, x.data_ptr(), t, hidden, x.stride(0), weights.data_ptr(), ids.data_ptr(), top,
+            gate.data_ptr(), None if up is None else up.data_ptr(), down.data_ptr(), experts, inter, w_df, _ACTIVATIONS[activation],
+            out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel())
     return out
 
 
@@ -350,15 +348,12 @@ def moe_layer(x, w_router, top, gate, up, down, inter, w_df=DF.Bfp4_b, activatio
         raise RuntimeError(f"moe_layer: the router has {w_router.shape[0]} rows for {experts} experts")
     t, hidden = x.shape
     out = _output("moe_layer", out, x, t, hidden, torch.bfloat16)
-    stream, guard = _on(x.device)
-    with guard:
-        ws = _workspace(x, top, inter)
-        choice = torch.empty((2, t, top), dtype=torch.int32, device=x.device)    # ids, then the weights' bits
-        check(_cabi.lib.buda_moe_layer(x.data_ptr(), t, hidden, x.stride(0), w_router.data_ptr(),
-                                       5 if w_router.dtype == torch.bfloat16 else 0, w_router.stride(0), top, renormalize, gate.data_ptr(),
-                                       None if up is None else up.data_ptr(), down.data_ptr(), experts, inter, w_df,
-                                       _ACTIVATIONS[activation], choice.data_ptr() + 4 * t * top, choice.data_ptr(), out.data_ptr(),
-                                       out.stride(0), ws.data_ptr(), ws.numel(), stream))
+    ws = _workspace(x, top, inter, 8 * t * top)      # the choice (weights, ids) behind the intermediate rows
+    choice = ws.data_ptr() + ws.numel() - 8 * t * top
+    _launch(x.device, _cabi.lib.buda_moe_layer, x.data_ptr(), t, hidden, x.stride(0), w_router.data_ptr(),
+            5 if w_router.dtype == torch.bfloat16 else 0, w_router.stride(0), top, renormalize, gate.data_ptr(),
+            None if up is None else up.data_ptr(), down.data_ptr(), experts, inter, w_df, _ACTIVATIONS[activation], choice,
+            choice + 4 * t * top, out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel())
     return out
 
 
