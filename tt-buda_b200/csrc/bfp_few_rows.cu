@@ -26,6 +26,7 @@
 #include <cuda_bf16.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "few_rows.cuh"
 
@@ -40,8 +41,12 @@ constexpr int kDown = 24;               // single-token sums are held times 2^-2
 
 enum { kMatvec = 0, kExpertsIn = 1, kExpertsOut = 2 };
 
-// CTAs that an SM holds, by registers: 80 suffice for one token (but for the two pieces of experts-out), 128 for up to 16 tokens
-__host__ __device__ constexpr int ctas_per_sm(int nt, int mode) { return nt == 0 && mode != kExpertsOut ? 3 : nt <= 2 ? 2 : 1; }
+// CTAs that an SM holds, by registers: 80 suffice for one token (but for 8-bit data and the two pieces of experts-out), 128 for
+// up to 16 tokens
+__host__ __device__ constexpr int ctas_per_sm(int mb, int nt, int mode)
+{
+    return nt == 0 && mb != 7 && mode != kExpertsOut ? 3 : nt <= 2 ? 2 : 1;
+}
 
 template <int MB>
 struct Fmt {
@@ -49,7 +54,7 @@ struct Fmt {
     static constexpr int kFace = 16 * kRow;
     static constexpr int kRec = 64 + 4 * kFace;
     static constexpr int kStage = kGroupTiles * kRec;
-    static constexpr int kStages = MB == 7 ? 2 : MB == 3 ? 4 : 7;   // about 72 KB of rings: three CTAs fit an SM
+    static constexpr int kStages = MB == 7 ? 3 : MB == 3 ? 4 : 7;   // 72 KB of rings: three CTAs fit an SM; 8-bit data: 102 KB, two
 };
 
 struct Args {
@@ -311,160 +316,192 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     constexpr int PIECES = MODE == kExpertsOut ? 2 : 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint8_t *ring = smem + warp * S * F::kStage;
-    const int64_t image = (int64_t)A.Kt * A.Nt * F::kRec;
+    const int64_t image = (int64_t)A.Kt * A.Nt * F::kRec, row_bytes = (int64_t)A.Nt * F::kRec;
     const int u0 = (int)((int64_t)W.units * me / workers), n = (int)((int64_t)W.units * (me + 1) / workers) - u0;
+    const int s0 = MODE == kExpertsOut ? u0 / A.Kt : 0, kt0 = u0 - s0 * A.Kt;
     const bool gated = MODE == kExpertsIn && A.w1 != nullptr;
     const int span = gated ? kGroupTiles / 2 : kGroupTiles;
-    const int nt0 = group * span;
-    const uint32_t bytes = (uint32_t)min(span, A.Nt - nt0) * F::kRec;
+    const int64_t col_off = (int64_t)group * span * F::kRec;
+    const uint32_t bytes = (uint32_t)min(span, A.Nt - group * span) * F::kRec;
 
-    // the copies of the warp's next tile row: (i_s, i_kt) and the ring stage advance with every call
-    int i_s = MODE == kExpertsOut ? u0 / A.Kt : 0, i_kt = MODE == kExpertsOut ? u0 % A.Kt : u0, i_st = 0;
-    auto issue = [&]() {
-        const int64_t off = (MODE == kExpertsOut ? W.list[i_s] * image : W.w_off) + ((int64_t)i_kt * A.Nt + nt0) * F::kRec;
-        uint8_t *dst = ring + i_st * F::kStage;
-        uint64_t *bar = bars + i_st;
-        mbar_arrive_expect_tx(bar, gated ? 2 * bytes : bytes);
-        bulk_g2s(dst, A.w0 + off, bytes, bar);
-        if (gated) bulk_g2s(dst + F::kStage / 2, A.w1 + off, bytes, bar);
-        i_st = i_st + 1 == S ? 0 : i_st + 1;
-        i_kt++;
-        if (MODE == kExpertsOut && i_kt == A.Kt) {
-            i_kt = 0;
-            i_s++;
-        }
-    };
-    __syncwarp();
-    if (lane == 0)
-        for (int i = 0; i < min(S, n); i++) issue();
-    // The weights were asked for before what the launch in front of this one computes is waited for: it writes activations, never
-    // weights, and what was in front of that one was complete before it let this launch begin.
-    if (MODE != kExpertsIn) griddep_wait();
-    if (MODE == kMatvec) griddep_launch();
-
-    // The tokens' values of one tile row: lane (g, t) holds token g, k = 2t, 2t+1, 2t+8, 2t+9 of both face rows.  Lanes past the
-    // last token read the first one's row: their columns of the product are dropped.
-    const __nv_bfloat16 *xp[NT];
-    uint32_t present[NT];                 // experts-out: all ones where the token has this expert
     const bool vec = MODE == kExpertsOut || ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 3) == 0;
-    int x_s = i_s, x_kt = 0;
-    auto rows_of = [&]() {
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            int tk = SINGLE ? 0 : nt * 8 + g;
-            if (tk >= W.n_tok) tk = 0;
-            present[nt] = ~0u;
-            if (MODE == kMatvec) {
-                xp[nt] = A.x + (int64_t)(W.tok0 + tk) * A.ldx + 2 * t;
-            } else if (MODE == kExpertsIn) {
-                xp[nt] = A.x + (int64_t)(W.list[2 * (W.tok0 + tk)] / A.top) * A.ldx + 2 * t;
-            } else {
-                const int r = W.rows[x_s * tok_pitch + tk];
-                if (r < 0) present[nt] = 0u;
-                xp[nt] = A.h + (int64_t)max(r, 0) * 2 * A.hpad + 2 * t;
-            }
-        }
-    };
-    uint32_t xb[2][PIECES][NT][2], ahead[2][PIECES][NT][2];   // this tile row's, and the next one's on their way
-    auto load_x = [&]() {
-        if (MODE == kExpertsOut && x_kt == A.Kt) {
-            x_kt = 0;
-            x_s++;
-            rows_of();
-        }
-        const int k0 = x_kt * 32;
-        if (MODE == kExpertsOut || (vec && k0 + 32 <= A.K)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int q = 0; q < PIECES; q++) {
-                    const uint32_t *at = reinterpret_cast<const uint32_t *>(xp[nt] + q * A.hpad + k0);
-#pragma unroll
-                    for (int f = 0; f < 2; f++)
-#pragma unroll
-                        for (int p = 0; p < 2; p++) {
-                            if (MODE == kExpertsOut) ahead[f][q][nt][p] = __ldcg(at + f * 8 + p * 4);
-                            else ahead[f][q][nt][p] = at[f * 8 + p * 4];
-                            if (MODE == kExpertsOut && !SINGLE) ahead[f][q][nt][p] &= present[nt];
-                        }
-                }
-        } else {
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int v = 0; v < 4; v++) ahead[v >> 1][0][nt][v & 1] = load_pair(xp[nt] - 2 * t, k0 + v * 8 + 2 * t, A.K, vec);
-        }
-        x_kt++;
-    };
-
-    float acc[8][NT][4];
-#pragma unroll
-    for (int j = 0; j < 8; j++)
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int v = 0; v < 4; v++) acc[j][nt][v] = 0.0f;
-
+    const int whole = MODE == kExpertsOut ? A.Kt : vec ? A.K / 32 : 0;    // tile rows whose activations are plain pairs
     // lane group g reads face column (g >> 1) & 1 of tile (g & 1) + 2 * (g >> 2): neighbours in g are records apart, which
     // puts the 8 lanes of a 128-bit access in distinct banks
-    const int tile = (g & 1) | ((g >> 2) << 1), fc = (g >> 1) & 1, odd = g & 1;
+    const int fc = (g >> 1) & 1, odd = g & 1;
+    const uint32_t rec_off = ((g & 1) | ((g >> 2) << 1)) * F::kRec;
     const uint32_t sel_flip = MB == 7 && odd ? 0x4444u : 0u;
+
+    float acc[8][NT][4];
     bool ok = true;
-    int done = 0, st = 0, phase = 0;
-    if (n > 0) {
-        x_kt = MODE == kExpertsOut ? u0 % A.Kt : u0;
-        x_s = MODE == kExpertsOut ? u0 / A.Kt : 0;
-        rows_of();
-        load_x();
-    }
-    for (; done < n; done++) {
+    int st = 0, phase = 0;            // ring stage of the next tile row and its barrier's parity, kept over both sweeps
+    uint32_t seen = 0;                // all shared exponents met, ORed
+
+    // One sweep over the share.  The first one takes every step as it usually is and looks afterwards whether one was not (an
+    // exponent of 128 or more, a column that is no finite number): then all is done again with the exact wide steps.
+    auto sweep = [&](auto wide_tag) {
+        constexpr bool WIDE = decltype(wide_tag)::value;
 #pragma unroll
-        for (int v = 0; v < 4 * PIECES * NT; v++) (&xb[0][0][0][0])[v] = (&ahead[0][0][0][0])[v];
-        if (done + 1 < n) load_x();
-        ok = mbar_wait_bounded(bars + st, phase, const_cast<int *>(abort_flag), A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint8_t *rec = ring + st * F::kStage + tile * F::kRec;
+        for (int j = 0; j < 8; j++)
 #pragma unroll
-        for (int f = 0; f < 2; f++) {
-            const int face = 2 * f + fc;
-            Raw<MB> raw;
-            load_raw<MB>(raw, rec + 64 + face * F::kFace, t, odd);
-            uint32_t e[2];
-            e[0] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t);
-            e[1] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t + 8);
-            bool wide = ((e[0] | e[1]) & 0x8080u) != 0;
-            if constexpr (SINGLE) {
-                uint32_t b[PIECES][2], x[PIECES][2];
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int p = 0; p < 2; p++) {
-                    const uint32_t s = scale_pair(e[p], -kDown);
+                for (int v = 0; v < 4; v++) acc[j][nt][v] = 0.0f;
+        // the copies of the next tile row to ask for
+        int i_s = s0, i_kt = kt0, i_st = st;
+        int64_t i_off = (MODE == kExpertsOut ? (n > 0 ? W.list[s0] * image : 0) : W.w_off) + kt0 * row_bytes + col_off;
+        auto issue = [&]() {
+            uint8_t *dst = ring + i_st * F::kStage;
+            uint64_t *bar = bars + i_st;
+            mbar_arrive_expect_tx(bar, gated ? 2 * bytes : bytes);
+            bulk_g2s(dst, A.w0 + i_off, bytes, bar);
+            if (gated) bulk_g2s(dst + F::kStage / 2, A.w1 + i_off, bytes, bar);
+            i_st = i_st + 1 == S ? 0 : i_st + 1;
+            i_off += row_bytes;
+            if (MODE == kExpertsOut && ++i_kt == A.Kt) {
+                i_kt = 0;
+                if (++i_s * A.Kt < W.units) i_off = W.list[i_s] * image + col_off;
+            }
+        };
+        __syncwarp();
+        if (lane == 0)
+            for (int i = 0; i < min(S, n); i++) issue();
+        // The weights were asked for before what the launch in front of this one computes is waited for: it writes activations,
+        // never weights, and what was in front of that one was complete before it let this launch begin.
+        if (!WIDE) {
+            if (MODE != kExpertsIn) griddep_wait();
+            if (MODE == kMatvec) griddep_launch();
+        }
+
+        // The tokens' values of one tile row: lane (g, t) holds token g, k = 2t, 2t+1, 2t+8, 2t+9 of both face rows.  Lanes past
+        // the last token read the first one's row: their columns of the product are dropped.
+        const __nv_bfloat16 *xp[NT];
+        uint32_t present[NT];             // experts-out: all ones where the token has this expert
+        int x_s = s0, x_kt = kt0;
+        auto rows_of = [&]() {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                int tk = SINGLE ? 0 : nt * 8 + g;
+                if (tk >= W.n_tok) tk = 0;
+                present[nt] = ~0u;
+                if (MODE == kMatvec) {
+                    xp[nt] = A.x + (int64_t)(W.tok0 + tk) * A.ldx;
+                } else if (MODE == kExpertsIn) {
+                    xp[nt] = A.x + (int64_t)(W.list[2 * (W.tok0 + tk)] / A.top) * A.ldx;
+                } else {
+                    const int r = W.rows[x_s * tok_pitch + tk];
+                    if (r < 0) present[nt] = 0u;
+                    xp[nt] = A.h + (int64_t)max(r, 0) * 2 * A.hpad;
+                }
+                xp[nt] += x_kt * 32 + 2 * t;
+            }
+        };
+        uint32_t xb[2][PIECES][NT][2], ahead[2][PIECES][NT][2];   // this tile row's, and the next one's on their way
+        auto load_x = [&]() {
+            if (MODE == kExpertsOut && x_kt == A.Kt) {
+                x_kt = 0;
+                x_s++;
+                rows_of();
+            }
+            if (MODE == kExpertsOut || x_kt < whole) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int q = 0; q < PIECES; q++) {
-                        x[q][p] = xb[f][q][0][p];
-                        b[q][p] = mul_bf16x2(x[q][p], s);
-                        wide |= not_finite_pair(b[q][p]);
+                        const uint32_t *at = reinterpret_cast<const uint32_t *>(xp[nt] + q * A.hpad);
+#pragma unroll
+                        for (int f = 0; f < 2; f++)
+#pragma unroll
+                            for (int p = 0; p < 2; p++) {
+                                if (MODE == kExpertsOut) ahead[f][q][nt][p] = __ldcg(at + f * 8 + p * 4);
+                                else ahead[f][q][nt][p] = at[f * 8 + p * 4];
+                                if (MODE == kExpertsOut && !SINGLE) ahead[f][q][nt][p] &= present[nt];
+                            }
                     }
-                }
-                if (__any_sync(0xffffffffu, wide)) single_step_wide<MB, PIECES>(acc, raw, e, sel_flip, x);
-                else single_step<MB, PIECES>(acc, raw, sel_flip, b);
             } else {
-                if (__any_sync(0xffffffffu, wide)) step<MB, NT, PIECES, true>(acc, raw, e, sel_flip, xb[f]);
-                else step<MB, NT, PIECES, false>(acc, raw, e, sel_flip, xb[f]);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++)
+                        ahead[v >> 1][0][nt][v & 1] = load_pair(xp[nt] - x_kt * 32 - 2 * t, x_kt * 32 + v * 8 + 2 * t, A.K, vec);
+            }
+            x_kt++;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) xp[nt] += 32;
+        };
+        if (n > 0) {
+            rows_of();
+            load_x();
+        }
+        int done = 0;
+        for (; done < n; done++) {
+#pragma unroll
+            for (int v = 0; v < 4 * PIECES * NT; v++) (&xb[0][0][0][0])[v] = (&ahead[0][0][0][0])[v];
+            if (done + 1 < n) load_x();
+            ok = __all_sync(0xffffffffu, mbar_try_wait(bars + st, phase));
+            if (!ok) {
+                ok = mbar_wait_bounded(bars + st, phase, const_cast<int *>(abort_flag), A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
+            const uint8_t *rec = ring + st * F::kStage + rec_off;
+#pragma unroll
+            for (int f = 0; f < 2; f++) {
+                const int face = 2 * f + fc;
+                Raw<MB> raw;
+                load_raw<MB>(raw, rec + 64 + face * F::kFace, t, odd);
+                uint32_t e[2];
+                e[0] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t);
+                e[1] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t + 8);
+                if constexpr (SINGLE) {
+                    uint32_t b[PIECES][2];
+                    if constexpr (WIDE) {
+#pragma unroll
+                        for (int q = 0; q < PIECES; q++) b[q][0] = xb[f][q][0][0], b[q][1] = xb[f][q][0][1];
+                        single_step_wide<MB, PIECES>(acc, raw, e, sel_flip, b);
+                    } else {
+                        seen |= e[0] | e[1];
+#pragma unroll
+                        for (int p = 0; p < 2; p++) {
+                            const uint32_t s = scale_pair(e[p], -kDown);
+#pragma unroll
+                            for (int q = 0; q < PIECES; q++) b[q][p] = mul_bf16x2(xb[f][q][0][p], s);
+                        }
+                        single_step<MB, PIECES>(acc, raw, sel_flip, b);
+                    }
+                } else {
+                    if (!WIDE) seen |= e[0] | e[1];
+                    step<MB, NT, PIECES, WIDE>(acc, raw, e, sel_flip, xb[f]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0 && done + S < n) issue();
+            if (++st == S) {
+                st = 0;
+                phase ^= 1;
             }
         }
-        __syncwarp();
-        if (lane == 0 && done + S < n) issue();
-        if (++st == S) {
-            st = 0;
-            phase ^= 1;
+        if (!ok) {   // a copy that did not arrive in time: let those in flight land before the memory is given up (again bounded)
+            for (int i = done; i < min(n, done + S); i++) {
+                int own = 0;
+                (void)mbar_wait_bounded(bars + st, phase, &own, A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
+                if (++st == S) {
+                    st = 0;
+                    phase ^= 1;
+                }
+            }
         }
+    };
+    sweep(std::false_type());
+    bool again = (seen & 0x8080u) != 0;
+    if constexpr (SINGLE) {
+        if (t == (g >> 1))
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                again |= !isfinite((g & 1) ? acc[j][0][1] : acc[j][0][0]) || !isfinite((g & 1) ? acc[j][0][3] : acc[j][0][2]);
     }
-    if (!ok)   // a copy that did not arrive in time: let those in flight land before the memory is given up (again bounded)
-        for (int i = done; i < min(n, done + S); i++) {
-            int own = 0;
-            (void)mbar_wait_bounded(bars + i % S, (i / S) & 1, &own, A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
-        }
+    if (__any_sync(0xffffffffu, again) && ok) sweep(std::true_type());
+
     __syncthreads();                      // every warp is done with its ring: the sums take its place
     float *sums = reinterpret_cast<float *>(smem);
     if constexpr (SINGLE) {
@@ -490,7 +527,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
 
 // NT: groups of 8 tokens in one pass; 0: one token.
 template <int MB, int NT, int MODE>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT, MODE)) few_rows_kernel(const Args A)
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(MB, NT, MODE)) few_rows_kernel(const Args A)
 {
     using F = Fmt<MB>;
     using L = Lay<MB, NT>;
@@ -729,12 +766,11 @@ cudaError_t dispatch(int mant_bits, int nt, const Args &a, dim3 grid, cudaStream
 #undef BUDA_FEW
 }
 
-// How many CTAs share the tile rows of one column group: doubled while the launch does not fill the device's resident
-// CTAs and every warp keeps a tile row.
+// How many CTAs share the tile rows of one column group: as many as the device holds at once, while every warp keeps a tile row.
 int split_of(int64_t groups, int64_t tile_rows, int sm_count, int per_sm)
 {
     int c = 1;
-    while (c < 8 && groups * c * 2 <= (int64_t)sm_count * per_sm && tile_rows >= (int64_t)c * 2 * kWarps) c *= 2;
+    while (c < 8 && groups * (c + 1) <= (int64_t)sm_count * per_sm && tile_rows >= (int64_t)(c + 1) * kWarps) c++;
     return c;
 }
 
@@ -752,7 +788,7 @@ cudaError_t launch_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, 
     a.out = Y; a.ldo = ldy; a.out_f32 = out_f32;
     a.status = status;
     const int nt = groups_of_8(a.rows), groups = (a.Nt + kGroupTiles - 1) / kGroupTiles, passes = passes_of(a.rows);
-    a.cluster = split_of((int64_t)groups * passes, a.Kt, sm_count, ctas_per_sm(nt, kMatvec));
+    a.cluster = split_of((int64_t)groups * passes, a.Kt, sm_count, ctas_per_sm(mant_bits, nt, kMatvec));
     return dispatch<kMatvec>(mant_bits, nt, a, dim3(groups * a.cluster, passes), stream);
 }
 
@@ -769,14 +805,14 @@ cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stre
     a.h = (__nv_bfloat16 *)m.h; a.hpad = 32 * It;
     a.status = status;
     const int span = m.up ? kGroupTiles / 2 : kGroupTiles, groups = (It + span - 1) / span;
-    a.cluster = split_of((int64_t)groups * most, Ht, sm_count, ctas_per_sm(nt, kExpertsIn));
+    a.cluster = split_of((int64_t)groups * most, Ht, sm_count, ctas_per_sm(m.mant_bits, nt, kExpertsIn));
     cudaError_t e = dispatch<kExpertsIn>(m.mant_bits, nt, a, dim3(groups * a.cluster, most, passes), stream);
     if (e != cudaSuccess) return e;
     a.K = m.I; a.Kt = It; a.N = m.H; a.Nt = Ht;
     a.w0 = (const uint8_t *)m.down; a.w1 = nullptr;
     a.out = m.y; a.ldo = m.ldy; a.out_f32 = 0;
     const int groups2 = (Ht + kGroupTiles - 1) / kGroupTiles;
-    a.cluster = split_of((int64_t)groups2 * passes, (int64_t)It * most, sm_count, ctas_per_sm(nt, kExpertsOut));
+    a.cluster = split_of((int64_t)groups2 * passes, (int64_t)It * most, sm_count, ctas_per_sm(m.mant_bits, nt, kExpertsOut));
     return dispatch<kExpertsOut>(m.mant_bits, nt, a, dim3(groups2 * a.cluster, passes), stream);
 }
 
