@@ -33,17 +33,16 @@
 namespace buda {
 namespace few {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
+constexpr int kUnitWarps = 8;           // a CTA has 1, 2 or 3 times as many warps
 constexpr int kGroupTiles = 4;          // tile columns of one warp
 constexpr int kPitch = 132;             // floats per token of a warp's sums: 8-byte stores of 4 x 4 lanes meet no bank twice
 constexpr int kDown = 24;               // single-token sums are held times 2^-24 (see single_step)
 
 enum { kMatvec = 0, kExpertsIn = 1, kExpertsOut = 2 };
 
-// CTAs that an SM holds, by registers: 80 suffice for one token (but for 8-bit data and the two pieces of experts-out), 128 for
-// up to 16 tokens
-__host__ __device__ constexpr int ctas_per_sm(int mb, int nt, int mode)
+// How many units of 8 warps an SM holds, by registers: 80 a thread suffice for one token (but for 8-bit data and the two pieces of
+// experts-out), 128 for up to 16 tokens
+__host__ __device__ constexpr int units_per_sm(int mb, int nt, int mode)
 {
     return nt == 0 && mb != 7 && mode != kExpertsOut ? 3 : nt <= 2 ? 2 : 1;
 }
@@ -284,17 +283,21 @@ __device__ __forceinline__ float activate(float v, int act)
 template <int MB, int NT>
 struct Lay {
     static constexpr int kTok = NT ? 8 * NT : 1;
-    static constexpr int kRing = kWarps * Fmt<MB>::kStages * Fmt<MB>::kStage;
-    static constexpr int kSums = kWarps * kTok * kPitch * 4;
-    static constexpr int kFirst = kRing > kSums ? kRing : kSums;
-    static constexpr int kPart = kFirst;                                  // [kTok][128] floats
-    static constexpr int kBars = kPart + kTok * 128 * 4;
-    static constexpr int kTables = kBars + kWarps * Fmt<MB>::kStages * 8;
-    static constexpr int kMap = kTables;                                  // 8 words: bit e set where expert e has a token
+    static constexpr int kRing = Fmt<MB>::kStages * Fmt<MB>::kStage;      // of one warp
+    static constexpr int kSums = kTok * kPitch * 4;                       // of one warp
+    static constexpr int kWarp = kRing > kSums ? kRing : kSums;
+    // behind the warps' memory:
+    static constexpr int kPart = 0;                                       // [kTok][128] floats
+    static constexpr int kMap = kPart + kTok * 128 * 4;                   // 8 words: bit e set where expert e has a token
     static constexpr int kCtl = kMap + kMaxExperts / 8;                   // 4 words
-    static constexpr int kList = kCtl + 16;                               // in: (slot, weight) of the tokens; out: experts
-    static constexpr int kRows = kList + 4 * kMaxExperts;                 // out: slot of (expert, token)
-    static constexpr int kBytes(int mode) { return mode == kMatvec ? kList : mode == kExpertsIn ? kRows : kRows + 2 * kMaxExperts * kTok; }
+    static constexpr int kBars = kCtl + 16;
+    __host__ __device__ static constexpr int tables(int warps) { return kBars + warps * Fmt<MB>::kStages * 8; }
+    // tables: in: (slot, weight) of the tokens; out: experts, then the slot of (expert, token)
+    static constexpr int kRows = 4 * kMaxExperts;
+    static constexpr int bytes(int mode, int warps)
+    {
+        return warps * kWarp + tables(warps) + (mode == kMatvec ? 0 : mode == kExpertsIn ? kRows : kRows + 2 * kMaxExperts * kTok);
+    }
 };
 
 // What a warp works on: `units` tile rows of (expert, tile row) pairs, its own share of them, and its ring.
@@ -315,10 +318,11 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     constexpr int S = F::kStages;
     constexpr int PIECES = MODE == kExpertsOut ? 2 : 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    uint8_t *ring = smem + warp * S * F::kStage;
+    uint8_t *ring = smem + warp * Lay<MB, SINGLE ? 0 : NT>::kRing;
     const int64_t image = (int64_t)A.Kt * A.Nt * F::kRec, row_bytes = (int64_t)A.Nt * F::kRec;
-    const int u0 = (int)((int64_t)W.units * me / workers), n = (int)((int64_t)W.units * (me + 1) / workers) - u0;
-    const int s0 = MODE == kExpertsOut ? u0 / A.Kt : 0, kt0 = u0 - s0 * A.Kt;
+    const uint32_t each = (uint32_t)W.units / (uint32_t)workers, extra = (uint32_t)W.units - each * workers;
+    const int u0 = (int)(me * each + min((uint32_t)me, extra)), n = (int)(each + ((uint32_t)me < extra));
+    const int s0 = MODE == kExpertsOut ? (int)((uint32_t)u0 / (uint32_t)A.Kt) : 0, kt0 = u0 - s0 * A.Kt;
     const bool gated = MODE == kExpertsIn && A.w1 != nullptr;
     const int span = gated ? kGroupTiles / 2 : kGroupTiles;
     const int64_t col_off = (int64_t)group * span * F::kRec;
@@ -495,10 +499,12 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     sweep(std::false_type());
     bool again = (seen & 0x8080u) != 0;
     if constexpr (SINGLE) {
-        if (t == (g >> 1))
+        float z = 0.0f;                   // a sum of zeros, unless something is not finite
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                again |= !isfinite((g & 1) ? acc[j][0][1] : acc[j][0][0]) || !isfinite((g & 1) ? acc[j][0][3] : acc[j][0][2]);
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) z = fmaf(acc[j][0][v], 0.0f, z);
+        again |= z != 0.0f;
     }
     if (__any_sync(0xffffffffu, again) && ok) sweep(std::true_type());
 
@@ -527,20 +533,21 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
 
 // NT: groups of 8 tokens in one pass; 0: one token.
 template <int MB, int NT, int MODE>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(MB, NT, MODE)) few_rows_kernel(const Args A)
+__global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(MB, NT, MODE), 1) few_rows_kernel(const Args A)
 {
     using F = Fmt<MB>;
     using L = Lay<MB, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int c = A.cluster;
+    const int c = A.cluster, threads = blockDim.x, warps = threads >> 5;
     const int rank = c > 1 ? (int)cluster_rank() : 0;
     const int group = blockIdx.x / c;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars) + warp * F::kStages;
-    uint32_t *map = reinterpret_cast<uint32_t *>(smem + L::kMap);
-    volatile int *ctl = reinterpret_cast<volatile int *>(smem + L::kCtl);   // [0] abort flag, [1] count
-    int *list = reinterpret_cast<int *>(smem + L::kList);
-    int16_t *rows = reinterpret_cast<int16_t *>(smem + L::kRows);
+    uint8_t *base = smem + warps * L::kWarp;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(base + L::kBars) + warp * F::kStages;
+    uint32_t *map = reinterpret_cast<uint32_t *>(base + L::kMap);
+    volatile int *ctl = reinterpret_cast<volatile int *>(base + L::kCtl);   // [0] abort flag, [1] count
+    int *list = reinterpret_cast<int *>(base + L::tables(warps));
+    int16_t *rows = reinterpret_cast<int16_t *>(base + L::tables(warps) + L::kRows);
 
     if (lane == 0) {
         for (int i = 0; i < F::kStages; i++) mbar_init(bars + i, 1);
@@ -567,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(MB, NT, MODE)) few_rows_
         }
         __syncthreads();
         const int t_end = MODE == kExpertsOut ? min(A.rows, W.tok0 + L::kTok) : A.rows;
-        for (int i = W.tok0 * A.top + tid; i < t_end * A.top; i += kThreads) {
+        for (int i = W.tok0 * A.top + tid; i < t_end * A.top; i += threads) {
             const int e = __ldcg(A.ids + i);
             if (e >= 0 && e < A.E) atomicOr(&map[e >> 5], 1u << (e & 31));
         }
@@ -618,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(MB, NT, MODE)) few_rows_
                     list[at] = tid;
                 }
             }
-            for (int i = tid; i < count * L::kTok; i += kThreads) rows[i] = -1;
+            for (int i = tid; i < count * L::kTok; i += threads) rows[i] = -1;
             __syncthreads();
             if (tid < W.n_tok)
                 for (int s = A.top - 1; s >= 0; s--) {
@@ -633,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(MB, NT, MODE)) few_rows_
         }
     }
 
-    const int workers = c * kWarps, me = rank * kWarps + warp;
+    const int workers = c * warps, me = rank * warps + warp;
     if constexpr (NT == 0) {
         products<MB, 1, MODE, true>(A, W, smem, bars, &ctl[0], group, me, workers, 1);
     } else if constexpr (MODE == kExpertsIn) {
@@ -643,26 +650,26 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(MB, NT, MODE)) few_rows_
         products<MB, NT, MODE, false>(A, W, smem, bars, &ctl[0], group, me, workers, L::kTok);
     }
 
-    // ---- join the warps
+    // ---- join the warps, and the CTAs of a cluster (each finishes its share of the outputs)
     const float *sums = reinterpret_cast<const float *>(smem);
-    float *part = reinterpret_cast<float *>(smem + L::kPart);
-    for (int i = tid; i < W.n_tok * 64; i += kThreads) {
-        const int tk = i >> 6, q = i & 63;
+    float *part = reinterpret_cast<float *>(base + L::kPart);
+    auto of_cta = [&](int tk, int q) {
         float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) {
+#pragma unroll 8
+        for (int w = 0; w < warps; w++) {
             const float2 v = *reinterpret_cast<const float2 *>(sums + (w * L::kTok + tk) * kPitch + 2 * q);
             s.x += v.x;
             s.y += v.y;
         }
-        *reinterpret_cast<float2 *>(part + tk * 128 + 2 * q) = s;
+        return s;
+    };
+    if (c > 1) {
+        for (int i = tid; i < W.n_tok * 64; i += threads) *reinterpret_cast<float2 *>(part + (i >> 6) * 128 + 2 * (i & 63)) = of_cta(i >> 6, i & 63);
+        cluster_sync();
     }
-    if (c > 1) cluster_sync(); else __syncthreads();
-
-    // ---- join the CTAs of the cluster (each finishes its share of the outputs) and write
     auto total = [&](int tk, int q) {
+        if (c == 1) return of_cta(tk, q);
         float2 s = make_float2(0.0f, 0.0f);
-        if (c == 1) return *reinterpret_cast<const float2 *>(part + tk * 128 + 2 * q);
         const uint32_t at = smem_u32(part + tk * 128 + 2 * q);
         for (int r = 0; r < c; r++) {
             const float2 v = ld_cluster_f2(map_rank(at, r));
@@ -674,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(MB, NT, MODE)) few_rows_
     const bool gated = MODE == kExpertsIn && A.w1 != nullptr;
     const int col0 = group * (gated ? kGroupTiles / 2 : kGroupTiles) * 32;
     const int per_tok = gated ? 32 : 64, items = W.n_tok * per_tok;
-    for (int i = rank * kThreads + tid; i < items; i += c * kThreads) {
+    for (int i = rank * threads + tid; i < items; i += c * threads) {
         const int tk = gated ? i >> 5 : i >> 6, r = i & (per_tok - 1);
         const int j = gated ? r >> 2 : r >> 3, gg = gated ? r & 3 : r & 7, q = j * 8 + gg;
         const int col = col0 + ((gg & 1) | ((gg >> 2) << 1)) * 32 + ((gg >> 1) & 1) * 16 + 2 * j;
@@ -717,22 +724,23 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(MB, NT, MODE)) few_rows_
 // Every launch may begin before the one in front of it is done (it waits for that one before it reads activations or ids, and
 // before it writes).  Only launches that say so let it: those of this file and of the router.
 template <int MB, int NT, int MODE>
-cudaError_t launch_one(const Args &a, dim3 grid, cudaStream_t stream)
+cudaError_t launch_one(const Args &a, dim3 grid, int warps, cudaStream_t stream)
 {
-    constexpr int bytes = Lay<MB, NT>::kBytes(MODE);
+    constexpr int most = Lay<MB, NT>::bytes(MODE, kUnitWarps * units_per_sm(MB, NT, MODE));
+    static_assert(most <= 227 * 1024, "shared memory of the largest CTA");
     static std::atomic<uint64_t> ready{0};      // devices whose kernel may take this much shared memory
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
-        e = cudaFuncSetAttribute(few_rows_kernel<MB, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        e = cudaFuncSetAttribute(few_rows_kernel<MB, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e != cudaSuccess) return e;
         ready.fetch_or(1ull << dev, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = bytes;
+    cfg.blockDim = dim3(32 * warps);
+    cfg.dynamicSmemBytes = Lay<MB, NT>::bytes(MODE, warps);
     cfg.stream = stream;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -748,15 +756,34 @@ cudaError_t launch_one(const Args &a, dim3 grid, cudaStream_t stream)
 int passes_of(int rows) { return rows <= 32 ? 1 : (rows + 31) / 32; }
 int groups_of_8(int rows) { return rows == 1 ? 0 : rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
-template <int MODE>
-cudaError_t dispatch(int mant_bits, int nt, const Args &a, dim3 grid, cudaStream_t stream)
+// How the tile rows of a column group are shared out: over the warps of a CTA, then over a cluster.
+struct Split {
+    int units, cluster;       // units of 8 warps in a CTA; CTAs
+};
+Split split_of(int64_t groups, int64_t tile_rows, int sm_count, int per_sm)
 {
+    int64_t f = (int64_t)sm_count * per_sm / groups;                 // units of 8 warps a group can have at once
+    const int64_t useful = (tile_rows + kUnitWarps - 1) / kUnitWarps;
+    if (f > useful) f = useful;
+    if (f < 1) f = 1;
+    if (f <= per_sm) return {(int)f, 1};
+    const int64_t c = f / per_sm;
+    return {per_sm, (int)(c < 8 ? c : 8)};
+}
+
+template <int MODE>
+cudaError_t dispatch(int mant_bits, int nt, Args &a, int64_t groups, int64_t copies, int64_t tile_rows, dim3 grid, int sm_count, cudaStream_t stream)
+{
+    const Split s = split_of(groups * copies, tile_rows, sm_count, units_per_sm(mant_bits, nt, MODE));
+    a.cluster = s.cluster;
+    grid.x = (unsigned)(groups * s.cluster);
+    const int warps = s.units * kUnitWarps;
 #define BUDA_FEW(MB)                                              \
     switch (nt) {                                                 \
-        case 0: return launch_one<MB, 0, MODE>(a, grid, stream);  \
-        case 1: return launch_one<MB, 1, MODE>(a, grid, stream);  \
-        case 2: return launch_one<MB, 2, MODE>(a, grid, stream);  \
-        default: return launch_one<MB, 4, MODE>(a, grid, stream); \
+        case 0: return launch_one<MB, 0, MODE>(a, grid, warps, stream);  \
+        case 1: return launch_one<MB, 1, MODE>(a, grid, warps, stream);  \
+        case 2: return launch_one<MB, 2, MODE>(a, grid, warps, stream);  \
+        default: return launch_one<MB, 4, MODE>(a, grid, warps, stream); \
     }
     switch (mant_bits) {
         case 7: BUDA_FEW(7);
@@ -764,14 +791,6 @@ cudaError_t dispatch(int mant_bits, int nt, const Args &a, dim3 grid, cudaStream
         default: BUDA_FEW(1);
     }
 #undef BUDA_FEW
-}
-
-// How many CTAs share the tile rows of one column group: as many as the device holds at once, while every warp keeps a tile row.
-int split_of(int64_t groups, int64_t tile_rows, int sm_count, int per_sm)
-{
-    int c = 1;
-    while (c < 8 && groups * (c + 1) <= (int64_t)sm_count * per_sm && tile_rows >= (int64_t)(c + 1) * kWarps) c++;
-    return c;
 }
 
 }  // namespace few
@@ -788,8 +807,7 @@ cudaError_t launch_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, 
     a.out = Y; a.ldo = ldy; a.out_f32 = out_f32;
     a.status = status;
     const int nt = groups_of_8(a.rows), groups = (a.Nt + kGroupTiles - 1) / kGroupTiles, passes = passes_of(a.rows);
-    a.cluster = split_of((int64_t)groups * passes, a.Kt, sm_count, ctas_per_sm(mant_bits, nt, kMatvec));
-    return dispatch<kMatvec>(mant_bits, nt, a, dim3(groups * a.cluster, passes), stream);
+    return dispatch<kMatvec>(mant_bits, nt, a, groups, passes, a.Kt, dim3(1, passes), sm_count, stream);
 }
 
 cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stream, unsigned int *status)
@@ -805,15 +823,13 @@ cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stre
     a.h = (__nv_bfloat16 *)m.h; a.hpad = 32 * It;
     a.status = status;
     const int span = m.up ? kGroupTiles / 2 : kGroupTiles, groups = (It + span - 1) / span;
-    a.cluster = split_of((int64_t)groups * most, Ht, sm_count, ctas_per_sm(m.mant_bits, nt, kExpertsIn));
-    cudaError_t e = dispatch<kExpertsIn>(m.mant_bits, nt, a, dim3(groups * a.cluster, most, passes), stream);
+    cudaError_t e = dispatch<kExpertsIn>(m.mant_bits, nt, a, groups, most, Ht, dim3(1, most, passes), sm_count, stream);
     if (e != cudaSuccess) return e;
     a.K = m.I; a.Kt = It; a.N = m.H; a.Nt = Ht;
     a.w0 = (const uint8_t *)m.down; a.w1 = nullptr;
     a.out = m.y; a.ldo = m.ldy; a.out_f32 = 0;
     const int groups2 = (Ht + kGroupTiles - 1) / kGroupTiles;
-    a.cluster = split_of((int64_t)groups2 * passes, (int64_t)It * most, sm_count, ctas_per_sm(m.mant_bits, nt, kExpertsOut));
-    return dispatch<kExpertsOut>(m.mant_bits, nt, a, dim3(groups2 * a.cluster, passes), stream);
+    return dispatch<kExpertsOut>(m.mant_bits, nt, a, groups2, passes, (int64_t)It * most, dim3(1, passes), sm_count, stream);
 }
 
 }  // namespace buda
