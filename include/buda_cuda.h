@@ -407,9 +407,9 @@ int buda_moe_route(const void *X, int64_t T, int64_t H, int64_t ldx, const void 
  * gate, up: images of [H,I] matrices, down: of [I,H] matrices, the E experts of one kind one after another (what packing a
  * [1,E,H,I] tensor gives); up == NULL: experts without a gate, act(X[t] @ gate_e) alone.  A slot whose id is outside
  * [0, E) counts nothing (a dropped or padded slot); a token without a slot gets zeros; an expert named twice by a token
- * counts with the sum of its weights.  Y may be X.  workspace: buda_moe_workspace_bytes(T, top, I) bytes, 16-byte
+ * counts with the sum of its weights.  Y may be X.  workspace: buda_moe_workspace_bytes(T, top, H, I) bytes, 16-byte
  * aligned, for this call alone until it has run (two captured graphs that replay at the same time need one each). */
-int64_t buda_moe_workspace_bytes(int64_t T, int top, int64_t I);
+int64_t buda_moe_workspace_bytes(int64_t T, int top, int64_t H, int64_t I);
 int buda_moe_experts(const void *X, int64_t T, int64_t H, int64_t ldx, const float *weights, const int32_t *ids, int top,
                      const void *gate, const void *up, const void *down, int64_t E, int64_t I, int w_df, int act, void *Y,
                      int64_t ldy, void *workspace, uint64_t workspace_bytes, void *stream);

@@ -359,6 +359,7 @@ def test_few_row_operators_refuse_bad_arguments():
         ops.moe_route(x, torch.zeros(4, 64), 2)
     with pytest.raises(RuntimeError, match="activation"):
         ops.moe_experts(x, torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int32), img.view(1, -1), None, img.view(1, -1), 64, activation="relu")
-    assert _cabi.lib.buda_moe_workspace_bytes(3, 2, 33) == 3 * 2 * 2 * 64 * 2
-    for bad in ((65, 2, 32), (-1, 2, 32), (1, 0, 32), (1, 17, 32), (1, 1, 0), (1, 1, 1 << 25)):
+    assert _cabi.lib.buda_moe_workspace_bytes(3, 2, 100, 33) == 3 * 2 * 2 * 64 * 2
+    assert _cabi.lib.buda_moe_workspace_bytes(9, 2, 100, 33) == 9 * 2 * (2 * 64 * 2 + 128 * 4)
+    for bad in ((65, 2, 32, 32), (-1, 2, 32, 32), (1, 0, 32, 32), (1, 17, 32, 32), (1, 1, 32, 0), (1, 1, 0, 32), (1, 1, 32, 1 << 25)):
         assert _cabi.lib.buda_moe_workspace_bytes(*bad) == -1, bad

@@ -1,8 +1,12 @@
 // K9: products of a few rows (tokens) with block-float weights, for serving.
 //
 //   matvec      Y[m, n]  = sum_k A[m, k] W[k, n]
-//   experts     h[s, i]  = w_s act((x_t G_e)[i]) (x_t U_e)[i]            (launch 1, "in")
-//               y[t, n]  = sum over the slots s of token t of sum_i h[s, i] D_e[i, n]   (launch 2, "out")
+//   experts     h[s, i]  = w_s act((x_t G_e)[i]) (x_t U_e)[i]            ("in")
+//               y[t, n]  = sum over the slots s of token t of sum_i h[s, i] D_e[i, n]
+// The second product of the experts has two forms.  Up to 8 tokens ("out"): a column group runs through all reached experts
+// as if their rows were one long sum, with zeros where a token has not chosen an expert; nothing is left to add up.  More
+// tokens ("each"): every expert's products on their own with only its own tokens, into binary32 rows of the workspace that a third
+// launch adds up -- otherwise most columns of the tensor product would be zeros (16 experts, 32 tokens, two each: 4 of 32).
 //
 // W, G, U, D are queue images in the default byte layout: tile records of 64 shared exponents and four 16x16 faces, a
 // stored datum of m magnitude bits standing for (-1)^s q 2^(E - 126 - m).
@@ -26,6 +30,7 @@
 #include <cuda_bf16.h>
 
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "few_rows.cuh"
@@ -38,13 +43,14 @@ constexpr int kGroupTiles = 4;          // tile columns of one warp
 constexpr int kPitch = 132;             // floats per token of a warp's sums: 8-byte stores of 4 x 4 lanes meet no bank twice
 constexpr int kDown = 24;               // single-token sums are held times 2^-24 (see single_step)
 
-enum { kMatvec = 0, kExpertsIn = 1, kExpertsOut = 2 };
+enum { kMatvec = 0, kExpertsIn = 1, kExpertsOut = 2, kExpertsEach = 3 };
+__host__ __device__ constexpr bool from_h(int mode) { return mode == kExpertsOut || mode == kExpertsEach; }
 
 // How many units of 8 warps an SM holds, by registers: 80 a thread suffice for one token (but for 8-bit data and the two pieces of
-// experts-out), 128 for up to 16 tokens
+// h), 128 for up to 8 tokens and, in the matvec of data below 8 bits, for up to 16
 __host__ __device__ constexpr int units_per_sm(int mb, int nt, int mode)
 {
-    return nt == 0 && mb != 7 && mode != kExpertsOut ? 3 : nt <= 2 ? 2 : 1;
+    return nt == 0 && mb != 7 && !from_h(mode) ? 3 : nt <= 1 || (nt == 2 && mb != 7 && mode == kMatvec) ? 2 : 1;
 }
 
 template <int MB>
@@ -69,6 +75,8 @@ struct Args {
     int top, E, act;
     __nv_bfloat16 *h;            // [rows * top][2][32 * tile rows of the down matrix]
     int hpad;
+    float *partial;              // experts-each: [rows * top][32 * tile columns of the down matrix]
+    uint32_t m4, m16, m64;       // 4, 16, 64: multiplying by a parameter keeps a shift off the integer pipe (see pair_of)
     int cluster;
     unsigned int *status;
 };
@@ -144,9 +152,11 @@ __device__ __forceinline__ void load_raw(Raw<MB> &r, const uint8_t *face, int t,
     }
 }
 
-// Weight columns 2j and 2j+1 of the pair of rows p as subnormal bfloat16 pairs (low half: the even row).
+// Weight columns 2j and 2j+1 of the pair of rows p as subnormal bfloat16 pairs (low half: the even row).  The integer pipe, which
+// permutes and masks, is what these kernels run into; the shifts go to the multiply-add pipe, as products with 4, 16 and 64 that the
+// compiler does not know.
 template <int MB>
-__device__ __forceinline__ void pair_of(const Raw<MB> &r, int p, int j, uint32_t sel_flip, uint32_t &even, uint32_t &odd)
+__device__ __forceinline__ void pair_of(const Raw<MB> &r, int p, int j, uint32_t sel_flip, const Args &A, uint32_t &even, uint32_t &odd)
 {
     constexpr uint32_t keep = 0x80008000u | (((0x7fu << (7 - MB)) & 0x7fu) * 0x00010001u);
     if constexpr (MB == 7) {
@@ -155,12 +165,12 @@ __device__ __forceinline__ void pair_of(const Raw<MB> &r, int p, int j, uint32_t
         odd = __byte_perm(r.w[p][0][w], r.w[p][1][w], (0x4400u + 0x1111u * (b + 1)) ^ sel_flip) & keep;
     } else if constexpr (MB == 3) {
         const uint32_t d = __byte_perm(r.w[p][0][j >> 2], r.w[p][1][j >> 2], 0x4400u + 0x1111u * (j & 3));
-        even = (d << 4) & keep;
+        even = (d * A.m16) & keep;
         odd = d & keep;
     } else {
         const uint32_t d = __byte_perm(r.w[p][0][0], r.w[p][1][0], 0x4400u + 0x1111u * (j >> 1));
-        even = (j & 1) ? (d << 2) & keep : (d << 6) & keep;
-        odd = (j & 1) ? d & keep : (d << 4) & keep;
+        even = (j & 1) ? (d * A.m4) & keep : (d * A.m64) & keep;
+        odd = (j & 1) ? d & keep : (d * A.m16) & keep;
     }
 }
 
@@ -178,7 +188,7 @@ __device__ __forceinline__ bool not_finite_pair(uint32_t v) { return (((v & 0x7f
 // One 16-row step for up to 8 * NT tokens: the weights are scaled.  BIG where a shared exponent is above 127 (2^E is no
 // bfloat16 then: up to three factors).
 template <int MB, int NT, int PIECES, bool BIG>
-__device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw, const uint32_t (&e)[2], uint32_t sel_flip,
+__device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw, const uint32_t (&e)[2], uint32_t sel_flip, const Args &A,
                                      const uint32_t (&x)[PIECES][NT][2])
 {
     uint32_t s[2], s2[2], s3[2];
@@ -198,7 +208,7 @@ __device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw,
         uint32_t a[4];
 #pragma unroll
         for (int p = 0; p < 2; p++) {
-            pair_of<MB>(raw, p, j, sel_flip, a[2 * p], a[2 * p + 1]);
+            pair_of<MB>(raw, p, j, sel_flip, A, a[2 * p], a[2 * p + 1]);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 uint32_t v = mul_bf16x2(a[2 * p + c], s[p]);
@@ -218,13 +228,13 @@ __device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw,
 // Only the diagonal (row group g, column g) counts.  The columns are held times 2^-24, which keeps x 2^E inside bfloat16
 // up to |x| max|w| = 2^24 (a product below 2^-102 is then rounded at 2^-125).
 template <int MB, int PIECES>
-__device__ __forceinline__ void single_step(float (&acc)[8][1][4], const Raw<MB> &raw, uint32_t sel_flip, const uint32_t (&b)[PIECES][2])
+__device__ __forceinline__ void single_step(float (&acc)[8][1][4], const Raw<MB> &raw, uint32_t sel_flip, const Args &A, const uint32_t (&b)[PIECES][2])
 {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         uint32_t a[4];
-        pair_of<MB>(raw, 0, j, sel_flip, a[0], a[1]);
-        pair_of<MB>(raw, 1, j, sel_flip, a[2], a[3]);
+        pair_of<MB>(raw, 0, j, sel_flip, A, a[0], a[1]);
+        pair_of<MB>(raw, 1, j, sel_flip, A, a[2], a[3]);
 #pragma unroll
         for (int q = 0; q < PIECES; q++) mma16816(acc[j][0], a, b[q][0], b[q][1]);
     }
@@ -232,7 +242,7 @@ __device__ __forceinline__ void single_step(float (&acc)[8][1][4], const Raw<MB>
 
 // One token where some x 2^(E - 24) is no finite bfloat16: what is too much for the column goes to the weights.
 template <int MB, int PIECES>
-__device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Raw<MB> &raw, const uint32_t (&e)[2], uint32_t sel_flip,
+__device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Raw<MB> &raw, const uint32_t (&e)[2], uint32_t sel_flip, const Args &A,
                                               const uint32_t (&x)[PIECES][2])
 {
 #pragma unroll
@@ -255,8 +265,8 @@ __device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Ra
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             uint32_t a[4];
-            pair_of<MB>(raw, 0, j, sel_flip, a[0], a[1]);
-            pair_of<MB>(raw, 1, j, sel_flip, a[2], a[3]);
+            pair_of<MB>(raw, 0, j, sel_flip, A, a[0], a[1]);
+            pair_of<MB>(raw, 1, j, sel_flip, A, a[2], a[3]);
 #pragma unroll
             for (int c = 0; c < 4; c++) a[c] = mul_bf16x2(mul_bf16x2(mul_bf16x2(a[c], s1[c >> 1]), s2[c >> 1]), s3[c >> 1]);
             mma16816(acc[j][0], a, b[0], b[1]);
@@ -289,20 +299,28 @@ struct Lay {
     // behind the warps' memory:
     static constexpr int kPart = 0;                                       // [kTok][128] floats
     static constexpr int kMap = kPart + kTok * 128 * 4;                   // 8 words: bit e set where expert e has a token
-    static constexpr int kCtl = kMap + kMaxExperts / 8;                   // 4 words
-    static constexpr int kBars = kCtl + 16;
+    static constexpr int kAbort = kMap + kMaxExperts / 8;                 // a flag for each warp
+    static constexpr int kCount = kAbort + 24 * 4;
+    static constexpr int kBars = kCount + 16;
     __host__ __device__ static constexpr int tables(int warps) { return kBars + warps * Fmt<MB>::kStages * 8; }
-    // tables: in: (slot, weight) of the tokens; out: experts, then the slot of (expert, token)
+    // tables: in, each: (slot, weight) of the expert's tokens; out: experts, then the slot of (expert, token); all: the ids
     static constexpr int kRows = 4 * kMaxExperts;
+    __host__ __device__ static constexpr int ids(int mode, int warps) { return tables(warps) + (mode == kExpertsOut ? kRows + 2 * kMaxExperts * kTok : kRows); }
     static constexpr int bytes(int mode, int warps)
     {
-        return warps * kWarp + tables(warps) + (mode == kMatvec ? 0 : mode == kExpertsIn ? kRows : kRows + 2 * kMaxExperts * kTok);
+        return warps * kWarp + (mode == kMatvec ? tables(warps) : ids(mode, warps) + (NT ? 4 * kMaxFewRows * kMaxTop : 0));
     }
+};
+
+// The ring of a warp: the stage of its next tile row and that stage's parity.
+struct Ring {
+    int st, phase;
 };
 
 // What a warp works on: `units` tile rows of (expert, tile row) pairs, its own share of them, and its ring.
 struct Work {
-    int n_tok, tok0;             // tokens of this CTA; the first one
+    int n_tok, tok0;             // tokens of this pass; the first one
+    bool begin;                  // the first pass of this CTA
     int units;
     int64_t w_off;               // experts-in: where this expert's images begin
     const int *list;
@@ -311,12 +329,12 @@ struct Work {
 
 // The sums of this warp's share of the tile rows, left in sums[warp][token][j][g][2].  SINGLE: one token (NT = 1 then).
 template <int MB, int NT, int MODE, bool SINGLE>
-__device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *smem, uint64_t *bars, volatile int *abort_flag, int group, int me,
+__device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *smem, uint64_t *bars, volatile int *abort_flag, Ring &R, int group, int me,
                                          int workers, int tok_pitch)
 {
     using F = Fmt<MB>;
     constexpr int S = F::kStages;
-    constexpr int PIECES = MODE == kExpertsOut ? 2 : 1;
+    constexpr int PIECES = from_h(MODE) ? 2 : 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint8_t *ring = smem + warp * Lay<MB, SINGLE ? 0 : NT>::kRing;
     const int64_t image = (int64_t)A.Kt * A.Nt * F::kRec, row_bytes = (int64_t)A.Nt * F::kRec;
@@ -328,8 +346,8 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     const int64_t col_off = (int64_t)group * span * F::kRec;
     const uint32_t bytes = (uint32_t)min(span, A.Nt - group * span) * F::kRec;
 
-    const bool vec = MODE == kExpertsOut || ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 3) == 0;
-    const int whole = MODE == kExpertsOut ? A.Kt : vec ? A.K / 32 : 0;    // tile rows whose activations are plain pairs
+    const bool vec = from_h(MODE) || ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 3) == 0;
+    const int whole = from_h(MODE) ? A.Kt : vec ? A.K / 32 : 0;    // tile rows whose activations are plain pairs
     // lane group g reads face column (g >> 1) & 1 of tile (g & 1) + 2 * (g >> 2): neighbours in g are records apart, which
     // puts the 8 lanes of a 128-bit access in distinct banks
     const int fc = (g >> 1) & 1, odd = g & 1;
@@ -338,7 +356,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
 
     float acc[8][NT][4];
     bool ok = true;
-    int st = 0, phase = 0;            // ring stage of the next tile row and its barrier's parity, kept over both sweeps
+    int st = R.st, phase = R.phase;   // kept over both sweeps
     uint32_t seen = 0;                // all shared exponents met, ORed
 
     // One sweep over the share.  The first one takes every step as it usually is and looks afterwards whether one was not (an
@@ -372,7 +390,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
             for (int i = 0; i < min(S, n); i++) issue();
         // The weights were asked for before what the launch in front of this one computes is waited for: it writes activations,
         // never weights, and what was in front of that one was complete before it let this launch begin.
-        if (!WIDE) {
+        if (!WIDE && W.begin) {
             if (MODE != kExpertsIn) griddep_wait();
             if (MODE == kMatvec) griddep_launch();
         }
@@ -392,6 +410,8 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
                     xp[nt] = A.x + (int64_t)(W.tok0 + tk) * A.ldx;
                 } else if (MODE == kExpertsIn) {
                     xp[nt] = A.x + (int64_t)(W.list[2 * (W.tok0 + tk)] / A.top) * A.ldx;
+                } else if (MODE == kExpertsEach) {
+                    xp[nt] = A.h + (int64_t)W.list[2 * (W.tok0 + tk)] * 2 * A.hpad;
                 } else {
                     const int r = W.rows[x_s * tok_pitch + tk];
                     if (r < 0) present[nt] = 0u;
@@ -407,7 +427,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
                 x_s++;
                 rows_of();
             }
-            if (MODE == kExpertsOut || x_kt < whole) {
+            if (from_h(MODE) || x_kt < whole) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -417,7 +437,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
                         for (int f = 0; f < 2; f++)
 #pragma unroll
                             for (int p = 0; p < 2; p++) {
-                                if (MODE == kExpertsOut) ahead[f][q][nt][p] = __ldcg(at + f * 8 + p * 4);
+                                if (from_h(MODE)) ahead[f][q][nt][p] = __ldcg(at + f * 8 + p * 4);
                                 else ahead[f][q][nt][p] = at[f * 8 + p * 4];
                                 if (MODE == kExpertsOut && !SINGLE) ahead[f][q][nt][p] &= present[nt];
                             }
@@ -462,7 +482,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
                     if constexpr (WIDE) {
 #pragma unroll
                         for (int q = 0; q < PIECES; q++) b[q][0] = xb[f][q][0][0], b[q][1] = xb[f][q][0][1];
-                        single_step_wide<MB, PIECES>(acc, raw, e, sel_flip, b);
+                        single_step_wide<MB, PIECES>(acc, raw, e, sel_flip, A, b);
                     } else {
                         seen |= e[0] | e[1];
 #pragma unroll
@@ -471,11 +491,11 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
 #pragma unroll
                             for (int q = 0; q < PIECES; q++) b[q][p] = mul_bf16x2(xb[f][q][0][p], s);
                         }
-                        single_step<MB, PIECES>(acc, raw, sel_flip, b);
+                        single_step<MB, PIECES>(acc, raw, sel_flip, A, b);
                     }
                 } else {
                     if (!WIDE) seen |= e[0] | e[1];
-                    step<MB, NT, PIECES, WIDE>(acc, raw, e, sel_flip, xb[f]);
+                    step<MB, NT, PIECES, WIDE>(acc, raw, e, sel_flip, A, xb[f]);
                 }
             }
             __syncwarp();
@@ -508,6 +528,8 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     }
     if (__any_sync(0xffffffffu, again) && ok) sweep(std::true_type());
 
+    R.st = st;
+    R.phase = phase;
     __syncthreads();                      // every warp is done with its ring: the sums take its place
     float *sums = reinterpret_cast<float *>(smem);
     if constexpr (SINGLE) {
@@ -533,7 +555,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
 
 // NT: groups of 8 tokens in one pass; 0: one token.
 template <int MB, int NT, int MODE>
-__global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(MB, NT, MODE), 1) few_rows_kernel(const Args A)
+__global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(MB, NT, MODE), 1) few_rows_kernel(const __grid_constant__ Args A)
 {
     using F = Fmt<MB>;
     using L = Lay<MB, NT>;
@@ -544,17 +566,21 @@ __global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(MB, NT, MODE), 
     const int group = blockIdx.x / c;
     uint8_t *base = smem + warps * L::kWarp;
     uint64_t *bars = reinterpret_cast<uint64_t *>(base + L::kBars) + warp * F::kStages;
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(base + L::kAbort) + warp;
     uint32_t *map = reinterpret_cast<uint32_t *>(base + L::kMap);
-    volatile int *ctl = reinterpret_cast<volatile int *>(base + L::kCtl);   // [0] abort flag, [1] count
+    volatile int *found_at = reinterpret_cast<volatile int *>(base + L::kCount);
     int *list = reinterpret_cast<int *>(base + L::tables(warps));
     int16_t *rows = reinterpret_cast<int16_t *>(base + L::tables(warps) + L::kRows);
+    int *ids = reinterpret_cast<int *>(base + L::ids(MODE, warps));
 
+    // ring and flag are this warp's alone: it needs no other to begin
     if (lane == 0) {
         for (int i = 0; i < F::kStages; i++) mbar_init(bars + i, 1);
+        *abort_flag = 0;
         mbar_fence_init();
     }
-    if (tid == 0) ctl[0] = 0;
-    if (MODE != kMatvec && tid < kMaxExperts / 32) map[tid] = 0;
+    __syncwarp();
+    Ring R = {0, 0};
 
     // ---- which tokens and which matrices
     Work W;
@@ -563,96 +589,122 @@ __global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(MB, NT, MODE), 
     W.units = A.Kt;
     W.w_off = 0;
     W.tok0 = blockIdx.y * L::kTok;
+    W.begin = true;
+    int found = 0;                                     // in, each: the tokens of this CTA's expert
+    const int64_t image = (int64_t)A.Kt * A.Nt * F::kRec;
     if (MODE == kMatvec) {
-        __syncthreads();
         W.n_tok = min(A.rows - W.tok0, L::kTok);
     } else {
         if (MODE == kExpertsIn) {
             griddep_wait();
             griddep_launch();
+        }
+        if constexpr (NT == 0) {
+            // One token: lane s looks at slot s.  A slot counts where its expert exists and is not named before.
+            const int e = lane < A.top ? __ldcg(A.ids + lane) : -1;
+            const float w = lane < A.top ? __ldcg(A.wts + lane) : 0.0f;
+            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            const bool counts = e >= 0 && e < A.E && __ffs(same) - 1 == lane;
+            const uint32_t m = __ballot_sync(0xffffffffu, counts);
+            const int count = __popc(m);
+            W.n_tok = 1;
             W.tok0 = 0;
-        }
-        __syncthreads();
-        const int t_end = MODE == kExpertsOut ? min(A.rows, W.tok0 + L::kTok) : A.rows;
-        for (int i = W.tok0 * A.top + tid; i < t_end * A.top; i += threads) {
-            const int e = __ldcg(A.ids + i);
-            if (e >= 0 && e < A.E) atomicOr(&map[e >> 5], 1u << (e & 31));
-        }
-        __syncthreads();
-        int count = 0;
-        for (int w = 0; w < kMaxExperts / 32; w++) count += __popc(map[w]);
-        if (MODE == kExpertsIn) {
-            if ((int)blockIdx.y >= count) return;      // the whole cluster: it shares blockIdx.y
-            int e = 0, left = blockIdx.y;
-            for (int w = 0; w < kMaxExperts / 32; w++) {
-                const int here = __popc(map[w]);
-                if (left >= 0 && left < here) e = 32 * w + (int)__fns(map[w], 0, left + 1);
-                left -= here;
-            }
-            W.w_off = e * ((int64_t)A.Kt * A.Nt * F::kRec);
-            if (warp == 0) {                           // the tokens of this expert, in order; a repeated slot adds its weight
-                int found = 0;
-                for (int base = 0; base < A.rows; base += 32) {
-                    const int tk = base + lane;
-                    int first = -1;
-                    float w = 0.0f;
-                    if (tk < A.rows)
-                        for (int s = 0; s < A.top; s++)
-                            if (__ldcg(A.ids + tk * A.top + s) == e) {
-                                w += __ldcg(A.wts + tk * A.top + s);
-                                if (first < 0) first = s;
-                            }
-                    const uint32_t m = __ballot_sync(0xffffffffu, first >= 0);
-                    if (first >= 0) {
-                        const int at = found + __popc(m & ((1u << lane) - 1u));
-                        list[2 * at] = tk * A.top + first;
-                        list[2 * at + 1] = __float_as_int(w);
-                    }
-                    found += __popc(m);
+            if (MODE == kExpertsIn) {
+                if ((int)blockIdx.y >= count) return;  // the whole cluster: it shares blockIdx.y
+                const int s = (int)__fns(m, 0, blockIdx.y + 1);
+                W.w_off = __shfl_sync(0xffffffffu, e, s) * image;
+                float sum = 0.0f;                      // in the order of the slots
+                for (int i = 0; i < A.top; i++) {
+                    const float wi = __shfl_sync(0xffffffffu, w, i);
+                    if (__shfl_sync(0xffffffffu, e, i) == __shfl_sync(0xffffffffu, e, s)) sum += wi;
                 }
-                if (lane == 0) ctl[1] = found;
+                if (lane == 0) {                       // every warp writes the same
+                    list[0] = s;
+                    list[1] = __float_as_int(sum);
+                }
+            } else {
+                if (counts) {
+                    list[__popc(m & ((1u << lane) - 1u))] = e;
+                    rows[__popc(m & ((1u << lane) - 1u))] = (int16_t)lane;
+                }
+                W.units = count * A.Kt;
+            }
+            __syncwarp();
+        } else {
+            if (MODE != kExpertsOut) W.tok0 = 0;
+            const int t_end = MODE == kExpertsOut ? min(A.rows, W.tok0 + L::kTok) : A.rows, first = W.tok0 * A.top, slots = t_end * A.top - first;
+            if (tid < kMaxExperts / 32) map[tid] = 0;
+            __syncthreads();
+            for (int i = tid; i < slots; i += threads) {
+                int e = __ldcg(A.ids + first + i);
+                if (e < 0 || e >= A.E) e = -1;
+                ids[i] = e;
+                if (e >= 0) atomicOr(&map[e >> 5], 1u << (e & 31));
             }
             __syncthreads();
-            W.tok0 = blockIdx.z * L::kTok;
-            W.n_tok = min(ctl[1] - W.tok0, L::kTok);
-            if (W.n_tok <= 0) return;                  // the whole cluster here too
-        } else {
-            W.n_tok = t_end - W.tok0;
-            if (tid < kMaxExperts) {                   // expert e is number (set bits below e)
-                if (map[tid >> 5] >> (tid & 31) & 1u) {
+            int count = 0;
+            for (int w = 0; w < kMaxExperts / 32; w++) count += __popc(map[w]);
+            if (MODE == kExpertsOut) {
+                W.n_tok = t_end - W.tok0;
+                if (tid < kMaxExperts && (map[tid >> 5] >> (tid & 31) & 1u)) {     // expert e is number (set bits below e)
                     int at = __popc(map[tid >> 5] & ((1u << (tid & 31)) - 1u));
                     for (int w = 0; w < (tid >> 5); w++) at += __popc(map[w]);
                     list[at] = tid;
                 }
-            }
-            for (int i = tid; i < count * L::kTok; i += threads) rows[i] = -1;
-            __syncthreads();
-            if (tid < W.n_tok)
-                for (int s = A.top - 1; s >= 0; s--) {
-                    const int e = __ldcg(A.ids + (W.tok0 + tid) * A.top + s);
-                    if (e < 0 || e >= A.E) continue;
-                    int at = __popc(map[e >> 5] & ((1u << (e & 31)) - 1u));
-                    for (int w = 0; w < (e >> 5); w++) at += __popc(map[w]);
-                    rows[at * L::kTok + tid] = (int16_t)((W.tok0 + tid) * A.top + s);
+                for (int i = tid; i < count * L::kTok; i += threads) rows[i] = -1;
+                __syncthreads();
+                if (tid < W.n_tok)
+                    for (int s = A.top - 1; s >= 0; s--) {                         // of a repeated expert the first slot stays
+                        const int e = ids[tid * A.top + s];
+                        if (e < 0) continue;
+                        int at = __popc(map[e >> 5] & ((1u << (e & 31)) - 1u));
+                        for (int w = 0; w < (e >> 5); w++) at += __popc(map[w]);
+                        rows[at * L::kTok + tid] = (int16_t)((W.tok0 + tid) * A.top + s);
+                    }
+                __syncthreads();
+                W.units = count * A.Kt;
+            } else {
+                if ((int)blockIdx.y >= count) return;                              // the whole cluster: it shares blockIdx.y
+                int e = 0, left = blockIdx.y;
+                for (int w = 0; w < kMaxExperts / 32; w++) {
+                    const int here = __popc(map[w]);
+                    if (left >= 0 && left < here) e = 32 * w + (int)__fns(map[w], 0, left + 1);
+                    left -= here;
                 }
-            __syncthreads();
-            W.units = count * A.Kt;
+                W.w_off = e * image;
+                if (warp == 0) {                       // the tokens of this expert, in order; a repeated slot adds its weight
+                    int n = 0;
+                    for (int b = 0; b < A.rows; b += 32) {
+                        const int tk = b + lane;
+                        int slot = -1;
+                        float w = 0.0f;
+                        if (tk < A.rows)
+                            for (int s = 0; s < A.top; s++)
+                                if (ids[tk * A.top + s] == e) {
+                                    if (MODE == kExpertsIn) w += __ldcg(A.wts + tk * A.top + s);
+                                    if (slot < 0) slot = s;
+                                }
+                        const uint32_t m = __ballot_sync(0xffffffffu, slot >= 0);
+                        if (slot >= 0) {
+                            const int at = n + __popc(m & ((1u << lane) - 1u));
+                            list[2 * at] = tk * A.top + slot;
+                            list[2 * at + 1] = __float_as_int(w);
+                        }
+                        n += __popc(m);
+                    }
+                    if (lane == 0) *found_at = n;
+                }
+                __syncthreads();
+                found = *found_at;
+            }
         }
     }
 
     const int workers = c * warps, me = rank * warps + warp;
-    if constexpr (NT == 0) {
-        products<MB, 1, MODE, true>(A, W, smem, bars, &ctl[0], group, me, workers, 1);
-    } else if constexpr (MODE == kExpertsIn) {
-        if (W.n_tok == 1) products<MB, 1, MODE, true>(A, W, smem, bars, &ctl[0], group, me, workers, L::kTok);
-        else products<MB, NT, MODE, false>(A, W, smem, bars, &ctl[0], group, me, workers, L::kTok);
-    } else {
-        products<MB, NT, MODE, false>(A, W, smem, bars, &ctl[0], group, me, workers, L::kTok);
-    }
-
-    // ---- join the warps, and the CTAs of a cluster (each finishes its share of the outputs)
     const float *sums = reinterpret_cast<const float *>(smem);
     float *part = reinterpret_cast<float *>(base + L::kPart);
+    const bool gated = MODE == kExpertsIn && A.w1 != nullptr;
+    const int col0 = group * (gated ? kGroupTiles / 2 : kGroupTiles) * 32;
     auto of_cta = [&](int tk, int q) {
         float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll 8
@@ -663,10 +715,6 @@ __global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(MB, NT, MODE), 
         }
         return s;
     };
-    if (c > 1) {
-        for (int i = tid; i < W.n_tok * 64; i += threads) *reinterpret_cast<float2 *>(part + (i >> 6) * 128 + 2 * (i & 63)) = of_cta(i >> 6, i & 63);
-        cluster_sync();
-    }
     auto total = [&](int tk, int q) {
         if (c == 1) return of_cta(tk, q);
         float2 s = make_float2(0.0f, 0.0f);
@@ -678,47 +726,97 @@ __global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(MB, NT, MODE), 
         }
         return s;
     };
-    const bool gated = MODE == kExpertsIn && A.w1 != nullptr;
-    const int col0 = group * (gated ? kGroupTiles / 2 : kGroupTiles) * 32;
-    const int per_tok = gated ? 32 : 64, items = W.n_tok * per_tok;
-    for (int i = rank * threads + tid; i < items; i += c * threads) {
-        const int tk = gated ? i >> 5 : i >> 6, r = i & (per_tok - 1);
-        const int j = gated ? r >> 2 : r >> 3, gg = gated ? r & 3 : r & 7, q = j * 8 + gg;
-        const int col = col0 + ((gg & 1) | ((gg >> 2) << 1)) * 32 + ((gg >> 1) & 1) * 16 + 2 * j;
-        float2 v = total(tk, q);
-        if (MODE == kExpertsIn) {
-            float2 up = make_float2(1.0f, 1.0f);
-            if (gated) up = total(tk, q + 4);
-            const float w = __int_as_float(list[2 * (W.tok0 + tk) + 1]);
-            float r2[2] = {activate(v.x, A.act) * up.x * w, activate(v.y, A.act) * up.y * w};
-            __nv_bfloat16 *h = A.h + (int64_t)list[2 * (W.tok0 + tk)] * 2 * A.hpad;
-            if (col < A.hpad) {
-                uint32_t hi = 0, lo = 0;
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    if (col + b >= A.N) continue;      // tile padding stays zero
-                    const __nv_bfloat16 a = __float2bfloat16_rn(r2[b]);
-                    // infinities and NaN are carried by the first piece alone
-                    const float rest = r2[b] - __bfloat162float(a);
-                    const __nv_bfloat16 d = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);
-                    hi |= (uint32_t)__bfloat16_as_ushort(a) << (16 * b);
-                    lo |= (uint32_t)__bfloat16_as_ushort(d) << (16 * b);
-                }
-                *reinterpret_cast<uint32_t *>(h + col) = hi;
-                *reinterpret_cast<uint32_t *>(h + A.hpad + col) = lo;
-            }
+
+    // ---- one pass, or (in, each) as many as the expert has groups of kTok tokens
+    while (true) {
+        if (NT != 0 && (MODE == kExpertsIn || MODE == kExpertsEach)) W.n_tok = min(found - W.tok0, L::kTok);
+        if constexpr (NT == 0) {
+            products<MB, 1, MODE, true>(A, W, smem, bars, abort_flag, R, group, me, workers, 1);
+        } else if constexpr (MODE == kExpertsIn || MODE == kExpertsEach) {
+            if (W.n_tok == 1) products<MB, 1, MODE, true>(A, W, smem, bars, abort_flag, R, group, me, workers, L::kTok);
+            else products<MB, NT, MODE, false>(A, W, smem, bars, abort_flag, R, group, me, workers, L::kTok);
         } else {
-            const int64_t at = (int64_t)(W.tok0 + tk) * A.ldo + col;
-#pragma unroll
-            for (int b = 0; b < 2; b++)
-                if (col + b < A.N) {
-                    const float f = b ? v.y : v.x;
-                    if (A.out_f32) reinterpret_cast<float *>(A.out)[at + b] = f;
-                    else reinterpret_cast<__nv_bfloat16 *>(A.out)[at + b] = __float2bfloat16_rn(f);
-                }
+            products<MB, NT, MODE, false>(A, W, smem, bars, abort_flag, R, group, me, workers, L::kTok);
         }
+
+        // join the warps, and the CTAs of a cluster (each finishes its share of the outputs)
+        if (c > 1) {
+            for (int i = tid; i < W.n_tok * 64; i += threads)
+                *reinterpret_cast<float2 *>(part + (i >> 6) * 128 + 2 * (i & 63)) = of_cta(i >> 6, i & 63);
+            cluster_sync();
+        }
+        const int per_tok = gated ? 32 : 64, items = W.n_tok * per_tok;
+        for (int i = rank * threads + tid; i < items; i += c * threads) {
+            const int tk = gated ? i >> 5 : i >> 6, r = i & (per_tok - 1);
+            const int j = gated ? r >> 2 : r >> 3, gg = gated ? r & 3 : r & 7, q = j * 8 + gg;
+            const int col = col0 + ((gg & 1) | ((gg >> 2) << 1)) * 32 + ((gg >> 1) & 1) * 16 + 2 * j;
+            float2 v = total(tk, q);
+            if (MODE == kExpertsIn) {
+                float2 up = make_float2(1.0f, 1.0f);
+                if (gated) up = total(tk, q + 4);
+                const float w = __int_as_float(list[2 * (W.tok0 + tk) + 1]);
+                float r2[2] = {activate(v.x, A.act) * up.x * w, activate(v.y, A.act) * up.y * w};
+                __nv_bfloat16 *h = A.h + (int64_t)list[2 * (W.tok0 + tk)] * 2 * A.hpad;
+                if (col < A.hpad) {
+                    uint32_t hi = 0, lo = 0;
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        if (col + b >= A.N) continue;  // tile padding stays zero
+                        const __nv_bfloat16 a = __float2bfloat16_rn(r2[b]);
+                        // infinities and NaN are carried by the first piece alone
+                        const float rest = r2[b] - __bfloat162float(a);
+                        const __nv_bfloat16 d = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);
+                        hi |= (uint32_t)__bfloat16_as_ushort(a) << (16 * b);
+                        lo |= (uint32_t)__bfloat16_as_ushort(d) << (16 * b);
+                    }
+                    *reinterpret_cast<uint32_t *>(h + col) = hi;
+                    *reinterpret_cast<uint32_t *>(h + A.hpad + col) = lo;
+                }
+            } else if (MODE == kExpertsEach) {
+                if (col < 32 * A.Nt)
+                    *reinterpret_cast<float2 *>(A.partial + (int64_t)list[2 * (W.tok0 + tk)] * 32 * A.Nt + col) = v;
+            } else {
+                const int64_t at = (int64_t)(W.tok0 + tk) * A.ldo + col;
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+                    if (col + b < A.N) {
+                        const float f = b ? v.y : v.x;
+                        if (A.out_f32) reinterpret_cast<float *>(A.out)[at + b] = f;
+                        else reinterpret_cast<__nv_bfloat16 *>(A.out)[at + b] = __float2bfloat16_rn(f);
+                    }
+            }
+        }
+        if (c > 1) cluster_sync();                     // no CTA goes on while another reads its sums
+        if (NT == 0 || MODE == kMatvec || MODE == kExpertsOut || W.tok0 + L::kTok >= found) break;
+        W.tok0 += L::kTok;
+        W.begin = false;
+        fence_async_smem();                            // the sums were written where the next copies land
+        __syncthreads();
     }
-    if (c > 1) cluster_sync();       // no CTA leaves while another reads its sums
+}
+
+// y[t] = the sum of the rows of token t's slots, each expert once: a block for 1024 columns of a token.
+__global__ void __launch_bounds__(256) sum_slots_kernel(const float *partial, int64_t pitch, const int *ids, int top, int E, int H,
+                                                        __nv_bfloat16 *y, int64_t ldy)
+{
+    griddep_wait();
+    const int t = blockIdx.y, lane = threadIdx.x & 31, col = blockIdx.x * 1024 + threadIdx.x * 4;
+    const int e = lane < top ? __ldcg(ids + t * top + lane) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    uint32_t m = __ballot_sync(0xffffffffu, e >= 0 && e < E && __ffs(same) - 1 == lane);
+    if (col >= H) return;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (; m; m &= m - 1) {
+        const float4 v = __ldcg(reinterpret_cast<const float4 *>(partial + (int64_t)(t * top + __ffs(m) - 1) * pitch + col));
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+    }
+    const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int b = 0; b < 4; b++)
+        if (col + b < H) y[(int64_t)t * ldy + col + b] = __float2bfloat16_rn(f[b]);
 }
 
 // Every launch may begin before the one in front of it is done (it waits for that one before it reads activations or ids, and
@@ -753,44 +851,58 @@ cudaError_t launch_one(const Args &a, dim3 grid, int warps, cudaStream_t stream)
     return cudaLaunchKernelEx(&cfg, few_rows_kernel<MB, NT, MODE>, a);
 }
 
-int passes_of(int rows) { return rows <= 32 ? 1 : (rows + 31) / 32; }
 int groups_of_8(int rows) { return rows == 1 ? 0 : rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
-// How the tile rows of a column group are shared out: over the warps of a CTA, then over a cluster.
+// How the tile rows of a column group are shared out: over the warps of a CTA and over a cluster.
 struct Split {
     int units, cluster;       // units of 8 warps in a CTA; CTAs
 };
+// First CTAs, one to an SM, while each warp of 8 keeps a tile row; then more warps in a CTA, while each keeps 8 tile rows.
+// Measured (us; B200): 1x1024x1024 Bfp4_b, 8 column groups: 4 CTAs of 8 warps 2.75, 8 of 8 3.30, 1 of 24 3.75.  8x4096x1024
+// Bfp8_b: 8 of 8 4.79, 8 of 16 5.05, 1 of 16 11.5.  1x4096x16384 Bfp4_b, 128 groups: 1 of 8 12.75, 1 of 16 11.0, 1 of 24 11.5, 2 of 8
+// 14.6 (the join over a cluster costs about 2.5).
 Split split_of(int64_t groups, int64_t tile_rows, int sm_count, int per_sm)
 {
-    int64_t f = (int64_t)sm_count * per_sm / groups;                 // units of 8 warps a group can have at once
     const int64_t useful = (tile_rows + kUnitWarps - 1) / kUnitWarps;
-    if (f > useful) f = useful;
-    if (f < 1) f = 1;
-    if (f <= per_sm) return {(int)f, 1};
-    const int64_t c = f / per_sm;
-    return {per_sm, (int)(c < 8 ? c : 8)};
+    int64_t c = sm_count / groups;
+    c = c < 1 ? 1 : c > 8 ? 8 : c;
+    if (c > useful) c = useful;
+    int64_t u = tile_rows / (c * kUnitWarps * 8);
+    const int64_t room = (int64_t)sm_count * per_sm / (groups * c);
+    if (u > room) u = room;
+    if (u > per_sm) u = per_sm;
+    return {(int)(u < 1 ? 1 : u), (int)c};
 }
 
-template <int MODE>
-cudaError_t dispatch(int mant_bits, int nt, Args &a, int64_t groups, int64_t copies, int64_t tile_rows, dim3 grid, int sm_count, cudaStream_t stream)
+template <int MODE, int MB>
+cudaError_t launch_nt(int nt, const Args &a, dim3 grid, int warps, cudaStream_t stream)
 {
-    const Split s = split_of(groups * copies, tile_rows, sm_count, units_per_sm(mant_bits, nt, MODE));
-    a.cluster = s.cluster;
-    grid.x = (unsigned)(groups * s.cluster);
+    // one sum over all experts serves up to 8 tokens, sums of their own more than that
+    if constexpr (MODE != kExpertsEach)
+        if (nt == 0) return launch_one<MB, 0, MODE>(a, grid, warps, stream);
+    if constexpr (MODE != kExpertsOut) {
+        if (nt == 2) return launch_one<MB, 2, MODE>(a, grid, warps, stream);
+        if (nt == 4) return launch_one<MB, 4, MODE>(a, grid, warps, stream);
+    }
+    return launch_one<MB, 1, MODE>(a, grid, warps, stream);
+}
+
+// groups: column groups; copies: how many times each, for other experts or rows; y: grid rows
+template <int MODE>
+cudaError_t dispatch(int mant_bits, int nt, Args &a, int groups, double copies, int64_t tile_rows, int y, int sm_count, cudaStream_t stream)
+{
+    const Split s = split_of((int64_t)(groups * copies + 0.5), tile_rows, sm_count, units_per_sm(mant_bits, nt, MODE));
+    const dim3 grid((unsigned)(groups * s.cluster), y);
     const int warps = s.units * kUnitWarps;
-#define BUDA_FEW(MB)                                              \
-    switch (nt) {                                                 \
-        case 0: return launch_one<MB, 0, MODE>(a, grid, warps, stream);  \
-        case 1: return launch_one<MB, 1, MODE>(a, grid, warps, stream);  \
-        case 2: return launch_one<MB, 2, MODE>(a, grid, warps, stream);  \
-        default: return launch_one<MB, 4, MODE>(a, grid, warps, stream); \
-    }
+    a.cluster = s.cluster;
+    a.m4 = 4;
+    a.m16 = 16;
+    a.m64 = 64;
     switch (mant_bits) {
-        case 7: BUDA_FEW(7);
-        case 3: BUDA_FEW(3);
-        default: BUDA_FEW(1);
+        case 7: return launch_nt<MODE, 7>(nt, a, grid, warps, stream);
+        case 3: return launch_nt<MODE, 3>(nt, a, grid, warps, stream);
+        default: return launch_nt<MODE, 1>(nt, a, grid, warps, stream);
     }
-#undef BUDA_FEW
 }
 
 }  // namespace few
@@ -806,15 +918,18 @@ cudaError_t launch_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, 
     a.w0 = (const uint8_t *)W;
     a.out = Y; a.ldo = ldy; a.out_f32 = out_f32;
     a.status = status;
-    const int nt = groups_of_8(a.rows), groups = (a.Nt + kGroupTiles - 1) / kGroupTiles, passes = passes_of(a.rows);
-    return dispatch<kMatvec>(mant_bits, nt, a, groups, passes, a.Kt, dim3(1, passes), sm_count, stream);
+    const int nt = groups_of_8(a.rows), groups = (a.Nt + kGroupTiles - 1) / kGroupTiles, passes = (a.rows + 31) / 32;
+    return dispatch<kMatvec>(mant_bits, nt, a, groups, passes, a.Kt, passes, sm_count, stream);
 }
 
 cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stream, unsigned int *status)
 {
-    const int nt = groups_of_8(m.T), passes = passes_of(m.T);
     const int Ht = (m.H + 31) / 32, It = (m.I + 31) / 32;
     const int slots = m.T * m.top, most = m.E < slots ? m.E : slots;
+    // the experts that independent choices reach on average, and the tokens of one: up to 4 fit a group of 8 nearly always
+    const double miss = m.top < m.E ? 1.0 - (double)m.top / m.E : 0.0, reached = m.E * (1.0 - pow(miss, m.T));
+    const double share = (double)slots / m.E;
+    const int nt = m.T == 1 ? 0 : m.T <= kOneSum || share <= 4.0 ? 1 : share <= 10.0 ? 2 : 4;
     Args a = {};
     a.x = (const __nv_bfloat16 *)m.x; a.ldx = m.ldx;
     a.rows = m.T; a.K = m.H; a.Kt = Ht; a.N = m.I; a.Nt = It;
@@ -822,14 +937,28 @@ cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stre
     a.ids = m.ids; a.wts = m.weights; a.top = m.top; a.E = m.E; a.act = m.act;
     a.h = (__nv_bfloat16 *)m.h; a.hpad = 32 * It;
     a.status = status;
-    const int span = m.up ? kGroupTiles / 2 : kGroupTiles, groups = (It + span - 1) / span;
-    cudaError_t e = dispatch<kExpertsIn>(m.mant_bits, nt, a, groups, most, Ht, dim3(1, most, passes), sm_count, stream);
+    const int span = m.up ? kGroupTiles / 2 : kGroupTiles;
+    cudaError_t e = dispatch<kExpertsIn>(m.mant_bits, nt, a, (It + span - 1) / span, reached, Ht, most, sm_count, stream);
     if (e != cudaSuccess) return e;
     a.K = m.I; a.Kt = It; a.N = m.H; a.Nt = Ht;
     a.w0 = (const uint8_t *)m.down; a.w1 = nullptr;
     a.out = m.y; a.ldo = m.ldy; a.out_f32 = 0;
-    const int groups2 = (Ht + kGroupTiles - 1) / kGroupTiles;
-    return dispatch<kExpertsOut>(m.mant_bits, nt, a, groups2, passes, (int64_t)It * most, dim3(1, passes), sm_count, stream);
+    const int groups = (Ht + kGroupTiles - 1) / kGroupTiles;
+    if (m.T <= kOneSum) return dispatch<kExpertsOut>(m.mant_bits, nt, a, groups, 1.0, (int64_t)(It * reached + 0.5), 1, sm_count, stream);
+    a.partial = reinterpret_cast<float *>((uint8_t *)m.h + moe_h_bytes(m.T, m.top, m.I));
+    e = dispatch<kExpertsEach>(m.mant_bits, nt, a, groups, reached, It, most, sm_count, stream);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((m.H + 1023) / 1024, m.T);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, sum_slots_kernel, (const float *)a.partial, (int64_t)32 * Ht, m.ids, m.top, m.E, m.H, (__nv_bfloat16 *)m.y,
+                              m.ldy);
 }
 
 }  // namespace buda

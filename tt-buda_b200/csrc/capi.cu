@@ -1414,13 +1414,13 @@ int buda_moe_route(const void *X, int64_t T, int64_t H, int64_t ldx, const void 
     return BUDA_SUCCESS;
 }
 
-int64_t buda_moe_workspace_bytes(int64_t T, int top, int64_t I)
+int64_t buda_moe_workspace_bytes(int64_t T, int top, int64_t H, int64_t I)
 {
-    if (T < 0 || T > kMaxFewRows || top < 1 || top > kMaxTop || I < 1 || I > (1 << 24)) {
-        fail(BUDA_RUNTIME_ERROR, "moe workspace: %lld tokens, %d experts each, intermediate size %lld", (long long)T, top, (long long)I);
+    if (T < 0 || T > kMaxFewRows || top < 1 || top > kMaxTop || H < 1 || H > (1 << 24) || I < 1 || I > (1 << 24)) {
+        fail(BUDA_RUNTIME_ERROR, "moe workspace: %lld tokens, %d experts each, sizes %lld and %lld", (long long)T, top, (long long)H, (long long)I);
         return -1;
     }
-    return moe_h_bytes(T, top, I);
+    return moe_workspace(T, top, H, I);
 }
 
 static int check_experts(const void *X, int64_t T, int64_t H, int64_t ldx, const float *weights, const int32_t *ids, int top,
@@ -1436,9 +1436,9 @@ static int check_experts(const void *X, int64_t T, int64_t H, int64_t ldx, const
     if (misaligned(gate, 16) || misaligned(up, 16) || misaligned(down, 16) || misaligned(workspace, 16))
         return fail(BUDA_RUNTIME_ERROR, "moe_experts: weight images and the workspace must be 16-byte aligned");
     if (misaligned(weights, 4) || misaligned(ids, 4) || misaligned(Y, 2)) return fail(BUDA_RUNTIME_ERROR, "moe_experts: misaligned pointer");
-    if ((uint64_t)moe_h_bytes(T, top, I) > workspace_bytes)
+    if ((uint64_t)moe_workspace(T, top, H, I) > workspace_bytes)
         return fail(BUDA_RUNTIME_ERROR, "moe_experts: workspace of %llu bytes, %lld are needed", (unsigned long long)workspace_bytes,
-                    (long long)moe_h_bytes(T, top, I));
+                    (long long)moe_workspace(T, top, H, I));
     return BUDA_SUCCESS;
 }
 
@@ -1455,7 +1455,7 @@ static int run_experts(DevCtx *ctx, const void *X, int64_t T, int64_t H, int64_t
     m.y = Y; m.ldy = ldy; m.h = workspace;
     cudaError_t e = launch_moe_experts(m, ctx->sm_count, (cudaStream_t)stream, ctx->status);
     if (e != cudaSuccess) return cuda_fail(e, "moe_experts launch failed");
-    g_launches.fetch_add(2, std::memory_order_relaxed);
+    g_launches.fetch_add(T > kOneSum ? 3 : 2, std::memory_order_relaxed);
     return BUDA_SUCCESS;
 }
 

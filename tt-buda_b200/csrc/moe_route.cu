@@ -7,8 +7,8 @@
 // first).  A cluster of 8 CTAs takes a block of tokens; its CTAs share the experts, the warps of a CTA share an expert's
 // row when there are fewer experts than warps, so that all of w is asked for at once.  The scores meet in distributed
 // shared memory; the warp of token i chooses in CTA i % 8.
-// Scores decide which experts run, so they are summed more exactly than a binary32 chain would: 8 products at a time in
-// binary32, the groups in binary64, kept in binary64 until the largest has been taken off.
+// Scores decide which experts run: a lane adds its products 8 at a time, the 32 lanes and the pieces of a row are joined in
+// binary64, and the result is rounded to binary32 once.
 #include <cuda_bf16.h>
 
 #include "few_rows.cuh"
@@ -17,7 +17,7 @@ namespace buda {
 namespace route {
 
 constexpr int kCluster = 8;
-constexpr int kWarps = 16;
+constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kPerCta = kMaxExperts / kCluster;
 
@@ -26,12 +26,12 @@ __device__ __forceinline__ void cluster_sync()
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ double ld_cluster_f64(const double *p, uint32_t rank)
+__device__ __forceinline__ float ld_cluster_f32(const float *p, uint32_t rank)
 {
     uint32_t a;
-    double v;
+    float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
     return v;
 }
 
@@ -87,21 +87,21 @@ struct Octet<float> {
     }
 };
 
-// Binary64 in an order that unsigned integers have: NaN below every number, 0 for "already chosen".
-__device__ __forceinline__ uint64_t order_of(double l)
+// Binary32 in an order that unsigned integers have: NaN below every number, 0 for "already chosen".
+__device__ __forceinline__ uint32_t order_of(float l)
 {
-    if (isnan(l)) return 1ull;
-    const uint64_t b = (uint64_t)__double_as_longlong(l + 0.0);
-    return b >> 63 ? ~b : b | 0x8000000000000000ull;
+    if (isnan(l)) return 1u;
+    const uint32_t b = __float_as_uint(l + 0.0f);
+    return b >> 31 ? ~b : b | 0x80000000u;
 }
 
 template <typename TW, int TB>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2)
     route_kernel(const __nv_bfloat16 *x, int64_t ldx, int T, int H, const TW *w, int64_t ldw, int E, int top, int renorm, int split,
                  float *weights, int *ids)
 {
     __shared__ double part[kPerCta * TB * kWarps];      // [expert of this CTA][token][piece of the row]
-    __shared__ double score[kPerCta * TB];
+    __shared__ float score[kPerCta * TB];
     asm volatile("griddepcontrol.wait;" ::: "memory");                // x may come from the launch in front of this one
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -116,10 +116,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1)
         const int el = task / split, piece = task % split;
         const TW *row = w + (int64_t)(rank + el * kCluster) * ldw;
         const int o1 = (int)((int64_t)octets * (piece + 1) / split);
-        double s[TB];
+        float s[TB];
 #pragma unroll
-        for (int i = 0; i < TB; i++) s[i] = 0.0;
-        constexpr int kBatch = 4;       // octets of a row on their way at once
+        for (int i = 0; i < TB; i++) s[i] = 0.0f;
+        constexpr int kBatch = TB > 1 ? 4 : 8;       // octets of a row on their way at once
         for (int o = (int)((int64_t)octets * piece / split) + lane; o < o1; o += 32 * kBatch) {
             Octet<TW> a[kBatch];
             Octet<__nv_bfloat16> b[kBatch][TB];
@@ -140,55 +140,62 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1)
                     b[u][i].get(bv);
 #pragma unroll
                     for (int v = 0; v < 8; v++) p = fmaf(av[v], bv[v], p);
-                    s[i] += (double)p;
+                    s[i] += p;
                 }
             }
         }
 #pragma unroll
         for (int i = 0; i < TB; i++) {
+            double all = s[i];
 #pragma unroll
-            for (int d = 16; d; d >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
-            if (lane == 0) part[(el * TB + i) * split + piece] = s[i];
+            for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+            if (lane == 0) part[(el * TB + i) * split + piece] = all;
         }
     }
     __syncthreads();
     for (int i = tid; i < mine * TB; i += kThreads) {
         double v = 0.0;
         for (int p = 0; p < split; p++) v += part[i * split + p];
-        score[i] = v;
+        score[i] = (float)v;
     }
     cluster_sync();
     // warp `warp` of CTA `rank` chooses for token 8 * warp + rank of the block
     const int i = warp * kCluster + (int)rank;
     if (i < nt) {
-        double l[kMaxExperts / 32];
-        uint64_t key[kMaxExperts / 32];
+        constexpr int kPer = kMaxExperts / 32;
+        const int per = (E + 31) / 32;
+        float l[kPer];
+        uint32_t key[kPer];
 #pragma unroll
-        for (int q = 0; q < kMaxExperts / 32; q++) {
-            const int e = q * 32 + lane;
-            l[q] = e < E ? ld_cluster_f64(&score[(e / kCluster) * TB + i], e % kCluster) : 0.0;
-            key[q] = e < E ? order_of(l[q]) : 0ull;
+        for (int q = 0; q < kPer; q++) {
+            l[q] = 0.0f;
+            key[q] = 0u;
+            if (q < per) {
+                const int e = q * 32 + lane;
+                if (e < E) {
+                    l[q] = ld_cluster_f32(&score[(e / kCluster) * TB + i], e % kCluster);
+                    key[q] = order_of(l[q]);
+                }
+            }
         }
         int my_id = 0;              // lane s keeps the s-th choice
-        double my_l = 0.0, most = 0.0;
+        float my_l = 0.0f, most = 0.0f;
         for (int s = 0; s < top; s++) {
-            uint64_t best = 0;
+            uint32_t best = 0;
             int at = 0;
-            double bl = 0.0;
+            float bl = 0.0f;
 #pragma unroll
-            for (int q = 0; q < kMaxExperts / 32; q++)
-                if (key[q] > best) {
+            for (int q = 0; q < kPer; q++)
+                if (q < per && key[q] > best) {
                     best = key[q];
                     at = q * 32 + lane;
                     bl = l[q];
                 }
-            const uint32_t hi = (uint32_t)(best >> 32), mhi = __reduce_max_sync(0xffffffffu, hi);
-            const uint32_t lo = hi == mhi ? (uint32_t)best : 0u, mlo = __reduce_max_sync(0xffffffffu, lo);
-            const bool in = hi == mhi && (uint32_t)best == mlo;
-            const uint32_t id = __reduce_min_sync(0xffffffffu, in ? (uint32_t)at : 0xffffffffu);
-            const double v = __shfl_sync(0xffffffffu, bl, id & 31);
+            const uint32_t top_key = __reduce_max_sync(0xffffffffu, best);
+            const uint32_t id = __reduce_min_sync(0xffffffffu, best == top_key ? (uint32_t)at : 0xffffffffu);
+            const float v = __shfl_sync(0xffffffffu, bl, id & 31);
 #pragma unroll
-            for (int q = 0; q < kMaxExperts / 32; q++)
+            for (int q = 0; q < kPer; q++)
                 if (q * 32 + lane == (int)id) key[q] = 0;
             if (s == 0) most = v;
             if (lane == s) {
@@ -198,18 +205,18 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1)
         }
         float sum = 0.0f;
         if (renorm) {
-            sum = lane < top ? expf((float)(my_l - most)) : 0.0f;
+            sum = lane < top ? expf(my_l - most) : 0.0f;
         } else {
 #pragma unroll
-            for (int q = 0; q < kMaxExperts / 32; q++)
-                if (q * 32 + lane < E) sum += expf((float)(l[q] - most));
+            for (int q = 0; q < kPer; q++)
+                if (q * 32 + lane < E) sum += expf(l[q] - most);
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (lane < top) {
             const int64_t o = (int64_t)(t0 + i) * top + lane;
             ids[o] = my_id;
-            weights[o] = expf((float)(my_l - most)) / sum;
+            weights[o] = expf(my_l - most) / sum;
         }
     }
     cluster_sync();      // no CTA leaves while another reads its scores
@@ -223,8 +230,8 @@ cudaError_t launch_tw(const void *x, int64_t ldx, int T, int H, const void *w, i
     const int clusters = sm_count / kCluster > 0 ? sm_count / kCluster : 1;
     const int tb = T <= clusters ? 1 : T <= 2 * clusters ? 2 : 4;
     const int most = (E + kCluster - 1) / kCluster;
-    int split = 1;
-    while (split < kWarps && split * 2 * most <= kWarps) split *= 2;
+    int split = 1;                                  // pieces of a row: as many warps as there are, but 32 octets for each
+    while (split * 2 * most <= kWarps && H >= split * 2 * 256) split *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((T + tb - 1) / tb * kCluster));
     cfg.blockDim = dim3(kThreads);

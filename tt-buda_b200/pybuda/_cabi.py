@@ -125,7 +125,7 @@ _SIGS = {
     "buda_i8_gemm": (_i, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _f, _i, _vp, _i64, _vp]),
     "buda_bfp_matvec": (_i, [_vp, _i64, _i64, _i64, _vp, _i64, _i, _vp, _i64, _i, _vp]),
     "buda_moe_route": (_i, [_vp, _i64, _i64, _i64, _vp, _i, _i64, _i64, _i, _i, _vp, _vp, _vp]),
-    "buda_moe_workspace_bytes": (_i64, [_i64, _i, _i64]),
+    "buda_moe_workspace_bytes": (_i64, [_i64, _i, _i64, _i64]),
     "buda_moe_experts": (_i, [_vp, _i64, _i64, _i64, _vp, _vp, _i, _vp, _vp, _vp, _i64, _i64, _i, _i, _vp, _i64, _vp, _u64, _vp]),
     "buda_moe_layer": (_i, [_vp, _i64, _i64, _i64, _vp, _i, _i64, _i, _i, _vp, _vp, _vp, _i64, _i64, _i, _i, _vp, _vp, _vp, _i64, _vp,
                             _u64, _vp]),

@@ -310,7 +310,7 @@ def _experts_check(x, gate, up, down, inter, w_df, activation):
 
 
 def _workspace(x, top, inter, more=0):
-    nbytes = _cabi.lib.buda_moe_workspace_bytes(x.shape[0], top, inter)
+    nbytes = _cabi.lib.buda_moe_workspace_bytes(x.shape[0], top, x.shape[1], inter)
     if nbytes < 0:
         raise _cabi.BudaError(_cabi.RUNTIME_ERROR, _cabi.last_error())
     return torch.empty(nbytes + more, dtype=torch.uint8, device=x.device)
