@@ -443,8 +443,7 @@ enum {
     BUDA_DEVSTAT_UNPACK_FULL_WAIT = 3,
     BUDA_DEVSTAT_UNPACK_EMPTY_WAIT = 4,
     BUDA_DEVSTAT_GEMM_WAIT = 5,
-    BUDA_DEVSTAT_SELFTEST_WAIT = 6,    /* buda_selftest_bounded_wait (buda_cuda_testing.h): the wait that nothing completes ran out */
-    BUDA_DEVSTAT_FEW_ROWS_WAIT = 7     /* few-row products: a warp waited too long for its weights */
+    BUDA_DEVSTAT_SELFTEST_WAIT = 6     /* buda_selftest_bounded_wait (buda_cuda_testing.h): the wait that nothing completes ran out */
 };
 
 /* Number of kernels this library has launched in this process (for launch accounting). */

@@ -12,19 +12,23 @@
 // stored datum of m magnitude bits standing for (-1)^s q 2^(E - 126 - m).
 //
 // Bound: bytes of the images (1.0625 / 0.5625 / 0.3125 a weight) -- every weight meets only a few rows.  What decides is
-// how many copies are in flight and how few instructions decode a weight:
-//   * A warp owns 128 output columns (4 tile columns) and walks tile rows.  One bulk copy brings the 4 adjacent records
-//     of a tile row into the warp's own ring in shared memory; no warp waits for another until the sums are joined.
+// how few instructions a weight costs on its way and how much of the images is on its way at once:
+//   * A warp owns 128 output columns (4 tile columns) and walks tile rows.  Each lane loads its own pieces of the records
+//     straight into registers, one tile row ahead: four whole face rows (4t .. 4t+3) of one face, the four exponents beside
+//     them, and the four activations they meet, each as one piece of consecutive bytes; the four lanes of a face read its 128 (Bfp4)
+//     bytes together.  With 16 to 24 warps an SM that is 37 to 55 KB under way.  (The same through bulk copies into a ring of
+//     shared memory took half as many instructions again: barrier, copy issue, second load.)
 //   * Decode: a datum's sign and magnitude bits are moved to bit 15 and to the top of the 7 mantissa bits of a
 //     bfloat16, which makes the subnormal number (-1)^s q 2^(-126 - m); a packed multiply by 2^E finishes it, exactly.
 //     One byte permute puts the same byte of two weight rows into both halves of a register in both places, so a pair
 //     costs one AND (plus a shift for all but one datum of a byte) and the multiply.
 //   * The products go through mma.sync m16n8k16 with the WEIGHTS as the 16-row operand and the tokens as the 8 columns:
-//     a lane's fragment is two weight columns at four weight rows, which is what its 64-bit piece of a face holds, so
-//     decoded weights never leave the registers.  (tcgen05 reads its operands from shared or tensor memory: the decoded
-//     weights would be written and read once more there for a product whose tensor work is a few per cent of its time.)
-//   * The tile rows are split over the 8 warps of a CTA and over a cluster of up to 8 CTAs; sums are joined through
-//     shared and distributed shared memory in a fixed order: no workspace, no atomics, the same bits every time.
+//     a lane's fragment is two weight columns at four weight rows (which four of the sum's rows a lane takes is free, as long as
+//     the activations follow), so decoded weights never leave the registers.  (tcgen05 reads its operands from shared or
+//     tensor memory: the decoded weights would be written and read once more there for a product whose tensor work is small.)
+//   * The tile rows are split over the warps of a CTA and, where there are few columns, over a cluster of up to 8 CTAs;
+//     sums are joined through shared and distributed shared memory in a fixed order: no workspace, no atomics, the same bits
+//     every time.
 // Sums are held in binary32 throughout.  h is carried between the two launches as two bfloat16 pieces (the rounded value and
 // the rounded rest, together within 2^-16 of h), so nothing is lost against a binary32 h at twice the tensor work.
 #include <cuda_bf16.h>
@@ -38,7 +42,7 @@
 namespace buda {
 namespace few {
 
-constexpr int kUnitWarps = 8;           // a CTA has 1, 2 or 3 times as many warps
+constexpr int kUnitWarps = 8;           // a CTA has once or twice as many warps
 constexpr int kGroupTiles = 4;          // tile columns of one warp
 constexpr int kPitch = 132;             // floats per token of a warp's sums: 8-byte stores of 4 x 4 lanes meet no bank twice
 constexpr int kDown = 24;               // single-token sums are held times 2^-24 (see single_step)
@@ -46,20 +50,15 @@ constexpr int kDown = 24;               // single-token sums are held times 2^-2
 enum { kMatvec = 0, kExpertsIn = 1, kExpertsOut = 2, kExpertsEach = 3 };
 __host__ __device__ constexpr bool from_h(int mode) { return mode == kExpertsOut || mode == kExpertsEach; }
 
-// How many units of 8 warps an SM holds, by registers: 80 a thread suffice for one token (but for 8-bit data and the two pieces of
-// h), 128 for up to 8 tokens and, in the matvec of data below 8 bits, for up to 16
-__host__ __device__ constexpr int units_per_sm(int mb, int nt, int mode)
-{
-    return nt == 0 && mb != 7 && !from_h(mode) ? 3 : nt <= 1 || (nt == 2 && mb != 7 && mode == kMatvec) ? 2 : 1;
-}
+// How many units of 8 warps an SM holds, by registers: 128 a thread suffice for up to 8 tokens and, in the matvec of data below 8
+// bits, for up to 16
+__host__ __device__ constexpr int units_per_sm(int mb, int nt, int mode) { return nt <= 1 || (nt == 2 && mb != 7 && mode == kMatvec) ? 2 : 1; }
 
 template <int MB>
 struct Fmt {
     static constexpr int kRow = 2 * (MB + 1);               // bytes of one face row
     static constexpr int kFace = 16 * kRow;
     static constexpr int kRec = 64 + 4 * kFace;
-    static constexpr int kStage = kGroupTiles * kRec;
-    static constexpr int kStages = MB == 7 ? 3 : MB == 3 ? 4 : 7;   // 72 KB of rings: three CTAs fit an SM; 8-bit data: 102 KB, two
 };
 
 struct Args {
@@ -78,7 +77,6 @@ struct Args {
     float *partial;              // experts-each: [rows * top][32 * tile columns of the down matrix]
     uint32_t m4, m16, m64;       // 4, 16, 64: multiplying by a parameter keeps a shift off the integer pipe (see pair_of)
     int cluster;
-    unsigned int *status;
 };
 
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b)
@@ -122,47 +120,57 @@ __device__ __forceinline__ uint32_t cluster_rank()
     return r;
 }
 
-// The raw data of one lane: face rows 2t, 2t+1 (p = 0) and 2t+8, 2t+9 (p = 1) of one face.
+// The raw data of one lane: face rows 4t, 4t+1 (p = 0) and 4t+2, 4t+3 (p = 1) of one face, and their exponents.
 template <int MB>
 struct Raw {
     uint32_t w[2][2][(MB + 1) / 2];   // [p][row][32-bit word]
+    uint32_t e;
 };
 
-// 8-bit data: the two 16-byte rows are fetched in opposite order by the lanes of odd g, which keeps the 8 lanes of a
-// 128-bit access in distinct banks; the byte permutes undo it.
-template <int MB>
-__device__ __forceinline__ void load_raw(Raw<MB> &r, const uint8_t *face, int t, int odd)
+__device__ __forceinline__ uint4 load_once(const uint8_t *p)
 {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// data, exps: this lane's four rows and their exponents
+template <int MB>
+__device__ __forceinline__ void load_raw(Raw<MB> &r, const uint8_t *data, const uint8_t *exps)
+{
+    if constexpr (MB == 7) {
 #pragma unroll
-    for (int p = 0; p < 2; p++) {
-        const uint8_t *at = face + (2 * t + 8 * p) * Fmt<MB>::kRow;
-        if constexpr (MB == 7) {
-            const uint4 a = *reinterpret_cast<const uint4 *>(at + 16 * odd), b = *reinterpret_cast<const uint4 *>(at + 16 * (odd ^ 1));
-            r.w[p][0][0] = a.x; r.w[p][0][1] = a.y; r.w[p][0][2] = a.z; r.w[p][0][3] = a.w;
-            r.w[p][1][0] = b.x; r.w[p][1][1] = b.y; r.w[p][1][2] = b.z; r.w[p][1][3] = b.w;
-        } else if constexpr (MB == 3) {
-            const uint4 a = *reinterpret_cast<const uint4 *>(at);
+        for (int i = 0; i < 4; i++) {
+            const uint4 a = load_once(data + 16 * i);
+            uint32_t (&w)[4] = r.w[i >> 1][i & 1];
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        }
+    } else if constexpr (MB == 3) {
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            const uint4 a = load_once(data + 16 * p);
             r.w[p][0][0] = a.x; r.w[p][0][1] = a.y;
             r.w[p][1][0] = a.z; r.w[p][1][1] = a.w;
-        } else {
-            const uint2 a = *reinterpret_cast<const uint2 *>(at);
-            r.w[p][0][0] = a.x;
-            r.w[p][1][0] = a.y;
         }
+    } else {
+        const uint4 a = load_once(data);
+        r.w[0][0][0] = a.x; r.w[0][1][0] = a.y;
+        r.w[1][0][0] = a.z; r.w[1][1][0] = a.w;
     }
+    r.e = __ldg(reinterpret_cast<const uint32_t *>(exps));
 }
 
 // Weight columns 2j and 2j+1 of the pair of rows p as subnormal bfloat16 pairs (low half: the even row).  The integer pipe, which
 // permutes and masks, is what these kernels run into; the shifts go to the multiply-add pipe, as products with 4, 16 and 64 that the
 // compiler does not know.
 template <int MB>
-__device__ __forceinline__ void pair_of(const Raw<MB> &r, int p, int j, uint32_t sel_flip, const Args &A, uint32_t &even, uint32_t &odd)
+__device__ __forceinline__ void pair_of(const Raw<MB> &r, int p, int j, const Args &A, uint32_t &even, uint32_t &odd)
 {
     constexpr uint32_t keep = 0x80008000u | (((0x7fu << (7 - MB)) & 0x7fu) * 0x00010001u);
     if constexpr (MB == 7) {
         const int w = j >> 1, b = (j & 1) * 2;
-        even = __byte_perm(r.w[p][0][w], r.w[p][1][w], (0x4400u + 0x1111u * b) ^ sel_flip) & keep;
-        odd = __byte_perm(r.w[p][0][w], r.w[p][1][w], (0x4400u + 0x1111u * (b + 1)) ^ sel_flip) & keep;
+        even = __byte_perm(r.w[p][0][w], r.w[p][1][w], 0x4400u + 0x1111u * b) & keep;
+        odd = __byte_perm(r.w[p][0][w], r.w[p][1][w], 0x4400u + 0x1111u * (b + 1)) & keep;
     } else if constexpr (MB == 3) {
         const uint32_t d = __byte_perm(r.w[p][0][j >> 2], r.w[p][1][j >> 2], 0x4400u + 0x1111u * (j & 3));
         even = (d * A.m16) & keep;
@@ -177,30 +185,27 @@ __device__ __forceinline__ void pair_of(const Raw<MB> &r, int p, int j, uint32_t
 // 2^a and 2^b (-127 < a, b <= 127) as a bfloat16 pair
 __device__ __forceinline__ uint32_t pow2_pair(int a, int b) { return ((uint32_t)(a + 127) << 7) | ((uint32_t)(b + 127) << 23); }
 
-// the two shared exponents of a row pair, moved by `by`, as a pair of powers of two (0 < exponent + by + 127 < 255)
-__device__ __forceinline__ uint32_t scale_pair(uint32_t e, int by)
+// the shared exponents of row pair p, moved by `by`, as a pair of powers of two (0 < exponent + by + 127 < 255)
+__device__ __forceinline__ uint32_t scale_pair(uint32_t e, int p, int by)
 {
-    return (__byte_perm(e, 0u, 0x4140u) + (uint32_t)(by + 127) * 0x00010001u) << 7;
+    return (__byte_perm(e, 0u, p ? 0x4342u : 0x4140u) + (uint32_t)(by + 127) * 0x00010001u) << 7;
 }
-
-__device__ __forceinline__ bool not_finite_pair(uint32_t v) { return (((v & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0; }
 
 // One 16-row step for up to 8 * NT tokens: the weights are scaled.  BIG where a shared exponent is above 127 (2^E is no
 // bfloat16 then: up to three factors).
 template <int MB, int NT, int PIECES, bool BIG>
-__device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw, const uint32_t (&e)[2], uint32_t sel_flip, const Args &A,
-                                     const uint32_t (&x)[PIECES][NT][2])
+__device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw, const Args &A, const uint2 (&x)[PIECES][NT])
 {
     uint32_t s[2], s2[2], s3[2];
 #pragma unroll
     for (int p = 0; p < 2; p++) {
         if constexpr (BIG) {
-            const int a = e[p] & 0xff, b = e[p] >> 8;
+            const int a = (raw.e >> (16 * p)) & 0xff, b = (raw.e >> (16 * p + 8)) & 0xff;
             s[p] = pow2_pair(min(a, 127), min(b, 127));
             s2[p] = pow2_pair(min(max(a - 127, 0), 127), min(max(b - 127, 0), 127));
             s3[p] = pow2_pair(max(a - 254, 0), max(b - 254, 0));
         } else {
-            s[p] = scale_pair(e[p], 0);
+            s[p] = scale_pair(raw.e, p, 0);
         }
     }
 #pragma unroll
@@ -208,7 +213,7 @@ __device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw,
         uint32_t a[4];
 #pragma unroll
         for (int p = 0; p < 2; p++) {
-            pair_of<MB>(raw, p, j, sel_flip, A, a[2 * p], a[2 * p + 1]);
+            pair_of<MB>(raw, p, j, A, a[2 * p], a[2 * p + 1]);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 uint32_t v = mul_bf16x2(a[2 * p + c], s[p]);
@@ -219,7 +224,7 @@ __device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw,
 #pragma unroll
         for (int q = 0; q < PIECES; q++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) mma16816(acc[j][nt], a, x[q][nt][0], x[q][nt][1]);
+            for (int nt = 0; nt < NT; nt++) mma16816(acc[j][nt], a, x[q][nt].x, x[q][nt].y);
     }
 }
 
@@ -228,13 +233,13 @@ __device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw,
 // Only the diagonal (row group g, column g) counts.  The columns are held times 2^-24, which keeps x 2^E inside bfloat16
 // up to |x| max|w| = 2^24 (a product below 2^-102 is then rounded at 2^-125).
 template <int MB, int PIECES>
-__device__ __forceinline__ void single_step(float (&acc)[8][1][4], const Raw<MB> &raw, uint32_t sel_flip, const Args &A, const uint32_t (&b)[PIECES][2])
+__device__ __forceinline__ void single_step(float (&acc)[8][1][4], const Raw<MB> &raw, const Args &A, const uint32_t (&b)[PIECES][2])
 {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         uint32_t a[4];
-        pair_of<MB>(raw, 0, j, sel_flip, A, a[0], a[1]);
-        pair_of<MB>(raw, 1, j, sel_flip, A, a[2], a[3]);
+        pair_of<MB>(raw, 0, j, A, a[0], a[1]);
+        pair_of<MB>(raw, 1, j, A, a[2], a[3]);
 #pragma unroll
         for (int q = 0; q < PIECES; q++) mma16816(acc[j][0], a, b[q][0], b[q][1]);
     }
@@ -242,8 +247,7 @@ __device__ __forceinline__ void single_step(float (&acc)[8][1][4], const Raw<MB>
 
 // One token where some x 2^(E - 24) is no finite bfloat16: what is too much for the column goes to the weights.
 template <int MB, int PIECES>
-__device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Raw<MB> &raw, const uint32_t (&e)[2], uint32_t sel_flip, const Args &A,
-                                              const uint32_t (&x)[PIECES][2])
+__device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Raw<MB> &raw, const Args &A, const uint2 (&x)[PIECES][1])
 {
 #pragma unroll
     for (int q = 0; q < PIECES; q++) {
@@ -253,11 +257,11 @@ __device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Ra
             int d[2], v[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const int E = (e[p] >> (8 * h)) & 0xff, ex = (x[q][p] >> (7 + 16 * h)) & 0xff;
+                const int E = (raw.e >> (16 * p + 8 * h)) & 0xff, ex = ((p ? x[q][0].y : x[q][0].x) >> (7 + 16 * h)) & 0xff;
                 d[h] = E == 255 ? 255 : max(ex + E - kDown - 254, 0);   // a weight of 2^128 and above stays an infinity
                 v[h] = E - kDown - d[h];
             }
-            b[p] = mul_bf16x2(mul_bf16x2(x[q][p], pow2_pair(min(v[0], 127), min(v[1], 127))), pow2_pair(max(v[0] - 127, 0), max(v[1] - 127, 0)));
+            b[p] = mul_bf16x2(mul_bf16x2(p ? x[q][0].y : x[q][0].x, pow2_pair(min(v[0], 127), min(v[1], 127))), pow2_pair(max(v[0] - 127, 0), max(v[1] - 127, 0)));
             s1[p] = pow2_pair(min(d[0], 127), min(d[1], 127));
             s2[p] = pow2_pair(min(max(d[0] - 127, 0), 127), min(max(d[1] - 127, 0), 127));
             s3[p] = pow2_pair(max(d[0] - 254, 0), max(d[1] - 254, 0));
@@ -265,8 +269,8 @@ __device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Ra
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             uint32_t a[4];
-            pair_of<MB>(raw, 0, j, sel_flip, A, a[0], a[1]);
-            pair_of<MB>(raw, 1, j, sel_flip, A, a[2], a[3]);
+            pair_of<MB>(raw, 0, j, A, a[0], a[1]);
+            pair_of<MB>(raw, 1, j, A, a[2], a[3]);
 #pragma unroll
             for (int c = 0; c < 4; c++) a[c] = mul_bf16x2(mul_bf16x2(mul_bf16x2(a[c], s1[c >> 1]), s2[c >> 1]), s3[c >> 1]);
             mma16816(acc[j][0], a, b[0], b[1]);
@@ -274,13 +278,14 @@ __device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Ra
     }
 }
 
-// Elements k, k+1 of a row (k even), zero past K.
-__device__ __forceinline__ uint32_t load_pair(const __nv_bfloat16 *row, int k, int K, bool vec)
+// Elements k .. k+3 of a row one by one, zero past K.
+__device__ __forceinline__ uint2 load_four(const __nv_bfloat16 *row, int k, int K)
 {
-    if (row == nullptr || k >= K) return 0u;
-    if (vec && k + 1 < K) return *reinterpret_cast<const uint32_t *>(row + k);
-    const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
-    return (uint32_t)p[k] | (k + 1 < K ? (uint32_t)p[k + 1] << 16 : 0u);
+    const uint16_t *p = reinterpret_cast<const uint16_t *>(row) + k;
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = k + i < K ? p[i] : 0u;
+    return make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
 }
 
 __device__ __forceinline__ float activate(float v, int act)
@@ -289,35 +294,25 @@ __device__ __forceinline__ float activate(float v, int act)
     return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
 }
 
-// Shared memory: [ring of every warp | the warps' sums, over the ring][the CTA's sums][barriers][tables]
+// Shared memory: [the warps' sums][the CTA's sums][tables]
 template <int MB, int NT>
 struct Lay {
     static constexpr int kTok = NT ? 8 * NT : 1;
-    static constexpr int kRing = Fmt<MB>::kStages * Fmt<MB>::kStage;      // of one warp
     static constexpr int kSums = kTok * kPitch * 4;                       // of one warp
-    static constexpr int kWarp = kRing > kSums ? kRing : kSums;
-    // behind the warps' memory:
+    // behind the warps' sums:
     static constexpr int kPart = 0;                                       // [kTok][128] floats
     static constexpr int kMap = kPart + kTok * 128 * 4;                   // 8 words: bit e set where expert e has a token
-    static constexpr int kAbort = kMap + kMaxExperts / 8;                 // a flag for each warp
-    static constexpr int kCount = kAbort + 24 * 4;
-    static constexpr int kBars = kCount + 16;
-    __host__ __device__ static constexpr int tables(int warps) { return kBars + warps * Fmt<MB>::kStages * 8; }
-    // tables: in, each: (slot, weight) of the expert's tokens; out: experts, then the slot of (expert, token); all: the ids
-    static constexpr int kRows = 4 * kMaxExperts;
-    __host__ __device__ static constexpr int ids(int mode, int warps) { return tables(warps) + (mode == kExpertsOut ? kRows + 2 * kMaxExperts * kTok : kRows); }
+    static constexpr int kCount = kMap + kMaxExperts / 8;
+    static constexpr int kList = kCount + 16;                             // in, each: (slot, weight) of the expert's tokens; out: experts
+    static constexpr int kRows = kList + 4 * kMaxExperts;                 // out: the slot of (expert, token)
+    __host__ __device__ static constexpr int ids(int mode) { return mode == kExpertsOut ? kRows + 2 * kMaxExperts * kTok : kRows; }
     static constexpr int bytes(int mode, int warps)
     {
-        return warps * kWarp + (mode == kMatvec ? tables(warps) : ids(mode, warps) + (NT ? 4 * kMaxFewRows * kMaxTop : 0));
+        return warps * kSums + (mode == kMatvec ? kMap : ids(mode) + (NT ? 4 * kMaxFewRows * kMaxTop : 0));
     }
 };
 
-// The ring of a warp: the stage of its next tile row and that stage's parity.
-struct Ring {
-    int st, phase;
-};
-
-// What a warp works on: `units` tile rows of (expert, tile row) pairs, its own share of them, and its ring.
+// What a CTA works on: `units` tile rows, in the out form of (expert, tile row) pairs.
 struct Work {
     int n_tok, tok0;             // tokens of this pass; the first one
     bool begin;                  // the first pass of this CTA
@@ -329,34 +324,39 @@ struct Work {
 
 // The sums of this warp's share of the tile rows, left in sums[warp][token][j][g][2].  SINGLE: one token (NT = 1 then).
 template <int MB, int NT, int MODE, bool SINGLE>
-__device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *smem, uint64_t *bars, volatile int *abort_flag, Ring &R, int group, int me,
-                                         int workers, int tok_pitch)
+__device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *smem, int group, int me, int workers, int tok_pitch)
 {
     using F = Fmt<MB>;
-    constexpr int S = F::kStages;
     constexpr int PIECES = from_h(MODE) ? 2 : 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    uint8_t *ring = smem + warp * Lay<MB, SINGLE ? 0 : NT>::kRing;
     const int64_t image = (int64_t)A.Kt * A.Nt * F::kRec, row_bytes = (int64_t)A.Nt * F::kRec;
     const uint32_t each = (uint32_t)W.units / (uint32_t)workers, extra = (uint32_t)W.units - each * workers;
     const int u0 = (int)(me * each + min((uint32_t)me, extra)), n = (int)(each + ((uint32_t)me < extra));
     const int s0 = MODE == kExpertsOut ? (int)((uint32_t)u0 / (uint32_t)A.Kt) : 0, kt0 = u0 - s0 * A.Kt;
+
+    // Lane group g reads face column (g >> 1) & 1 of tile (g & 1) + 2 * (g >> 2) of the column group; of gated experts the
+    // last two tiles are the up matrix's.  Tiles past the last column are read as the first one and dropped.
     const bool gated = MODE == kExpertsIn && A.w1 != nullptr;
     const int span = gated ? kGroupTiles / 2 : kGroupTiles;
-    const int64_t col_off = (int64_t)group * span * F::kRec;
-    const uint32_t bytes = (uint32_t)min(span, A.Nt - group * span) * F::kRec;
+    int tile = (g & 1) | ((g >> 2) << 1);
+    const uint8_t *matrix = A.w0;
+    if (gated && tile >= span) {
+        tile -= span;
+        matrix = A.w1;
+    }
+    const int col = group * span + tile, fc = (g >> 1) & 1;
+    matrix += (int64_t)(col < A.Nt ? col : group * span) * F::kRec;
 
-    const bool vec = from_h(MODE) || ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 3) == 0;
-    const int whole = from_h(MODE) ? A.Kt : vec ? A.K / 32 : 0;    // tile rows whose activations are plain pairs
-    // lane group g reads face column (g >> 1) & 1 of tile (g & 1) + 2 * (g >> 2): neighbours in g are records apart, which
-    // puts the 8 lanes of a 128-bit access in distinct banks
-    const int fc = (g >> 1) & 1, odd = g & 1;
-    const uint32_t rec_off = ((g & 1) | ((g >> 2) << 1)) * F::kRec;
-    const uint32_t sel_flip = MB == 7 && odd ? 0x4444u : 0u;
+    const bool vec = from_h(MODE) || ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 7) == 0;
+    const int whole = from_h(MODE) ? A.Kt : vec ? A.K / 32 : 0;    // tile rows whose activations are loaded four at a time
 
+    // What a lane needs of one tile row: its rows of the upper and the lower face, and token g's activations beside them.  Lanes
+    // past the last token read the first one's row: their columns of the product are dropped.
+    struct Part {
+        Raw<MB> raw[2];
+        uint2 x[2][PIECES][NT];
+    };
     float acc[8][NT][4];
-    bool ok = true;
-    int st = R.st, phase = R.phase;   // kept over both sweeps
     uint32_t seen = 0;                // all shared exponents met, ORed
 
     // One sweep over the share.  The first one takes every step as it usually is and looks afterwards whether one was not (an
@@ -369,34 +369,20 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int v = 0; v < 4; v++) acc[j][nt][v] = 0.0f;
-        // the copies of the next tile row to ask for
-        int i_s = s0, i_kt = kt0, i_st = st;
-        int64_t i_off = (MODE == kExpertsOut ? (n > 0 ? W.list[s0] * image : 0) : W.w_off) + kt0 * row_bytes + col_off;
-        auto issue = [&]() {
-            uint8_t *dst = ring + i_st * F::kStage;
-            uint64_t *bar = bars + i_st;
-            mbar_arrive_expect_tx(bar, gated ? 2 * bytes : bytes);
-            bulk_g2s(dst, A.w0 + i_off, bytes, bar);
-            if (gated) bulk_g2s(dst + F::kStage / 2, A.w1 + i_off, bytes, bar);
-            i_st = i_st + 1 == S ? 0 : i_st + 1;
-            i_off += row_bytes;
-            if (MODE == kExpertsOut && ++i_kt == A.Kt) {
-                i_kt = 0;
-                if (++i_s * A.Kt < W.units) i_off = W.list[i_s] * image + col_off;
+        int w_s = s0, w_kt = kt0;
+        const uint8_t *at = matrix + (MODE == kExpertsOut ? (n > 0 ? W.list[s0] * image : 0) : W.w_off) + kt0 * row_bytes;
+        auto load_w = [&](Part &P) {
+#pragma unroll
+            for (int f = 0; f < 2; f++) {
+                const int face = 2 * f + fc;
+                load_raw<MB>(P.raw[f], at + 64 + face * F::kFace + 4 * t * F::kRow, at + face * 16 + 4 * t);
+            }
+            at += row_bytes;
+            if (MODE == kExpertsOut && ++w_kt == A.Kt) {
+                w_kt = 0;
+                if (++w_s * A.Kt < W.units) at = matrix + W.list[w_s] * image;
             }
         };
-        __syncwarp();
-        if (lane == 0)
-            for (int i = 0; i < min(S, n); i++) issue();
-        // The weights were asked for before what the launch in front of this one computes is waited for: it writes activations,
-        // never weights, and what was in front of that one was complete before it let this launch begin.
-        if (!WIDE && W.begin) {
-            if (MODE != kExpertsIn) griddep_wait();
-            if (MODE == kMatvec) griddep_launch();
-        }
-
-        // The tokens' values of one tile row: lane (g, t) holds token g, k = 2t, 2t+1, 2t+8, 2t+9 of both face rows.  Lanes past
-        // the last token read the first one's row: their columns of the product are dropped.
         const __nv_bfloat16 *xp[NT];
         uint32_t present[NT];             // experts-out: all ones where the token has this expert
         int x_s = s0, x_kt = kt0;
@@ -417,107 +403,97 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
                     if (r < 0) present[nt] = 0u;
                     xp[nt] = A.h + (int64_t)max(r, 0) * 2 * A.hpad;
                 }
-                xp[nt] += x_kt * 32 + 2 * t;
+                xp[nt] += x_kt * 32 + 4 * t;
             }
         };
-        uint32_t xb[2][PIECES][NT][2], ahead[2][PIECES][NT][2];   // this tile row's, and the next one's on their way
-        auto load_x = [&]() {
+        auto load_x = [&](Part &P) {
             if (MODE == kExpertsOut && x_kt == A.Kt) {
                 x_kt = 0;
                 x_s++;
                 rows_of();
             }
-            if (from_h(MODE) || x_kt < whole) {
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int q = 0; q < PIECES; q++) {
-                        const uint32_t *at = reinterpret_cast<const uint32_t *>(xp[nt] + q * A.hpad);
+                for (int f = 0; f < 2; f++) {
+                    if (from_h(MODE) || x_kt < whole) {
 #pragma unroll
-                        for (int f = 0; f < 2; f++)
-#pragma unroll
-                            for (int p = 0; p < 2; p++) {
-                                if (from_h(MODE)) ahead[f][q][nt][p] = __ldcg(at + f * 8 + p * 4);
-                                else ahead[f][q][nt][p] = at[f * 8 + p * 4];
-                                if (MODE == kExpertsOut && !SINGLE) ahead[f][q][nt][p] &= present[nt];
+                        for (int q = 0; q < PIECES; q++) {
+                            const uint2 *p = reinterpret_cast<const uint2 *>(xp[nt] + q * A.hpad + f * 16);
+                            uint2 v = from_h(MODE) ? __ldcg(p) : *p;
+                            if (MODE == kExpertsOut && !SINGLE) {
+                                v.x &= present[nt];
+                                v.y &= present[nt];
                             }
+                            P.x[f][q][nt] = v;
+                        }
+                    } else {
+                        P.x[f][0][nt] = load_four(xp[nt] - x_kt * 32 - 4 * t, x_kt * 32 + f * 16 + 4 * t, A.K);
                     }
-            } else {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int v = 0; v < 4; v++)
-                        ahead[v >> 1][0][nt][v & 1] = load_pair(xp[nt] - x_kt * 32 - 2 * t, x_kt * 32 + v * 8 + 2 * t, A.K, vec);
-            }
+                }
             x_kt++;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) xp[nt] += 32;
         };
-        if (n > 0) {
-            rows_of();
-            load_x();
-        }
-        int done = 0;
-        for (; done < n; done++) {
-#pragma unroll
-            for (int v = 0; v < 4 * PIECES * NT; v++) (&xb[0][0][0][0])[v] = (&ahead[0][0][0][0])[v];
-            if (done + 1 < n) load_x();
-            ok = __all_sync(0xffffffffu, mbar_try_wait(bars + st, phase));
-            if (!ok) {
-                ok = mbar_wait_bounded(bars + st, phase, const_cast<int *>(abort_flag), A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-            }
-            const uint8_t *rec = ring + st * F::kStage + rec_off;
+        auto compute = [&](const Part &P) {
 #pragma unroll
             for (int f = 0; f < 2; f++) {
-                const int face = 2 * f + fc;
-                Raw<MB> raw;
-                load_raw<MB>(raw, rec + 64 + face * F::kFace, t, odd);
-                uint32_t e[2];
-                e[0] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t);
-                e[1] = *reinterpret_cast<const uint16_t *>(rec + face * 16 + 2 * t + 8);
-                if constexpr (SINGLE) {
-                    uint32_t b[PIECES][2];
-                    if constexpr (WIDE) {
-#pragma unroll
-                        for (int q = 0; q < PIECES; q++) b[q][0] = xb[f][q][0][0], b[q][1] = xb[f][q][0][1];
-                        single_step_wide<MB, PIECES>(acc, raw, e, sel_flip, A, b);
-                    } else {
-                        seen |= e[0] | e[1];
-#pragma unroll
-                        for (int p = 0; p < 2; p++) {
-                            const uint32_t s = scale_pair(e[p], -kDown);
-#pragma unroll
-                            for (int q = 0; q < PIECES; q++) b[q][p] = mul_bf16x2(xb[f][q][0][p], s);
-                        }
-                        single_step<MB, PIECES>(acc, raw, sel_flip, A, b);
-                    }
+                const Raw<MB> &raw = P.raw[f];
+                if (!WIDE) seen |= raw.e;
+                if constexpr (!SINGLE) {
+                    step<MB, NT, PIECES, WIDE>(acc, raw, A, P.x[f]);
+                } else if constexpr (WIDE) {
+                    single_step_wide<MB, PIECES>(acc, raw, A, P.x[f]);
                 } else {
-                    if (!WIDE) seen |= e[0] | e[1];
-                    step<MB, NT, PIECES, WIDE>(acc, raw, e, sel_flip, A, xb[f]);
+                    uint32_t b[PIECES][2];
+#pragma unroll
+                    for (int q = 0; q < PIECES; q++) {
+                        b[q][0] = mul_bf16x2(P.x[f][q][0].x, scale_pair(raw.e, 0, -kDown));
+                        b[q][1] = mul_bf16x2(P.x[f][q][0].y, scale_pair(raw.e, 1, -kDown));
+                    }
+                    single_step<MB, PIECES>(acc, raw, A, b);
                 }
             }
-            __syncwarp();
-            if (lane == 0 && done + S < n) issue();
-            if (++st == S) {
-                st = 0;
-                phase ^= 1;
+        };
+        Part P0;
+        if constexpr (WIDE) {             // rare: nothing ahead, which leaves the registers to the usual sweep
+            if (n > 0) rows_of();
+#pragma unroll 1
+            for (int i = 0; i < n; i++) {
+                load_w(P0);
+                load_x(P0);
+                compute(P0);
             }
-        }
-        if (!ok) {   // a copy that did not arrive in time: let those in flight land before the memory is given up (again bounded)
-            for (int i = done; i < min(n, done + S); i++) {
-                int own = 0;
-                (void)mbar_wait_bounded(bars + st, phase, &own, A.status, BUDA_DEVSTAT_FEW_ROWS_WAIT);
-                if (++st == S) {
-                    st = 0;
-                    phase ^= 1;
+        } else {
+            if (n > 0) load_w(P0);
+            // The weights were asked for before what the launch in front of this one computes is waited for: it writes activations,
+            // never weights, and what was in front of that one was complete before it let this launch begin.
+            if (W.begin) {
+                if (MODE != kExpertsIn) griddep_wait();
+                if (MODE == kMatvec) griddep_launch();
+            }
+            if (n > 0) {
+                rows_of();
+                load_x(P0);
+            }
+            Part P1;
+            for (int i = 0; i < n; i += 2) {
+                if (i + 1 < n) {
+                    load_w(P1);
+                    load_x(P1);
                 }
+                compute(P0);
+                if (i + 1 >= n) break;
+                if (i + 2 < n) {
+                    load_w(P0);
+                    load_x(P0);
+                }
+                compute(P1);
             }
         }
     };
     sweep(std::false_type());
-    bool again = (seen & 0x8080u) != 0;
+    bool again = (seen & 0x80808080u) != 0;
     if constexpr (SINGLE) {
         float z = 0.0f;                   // a sum of zeros, unless something is not finite
 #pragma unroll
@@ -526,11 +502,8 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
             for (int v = 0; v < 4; v++) z = fmaf(acc[j][0][v], 0.0f, z);
         again |= z != 0.0f;
     }
-    if (__any_sync(0xffffffffu, again) && ok) sweep(std::true_type());
+    if (__any_sync(0xffffffffu, again)) sweep(std::true_type());
 
-    R.st = st;
-    R.phase = phase;
-    __syncthreads();                      // every warp is done with its ring: the sums take its place
     float *sums = reinterpret_cast<float *>(smem);
     if constexpr (SINGLE) {
         if (t == (g >> 1))
@@ -564,23 +537,12 @@ __global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(MB, NT, MODE), 
     const int c = A.cluster, threads = blockDim.x, warps = threads >> 5;
     const int rank = c > 1 ? (int)cluster_rank() : 0;
     const int group = blockIdx.x / c;
-    uint8_t *base = smem + warps * L::kWarp;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(base + L::kBars) + warp * F::kStages;
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(base + L::kAbort) + warp;
+    uint8_t *base = smem + warps * L::kSums;
     uint32_t *map = reinterpret_cast<uint32_t *>(base + L::kMap);
     volatile int *found_at = reinterpret_cast<volatile int *>(base + L::kCount);
-    int *list = reinterpret_cast<int *>(base + L::tables(warps));
-    int16_t *rows = reinterpret_cast<int16_t *>(base + L::tables(warps) + L::kRows);
-    int *ids = reinterpret_cast<int *>(base + L::ids(MODE, warps));
-
-    // ring and flag are this warp's alone: it needs no other to begin
-    if (lane == 0) {
-        for (int i = 0; i < F::kStages; i++) mbar_init(bars + i, 1);
-        *abort_flag = 0;
-        mbar_fence_init();
-    }
-    __syncwarp();
-    Ring R = {0, 0};
+    int *list = reinterpret_cast<int *>(base + L::kList);
+    int16_t *rows = reinterpret_cast<int16_t *>(base + L::kRows);
+    int *ids = reinterpret_cast<int *>(base + L::ids(MODE));
 
     // ---- which tokens and which matrices
     Work W;
@@ -731,12 +693,9 @@ __global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(MB, NT, MODE), 
     while (true) {
         if (NT != 0 && (MODE == kExpertsIn || MODE == kExpertsEach)) W.n_tok = min(found - W.tok0, L::kTok);
         if constexpr (NT == 0) {
-            products<MB, 1, MODE, true>(A, W, smem, bars, abort_flag, R, group, me, workers, 1);
-        } else if constexpr (MODE == kExpertsIn || MODE == kExpertsEach) {
-            if (W.n_tok == 1) products<MB, 1, MODE, true>(A, W, smem, bars, abort_flag, R, group, me, workers, L::kTok);
-            else products<MB, NT, MODE, false>(A, W, smem, bars, abort_flag, R, group, me, workers, L::kTok);
+            products<MB, 1, MODE, true>(A, W, smem, group, me, workers, 1);
         } else {
-            products<MB, NT, MODE, false>(A, W, smem, bars, abort_flag, R, group, me, workers, L::kTok);
+            products<MB, NT, MODE, false>(A, W, smem, group, me, workers, L::kTok);
         }
 
         // join the warps, and the CTAs of a cluster (each finishes its share of the outputs)
@@ -790,8 +749,7 @@ __global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(MB, NT, MODE), 
         if (NT == 0 || MODE == kMatvec || MODE == kExpertsOut || W.tok0 + L::kTok >= found) break;
         W.tok0 += L::kTok;
         W.begin = false;
-        fence_async_smem();                            // the sums were written where the next copies land
-        __syncthreads();
+        __syncthreads();                               // the sums are read: they may be written again
     }
 }
 
@@ -910,19 +868,18 @@ cudaError_t dispatch(int mant_bits, int nt, Args &a, int groups, double copies, 
 using namespace few;
 
 cudaError_t launch_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, const void *W, int64_t N, int mant_bits, void *Y, int64_t ldy,
-                              int out_f32, int sm_count, cudaStream_t stream, unsigned int *status)
+                              int out_f32, int sm_count, cudaStream_t stream)
 {
     Args a = {};
     a.x = (const __nv_bfloat16 *)A; a.ldx = lda;
     a.rows = (int)M; a.K = (int)K; a.Kt = (int)((K + 31) / 32); a.N = (int)N; a.Nt = (int)((N + 31) / 32);
     a.w0 = (const uint8_t *)W;
     a.out = Y; a.ldo = ldy; a.out_f32 = out_f32;
-    a.status = status;
     const int nt = groups_of_8(a.rows), groups = (a.Nt + kGroupTiles - 1) / kGroupTiles, passes = (a.rows + 31) / 32;
     return dispatch<kMatvec>(mant_bits, nt, a, groups, passes, a.Kt, passes, sm_count, stream);
 }
 
-cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stream, unsigned int *status)
+cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stream)
 {
     const int Ht = (m.H + 31) / 32, It = (m.I + 31) / 32;
     const int slots = m.T * m.top, most = m.E < slots ? m.E : slots;
@@ -936,7 +893,6 @@ cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stre
     a.w0 = (const uint8_t *)m.gate; a.w1 = (const uint8_t *)m.up;
     a.ids = m.ids; a.wts = m.weights; a.top = m.top; a.E = m.E; a.act = m.act;
     a.h = (__nv_bfloat16 *)m.h; a.hpad = 32 * It;
-    a.status = status;
     const int span = m.up ? kGroupTiles / 2 : kGroupTiles;
     cudaError_t e = dispatch<kExpertsIn>(m.mant_bits, nt, a, (It + span - 1) / span, reached, Ht, most, sm_count, stream);
     if (e != cudaSuccess) return e;

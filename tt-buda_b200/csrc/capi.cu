@@ -42,10 +42,10 @@ cudaError_t launch_i8_gemm(const void *A, int64_t M, int64_t K, int64_t lda, con
                            int64_t scale_len, float zero_point, int out_mode, void *C, int64_t ldc, int sm_count, cudaStream_t stream,
                            unsigned int *status, char *err, size_t err_len);
 cudaError_t launch_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, const void *W, int64_t N, int mant_bits, void *Y, int64_t ldy,
-                              int out_f32, int sm_count, cudaStream_t stream, unsigned int *status);
+                              int out_f32, int sm_count, cudaStream_t stream);
 cudaError_t launch_moe_route(const void *x, int64_t ldx, int T, int H, const void *w, int w_f32, int64_t ldw, int E, int top, int renorm,
                              float *weights, int *ids, int sm_count, cudaStream_t stream);
-cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stream, unsigned int *status);
+cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stream);
 
 // One CTA, one thread waiting: the barrier expects one arrival that never comes.  The other 31 lanes only take part in
 // the final warp convergence.  The wait is the product kernels' own mbar_wait_bounded with a caller-given limit.
@@ -1377,7 +1377,7 @@ int buda_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, const void
     if (misaligned(W_tiles, 16)) return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: weight images must be 16-byte aligned");
     if (misaligned(Y, y_df == BUDA_DF_Float32 ? 4 : 2)) return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: misaligned output");
     cudaError_t e = launch_bfp_matvec(A, M, K, lda, W_tiles, N, bfp_mant_bits(w_df), Y, ldy, y_df == BUDA_DF_Float32, ctx->sm_count,
-                                      (cudaStream_t)stream, ctx->status);
+                                      (cudaStream_t)stream);
     if (e != cudaSuccess) return cuda_fail(e, "bfp_matvec launch failed");
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return BUDA_SUCCESS;
@@ -1453,7 +1453,7 @@ static int run_experts(DevCtx *ctx, const void *X, int64_t T, int64_t H, int64_t
     m.weights = weights; m.ids = ids;
     m.gate = gate; m.up = up; m.down = down;
     m.y = Y; m.ldy = ldy; m.h = workspace;
-    cudaError_t e = launch_moe_experts(m, ctx->sm_count, (cudaStream_t)stream, ctx->status);
+    cudaError_t e = launch_moe_experts(m, ctx->sm_count, (cudaStream_t)stream);
     if (e != cudaSuccess) return cuda_fail(e, "moe_experts launch failed");
     g_launches.fetch_add(T > kOneSum ? 3 : 2, std::memory_order_relaxed);
     return BUDA_SUCCESS;
