@@ -350,11 +350,12 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     const bool vec = from_h(MODE) || ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 7) == 0;
     const int whole = from_h(MODE) ? A.Kt : vec ? A.K / 32 : 0;    // tile rows whose activations are loaded four at a time
 
-    // What a lane needs of one tile row: its rows of the upper and the lower face, and token g's activations beside them.  Lanes
-    // past the last token read the first one's row: their columns of the product are dropped.
+    // What a lane loads ahead: its rows of one face or of the upper and the lower one, and token g's activations beside them.
+    // Lanes past the last token read the first one's row: their columns of the product are dropped.
+    constexpr int HALVES = MB == 7 || NT > 1 ? 1 : 2;      // by registers
     struct Part {
-        Raw<MB> raw[2];
-        uint2 x[2][PIECES][NT];
+        Raw<MB> raw[HALVES];
+        uint2 x[HALVES][PIECES][NT];
     };
     float acc[8][NT][4];
     uint32_t seen = 0;                // all shared exponents met, ORed
@@ -369,14 +370,14 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int v = 0; v < 4; v++) acc[j][nt][v] = 0.0f;
-        int w_s = s0, w_kt = kt0;
-        const uint8_t *at = matrix + (MODE == kExpertsOut ? (n > 0 ? W.list[s0] * image : 0) : W.w_off) + kt0 * row_bytes;
-        auto load_w = [&](Part &P) {
-#pragma unroll
-            for (int f = 0; f < 2; f++) {
-                const int face = 2 * f + fc;
-                load_raw<MB>(P.raw[f], at + 64 + face * F::kFace + 4 * t * F::kRow, at + face * 16 + 4 * t);
-            }
+        int w_s = s0, w_kt = kt0, x_s = s0, x_kt = kt0;     // the tile rows that weights and activations are asked for
+        const int64_t first = kt0 * row_bytes + (MODE == kExpertsOut ? (n > 0 ? W.list[s0] * image : 0) : W.w_off);
+        const uint8_t *at = matrix + first;
+        auto load_w = [&](Raw<MB> &raw, int f) {
+            const int face = 2 * f + fc;
+            load_raw<MB>(raw, at + 64 + face * F::kFace + 4 * t * F::kRow, at + face * 16 + 4 * t);
+        };
+        auto next_w = [&]() {
             at += row_bytes;
             if (MODE == kExpertsOut && ++w_kt == A.Kt) {
                 w_kt = 0;
@@ -385,7 +386,6 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
         };
         const __nv_bfloat16 *xp[NT];
         uint32_t present[NT];             // experts-out: all ones where the token has this expert
-        int x_s = s0, x_kt = kt0;
         auto rows_of = [&]() {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
@@ -406,53 +406,48 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
                 xp[nt] += x_kt * 32 + 4 * t;
             }
         };
-        auto load_x = [&](Part &P) {
-            if (MODE == kExpertsOut && x_kt == A.Kt) {
-                x_kt = 0;
-                x_s++;
-                rows_of();
-            }
+        auto load_x = [&](uint2 (&x)[PIECES][NT], int f) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+            for (int nt = 0; nt < NT; nt++) {
+                if (from_h(MODE) || x_kt < whole) {
 #pragma unroll
-                for (int f = 0; f < 2; f++) {
-                    if (from_h(MODE) || x_kt < whole) {
-#pragma unroll
-                        for (int q = 0; q < PIECES; q++) {
-                            const uint2 *p = reinterpret_cast<const uint2 *>(xp[nt] + q * A.hpad + f * 16);
-                            uint2 v = from_h(MODE) ? __ldcg(p) : *p;
-                            if (MODE == kExpertsOut && !SINGLE) {
-                                v.x &= present[nt];
-                                v.y &= present[nt];
-                            }
-                            P.x[f][q][nt] = v;
+                    for (int q = 0; q < PIECES; q++) {
+                        const uint2 *p = reinterpret_cast<const uint2 *>(xp[nt] + q * A.hpad + f * 16);
+                        uint2 v = from_h(MODE) ? __ldcg(p) : *p;
+                        if (MODE == kExpertsOut && !SINGLE) {
+                            v.x &= present[nt];
+                            v.y &= present[nt];
                         }
-                    } else {
-                        P.x[f][0][nt] = load_four(xp[nt] - x_kt * 32 - 4 * t, x_kt * 32 + f * 16 + 4 * t, A.K);
+                        x[q][nt] = v;
                     }
+                } else {
+                    x[0][nt] = load_four(xp[nt] - x_kt * 32 - 4 * t, x_kt * 32 + f * 16 + 4 * t, A.K);
                 }
+            }
+        };
+        auto next_x = [&]() {
             x_kt++;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) xp[nt] += 32;
+            if (MODE == kExpertsOut && x_kt == A.Kt) {
+                x_kt = 0;
+                if (++x_s * A.Kt < W.units) rows_of();
+            }
         };
-        auto compute = [&](const Part &P) {
+        auto compute = [&](const Raw<MB> &raw, const uint2 (&x)[PIECES][NT]) {
+            if (!WIDE) seen |= raw.e;
+            if constexpr (!SINGLE) {
+                step<MB, NT, PIECES, WIDE>(acc, raw, A, x);
+            } else if constexpr (WIDE) {
+                single_step_wide<MB, PIECES>(acc, raw, A, x);
+            } else {
+                uint32_t b[PIECES][2];
 #pragma unroll
-            for (int f = 0; f < 2; f++) {
-                const Raw<MB> &raw = P.raw[f];
-                if (!WIDE) seen |= raw.e;
-                if constexpr (!SINGLE) {
-                    step<MB, NT, PIECES, WIDE>(acc, raw, A, P.x[f]);
-                } else if constexpr (WIDE) {
-                    single_step_wide<MB, PIECES>(acc, raw, A, P.x[f]);
-                } else {
-                    uint32_t b[PIECES][2];
-#pragma unroll
-                    for (int q = 0; q < PIECES; q++) {
-                        b[q][0] = mul_bf16x2(P.x[f][q][0].x, scale_pair(raw.e, 0, -kDown));
-                        b[q][1] = mul_bf16x2(P.x[f][q][0].y, scale_pair(raw.e, 1, -kDown));
-                    }
-                    single_step<MB, PIECES>(acc, raw, A, b);
+                for (int q = 0; q < PIECES; q++) {
+                    b[q][0] = mul_bf16x2(x[q][0].x, scale_pair(raw.e, 0, -kDown));
+                    b[q][1] = mul_bf16x2(x[q][0].y, scale_pair(raw.e, 1, -kDown));
                 }
+                single_step<MB, PIECES>(acc, raw, A, b);
             }
         };
         Part P0;
@@ -460,12 +455,21 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
             if (n > 0) rows_of();
 #pragma unroll 1
             for (int i = 0; i < n; i++) {
-                load_w(P0);
-                load_x(P0);
-                compute(P0);
+#pragma unroll
+                for (int f = 0; f < 2; f++) {
+                    load_w(P0.raw[0], f);
+                    load_x(P0.x[0], f);
+                    compute(P0.raw[0], P0.x[0]);
+                }
+                next_w();
+                next_x();
             }
         } else {
-            if (n > 0) load_w(P0);
+            if (n > 0) {
+#pragma unroll
+                for (int f = 0; f < HALVES; f++) load_w(P0.raw[f], f);
+                if (HALVES == 2) next_w();
+            }
             // The weights were asked for before what the launch in front of this one computes is waited for: it writes activations,
             // never weights, and what was in front of that one was complete before it let this launch begin.
             if (W.begin) {
@@ -474,21 +478,42 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
             }
             if (n > 0) {
                 rows_of();
-                load_x(P0);
+#pragma unroll
+                for (int f = 0; f < HALVES; f++) load_x(P0.x[f], f);
+                if (HALVES == 2) next_x();
             }
             Part P1;
-            for (int i = 0; i < n; i += 2) {
-                if (i + 1 < n) {
-                    load_w(P1);
-                    load_x(P1);
+            if constexpr (HALVES == 2) {
+                auto both = [&](Part &P) {
+                    load_w(P.raw[0], 0);
+                    load_w(P.raw[1], 1);
+                    next_w();
+                    load_x(P.x[0], 0);
+                    load_x(P.x[1], 1);
+                    next_x();
+                };
+                for (int i = 0; i < n; i += 2) {
+                    if (i + 1 < n) both(P1);
+                    compute(P0.raw[0], P0.x[0]);
+                    compute(P0.raw[1], P0.x[1]);
+                    if (i + 1 >= n) break;
+                    if (i + 2 < n) both(P0);
+                    compute(P1.raw[0], P1.x[0]);
+                    compute(P1.raw[1], P1.x[1]);
                 }
-                compute(P0);
-                if (i + 1 >= n) break;
-                if (i + 2 < n) {
-                    load_w(P0);
-                    load_x(P0);
+            } else {
+                for (int i = 0; i < n; i++) {
+                    load_w(P1.raw[0], 1);
+                    load_x(P1.x[0], 1);
+                    next_w();
+                    next_x();
+                    compute(P0.raw[0], P0.x[0]);
+                    if (i + 1 < n) {
+                        load_w(P0.raw[0], 0);
+                        load_x(P0.x[0], 0);
+                    }
+                    compute(P1.raw[0], P1.x[0]);
                 }
-                compute(P1);
             }
         }
     };
