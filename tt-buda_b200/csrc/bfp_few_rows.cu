@@ -14,10 +14,10 @@
 // Bound: bytes of the images (1.0625 / 0.5625 / 0.3125 a weight) -- every weight meets only a few rows.  What decides is
 // how few instructions a weight costs on its way and how much of the images is on its way at once:
 //   * A warp owns 128 output columns (4 tile columns) and walks tile rows.  Each lane loads its own pieces of the records
-//     straight into registers, one tile row ahead: four whole face rows (4t .. 4t+3) of one face, the four exponents beside
-//     them, and the four activations they meet, each as one piece of consecutive bytes; the four lanes of a face read its 128 (Bfp4)
-//     bytes together.  With 16 to 24 warps an SM that is 37 to 55 KB under way.  (The same through bulk copies into a ring of
-//     shared memory took half as many instructions again: barrier, copy issue, second load.)
+//     straight into registers, one tile row ahead: four whole rows (4t .. 4t+3) of a face, the four exponents beside them and
+//     the four activations they meet, each consecutive bytes; the four lanes of a face read its 128 bytes (Bfp4) in one
+//     access.  With 16 warps an SM that is 37 KB under way.  (The same through bulk copies into a ring of shared memory took half as many instructions again:
+//     barrier, copy issue, second load; 11.0 us against 9.8 for 1x4096x16384 Bfp4_b.)
 //   * Decode: a datum's sign and magnitude bits are moved to bit 15 and to the top of the 7 mantissa bits of a
 //     bfloat16, which makes the subnormal number (-1)^s q 2^(-126 - m); a packed multiply by 2^E finishes it, exactly.
 //     One byte permute puts the same byte of two weight rows into both halves of a register in both places, so a pair
@@ -120,44 +120,46 @@ __device__ __forceinline__ uint32_t cluster_rank()
     return r;
 }
 
-// The raw data of one lane: face rows 4t, 4t+1 (p = 0) and 4t+2, 4t+3 (p = 1) of one face, and their exponents.
+// The raw data of one lane for one 16-row step: four face rows, as pairs p = 0 and 1, and their exponents.
 template <int MB>
 struct Raw {
     uint32_t w[2][2][(MB + 1) / 2];   // [p][row][32-bit word]
     uint32_t e;
 };
 
-__device__ __forceinline__ uint4 load_once(const uint8_t *p)
+// 32 bytes that nothing reads again: a whole sector for every lane
+struct Words8 {
+    uint32_t v[8];
+};
+__device__ __forceinline__ Words8 load_sector(const uint8_t *p)
 {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+    Words8 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]), "=r"(r.v[4]), "=r"(r.v[5]), "=r"(r.v[6]), "=r"(r.v[7])
+                 : "l"(p));
+    return r;
 }
 
-// data, exps: this lane's four rows and their exponents
+// A lane's four rows, at `data`
 template <int MB>
-__device__ __forceinline__ void load_raw(Raw<MB> &r, const uint8_t *data, const uint8_t *exps)
+__device__ __forceinline__ void load_rows(Raw<MB> &r, const uint8_t *data)
 {
     if constexpr (MB == 7) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint4 a = load_once(data + 16 * i);
-            uint32_t (&w)[4] = r.w[i >> 1][i & 1];
-            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        for (int p = 0; p < 2; p++) {
+            const Words8 a = load_sector(data + p * 32);
+#pragma unroll
+            for (int i = 0; i < 8; i++) r.w[p][i >> 2][i & 3] = a.v[i];
         }
     } else if constexpr (MB == 3) {
+        const Words8 a = load_sector(data);
 #pragma unroll
-        for (int p = 0; p < 2; p++) {
-            const uint4 a = load_once(data + 16 * p);
-            r.w[p][0][0] = a.x; r.w[p][0][1] = a.y;
-            r.w[p][1][0] = a.z; r.w[p][1][1] = a.w;
-        }
+        for (int i = 0; i < 8; i++) r.w[i >> 2][(i >> 1) & 1][i & 1] = a.v[i];
     } else {
-        const uint4 a = load_once(data);
+        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(data));
         r.w[0][0][0] = a.x; r.w[0][1][0] = a.y;
         r.w[1][0][0] = a.z; r.w[1][1][0] = a.w;
     }
-    r.e = __ldg(reinterpret_cast<const uint32_t *>(exps));
 }
 
 // Weight columns 2j and 2j+1 of the pair of rows p as subnormal bfloat16 pairs (low half: the even row).  The integer pipe, which
@@ -278,9 +280,13 @@ __device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Ra
     }
 }
 
-// Elements k .. k+3 of a row one by one, zero past K.
-__device__ __forceinline__ uint2 load_four(const __nv_bfloat16 *row, int k, int K)
+// Elements k .. k+3 of a row (k a multiple of 4), zero past K; `pairs`: 4-byte loads are allowed.
+__device__ __forceinline__ uint2 load_four(const __nv_bfloat16 *row, int k, int K, bool pairs)
 {
+    if (pairs && k + 4 <= K) {
+        const uint32_t *p = reinterpret_cast<const uint32_t *>(row + k);
+        return make_uint2(p[0], p[1]);
+    }
     const uint16_t *p = reinterpret_cast<const uint16_t *>(row) + k;
     uint32_t v[4];
 #pragma unroll
@@ -348,6 +354,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     matrix += (int64_t)(col < A.Nt ? col : group * span) * F::kRec;
 
     const bool vec = from_h(MODE) || ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 7) == 0;
+    const bool pairs = ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 3) == 0;
     const int whole = from_h(MODE) ? A.Kt : vec ? A.K / 32 : 0;    // tile rows whose activations are loaded four at a time
 
     // What a lane loads ahead: its rows of one face or of the upper and the lower one, and token g's activations beside them.
@@ -373,9 +380,11 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
         int w_s = s0, w_kt = kt0, x_s = s0, x_kt = kt0;     // the tile rows that weights and activations are asked for
         const int64_t first = kt0 * row_bytes + (MODE == kExpertsOut ? (n > 0 ? W.list[s0] * image : 0) : W.w_off);
         const uint8_t *at = matrix + first;
+        // lane t of a quad takes rows 4t .. 4t+3 of the upper (f = 0), then of the lower face
         auto load_w = [&](Raw<MB> &raw, int f) {
             const int face = 2 * f + fc;
-            load_raw<MB>(raw, at + 64 + face * F::kFace + 4 * t * F::kRow, at + face * 16 + 4 * t);
+            load_rows<MB>(raw, at + 64 + face * F::kFace + 4 * t * F::kRow);
+            raw.e = __ldg(reinterpret_cast<const uint32_t *>(at + face * 16 + 4 * t));
         };
         auto next_w = [&]() {
             at += row_bytes;
@@ -413,16 +422,17 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
 #pragma unroll
                     for (int q = 0; q < PIECES; q++) {
                         const uint2 *p = reinterpret_cast<const uint2 *>(xp[nt] + q * A.hpad + f * 16);
-                        uint2 v = from_h(MODE) ? __ldcg(p) : *p;
-                        if (MODE == kExpertsOut && !SINGLE) {
-                            v.x &= present[nt];
-                            v.y &= present[nt];
-                        }
-                        x[q][nt] = v;
+                        x[q][nt] = from_h(MODE) ? __ldcg(p) : *p;
                     }
                 } else {
-                    x[0][nt] = load_four(xp[nt] - x_kt * 32 - 4 * t, x_kt * 32 + f * 16 + 4 * t, A.K);
+                    x[0][nt] = load_four(xp[nt] - x_kt * 32 - 4 * t, x_kt * 32 + f * 16 + 4 * t, A.K, pairs);
                 }
+                if (MODE == kExpertsOut && !SINGLE)
+#pragma unroll
+                    for (int q = 0; q < PIECES; q++) {
+                        x[q][nt].x &= present[nt];
+                        x[q][nt].y &= present[nt];
+                    }
             }
         };
         auto next_x = [&]() {

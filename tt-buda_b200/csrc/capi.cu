@@ -1374,7 +1374,7 @@ int buda_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, const void
     if (M > 1 && ldy < N) return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: output rows of %lld values overlap at a stride of %lld", (long long)N, (long long)ldy);
     if (M == 0) return BUDA_SUCCESS;
     if (!W_tiles || !Y) return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: null matrix pointer");
-    if (misaligned(W_tiles, 16)) return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: weight images must be 16-byte aligned");
+    if (misaligned(W_tiles, 32)) return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: weight images must be 32-byte aligned");
     if (misaligned(Y, y_df == BUDA_DF_Float32 ? 4 : 2)) return fail(BUDA_RUNTIME_ERROR, "bfp_matvec: misaligned output");
     cudaError_t e = launch_bfp_matvec(A, M, K, lda, W_tiles, N, bfp_mant_bits(w_df), Y, ldy, y_df == BUDA_DF_Float32, ctx->sm_count,
                                       (cudaStream_t)stream);
@@ -1433,8 +1433,8 @@ static int check_experts(const void *X, int64_t T, int64_t H, int64_t ldx, const
     if (act != BUDA_ACT_SILU && act != BUDA_ACT_GELU) return fail(BUDA_RUNTIME_ERROR, "moe_experts: unknown activation %d", act);
     if (T > 1 && ldy < H) return fail(BUDA_RUNTIME_ERROR, "moe_experts: output rows of %lld values overlap at a stride of %lld", (long long)H, (long long)ldy);
     if (!gate || !down || (T && (!weights || !ids || !Y || !workspace))) return fail(BUDA_RUNTIME_ERROR, "moe_experts: null pointer");
-    if (misaligned(gate, 16) || misaligned(up, 16) || misaligned(down, 16) || misaligned(workspace, 16))
-        return fail(BUDA_RUNTIME_ERROR, "moe_experts: weight images and the workspace must be 16-byte aligned");
+    if (misaligned(gate, 32) || misaligned(up, 32) || misaligned(down, 32) || misaligned(workspace, 16))
+        return fail(BUDA_RUNTIME_ERROR, "moe_experts: weight images must be 32-byte, the workspace 16-byte aligned");
     if (misaligned(weights, 4) || misaligned(ids, 4) || misaligned(Y, 2)) return fail(BUDA_RUNTIME_ERROR, "moe_experts: misaligned pointer");
     if ((uint64_t)moe_workspace(T, top, H, I) > workspace_bytes)
         return fail(BUDA_RUNTIME_ERROR, "moe_experts: workspace of %llu bytes, %lld are needed", (unsigned long long)workspace_bytes,
