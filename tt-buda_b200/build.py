@@ -1,6 +1,6 @@
 """In-tree build of the native parts: libbuda_cuda.so (CUDA kernels + C ABI, sm_100a only), the
-pybind11 module pybuda._C (C++ host layer that calls the C ABI), and libbuda_probe.so (bare streaming
-kernels that only the benchmark loads).
+pybind11 module pybuda._C (C++ host layer that calls the C ABI), pybuda._torch_ops (the few-row
+operators on torch tensors) and libbuda_probe.so (bare streaming kernels that only the benchmark loads).
 
     python tt-buda_b200/build.py [--force]
 
@@ -113,9 +113,31 @@ def build_pybind(force=False):
     return target
 
 
+def torch_ops_target():
+    return os.path.join(HERE, "pybuda", "_torch_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_torch_ops(force=False):
+    """pybuda._torch_ops: the operators whose calls are too short for ctypes, on torch tensors (torch's headers and libraries)."""
+    target = torch_ops_target()
+    src = os.path.join(HOST_DIR, "torch_ops", "few_rows.cpp")
+    if not (force or _newer(target, [src, os.path.join(INCLUDE, "buda_cuda.h")])):
+        return target
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    inc = [INCLUDE, sysconfig.get_paths()["include"], os.path.join(cuda_home, "include")] + cpp_extension.include_paths()
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] +
+         [a for i in inc for a in ("-isystem", i)] + [src, "-o", target, "-L", LIB_DIR, "-lbuda_cuda", "-Wl,-rpath,$ORIGIN/../lib"] +
+         [a for d in cpp_extension.library_paths() for a in ("-L", d)] + ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"])
+    return target
+
+
 def build_all(force=False, verbose=False):
     lib = build_cuda(force=force, verbose=verbose)
     mod = build_pybind(force=force) if os.path.isdir(HOST_DIR) else None
+    build_torch_ops(force=force)
     return lib, mod
 
 

@@ -12,6 +12,13 @@ import torch
 from . import _cabi
 from ._cabi import QueueGeom, check
 
+try:
+    from . import _torch_ops
+except ImportError as e:
+    raise ImportError("pybuda._torch_ops is missing or does not load: build it with `python tt-buda_b200/build.py`") from e
+
+_torch_ops.set_error(_cabi.BudaError)
+
 
 class DF(enum.IntEnum):
     """Integer values of the reference's DataFormat (pybuda/csrc/lower_to_buda/common.hpp:92-111)."""
@@ -214,71 +221,12 @@ def bfp8b_matmul(a, w_image, n, out=None):
     return out
 
 
-_ACTIVATIONS = {"silu": 0, "gelu": 1}
-_RECORD_BYTES = {DF.Bfp8_b: 1088, DF.Bfp4_b: 576, DF.Bfp2_b: 320}   # a tile record without header
-
-
-def _few_rows_check(what, x, images, rows, cols, w_df):
-    """Activations and the images of [rows, cols] matrices, all on one device and as the kernels read them."""
-    if w_df not in _RECORD_BYTES:
-        raise RuntimeError(f"{what}: weights must be Bfp8_b, Bfp4_b or Bfp2_b, got {w_df}")
-    if x.dtype != torch.bfloat16 or x.dim() != 2 or (x.shape[1] != 1 and x.stride(1) != 1):
-        raise RuntimeError(f"{what}: activations must be a bfloat16 matrix with dense rows")
-    if not x.is_cuda or images.device != x.device:
-        raise RuntimeError(f"{what}: works on CUDA tensors of one device only (no CPU fallback)")
-    if images.dtype != torch.uint8 or not images.is_contiguous():
-        raise RuntimeError(f"{what}: queue images are contiguous uint8 tensors")
-    return ((rows + 31) // 32) * ((cols + 31) // 32) * _RECORD_BYTES[w_df]
-
-
-def _output(what, out, x, rows, cols, dtype):
-    if out is None:
-        return torch.empty((rows, cols), dtype=dtype, device=x.device)
-    if out.shape != (rows, cols) or out.dtype != dtype or out.device != x.device or (cols != 1 and out.stride(1) != 1):
-        raise RuntimeError(f"{what}: out must be a {dtype} [{rows}, {cols}] tensor with dense rows on {x.device}")
-    return out
-
-
-def _launch(device, entry, *args):
-    """One C call on the current stream of `device`, whichever device is current.  (torch.cuda.current_stream() builds a Stream
-    object: 4 us, half of what a few-row call costs on the host.)"""
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
-        rc = entry(*args, stream)
-    else:
-        with torch.cuda.device(device):
-            rc = entry(*args, stream)
-    if rc:
-        check(rc)
-
-
 def bfp_matvec(a, w_image, n, w_df=DF.Bfp4_b, out=None, out_dtype=torch.bfloat16):
     """A @ W for a few rows: A bfloat16 [M,K] with M <= 64, W the Bfp8_b / Bfp4_b / Bfp2_b queue image of a [K,n] tensor
     (default geometry, no header; K and n that fill no tile: the image of the zero-padded tensor).  Returns [M,n] in
     out_dtype (bfloat16 or float32), or writes `out` (dense rows, must not overlap a).  Every image byte is read once;
     bfp8b_matmul is the one for many rows."""
-    need = _few_rows_check("bfp_matvec", a, w_image, a.shape[-1], n, w_df)
-    if w_image.numel() < need:
-        raise RuntimeError(f"bfp_matvec: the queue image holds {w_image.numel()} bytes, needs {need}")
-    m, k = a.shape
-    if out is not None:
-        out_dtype = out.dtype
-    if out_dtype not in (torch.bfloat16, torch.float32):
-        raise RuntimeError("bfp_matvec: the output is bfloat16 or float32")
-    out = _output("bfp_matvec", out, a, m, n, out_dtype)
-    _launch(a.device, _cabi.lib.buda_bfp_matvec, a.data_ptr(), m, k, a.stride(0), w_image.data_ptr(), n, w_df, out.data_ptr(),
-            out.stride(0), 5 if out_dtype == torch.bfloat16 else 0)
-    return out
-
-
-def _router_check(x, w_router):
-    if x.dtype != torch.bfloat16 or x.dim() != 2 or (x.shape[1] != 1 and x.stride(1) != 1):
-        raise RuntimeError("moe_route: activations must be a bfloat16 matrix with dense rows")
-    if not x.is_cuda or w_router.device != x.device:
-        raise RuntimeError("moe_route: works on CUDA tensors of one device only (no CPU fallback)")
-    if w_router.dtype not in (torch.bfloat16, torch.float32) or w_router.dim() != 2 or w_router.shape[1] != x.shape[1] or \
-            (w_router.shape[1] != 1 and w_router.stride(1) != 1):
-        raise RuntimeError(f"moe_route: router weights must be a bfloat16 or float32 [experts, {x.shape[1]}] matrix with dense rows")
+    return _torch_ops.bfp_matvec(a, w_image, n, w_df, out, out_dtype)
 
 
 def moe_route(x, w_router, top, renormalize=True):
@@ -286,34 +234,7 @@ def moe_route(x, w_router, top, renormalize=True):
     Returns (weights float32 [T,top], ids int32 [T,top]): for each token the experts of the largest scores x @ w_router.T in
     descending order (of equal ones the lowest index first; NaN ranks last) and their softmax values, with `renormalize`
     divided by their sum.  T <= 64, E <= 256, top <= 16."""
-    _router_check(x, w_router)
-    t, e = x.shape[0], w_router.shape[0]
-    weights = torch.empty((t, max(int(top), 0)), dtype=torch.float32, device=x.device)
-    ids = torch.empty(weights.shape, dtype=torch.int32, device=x.device)
-    _launch(x.device, _cabi.lib.buda_moe_route, x.data_ptr(), t, x.shape[1], x.stride(0), w_router.data_ptr(),
-            5 if w_router.dtype == torch.bfloat16 else 0, w_router.stride(0), e, top, renormalize, weights.data_ptr(), ids.data_ptr())
-    return weights, ids
-
-
-def _experts_check(x, gate, up, down, inter, w_df, activation):
-    if activation not in _ACTIVATIONS:
-        raise RuntimeError(f"moe_experts: activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
-    experts, hidden = gate.shape[0], x.shape[-1]
-    for images, rows, cols in ((gate, hidden, inter), (up, hidden, inter), (down, inter, hidden)):
-        if images is None:
-            continue
-        need = _few_rows_check("moe_experts", x, images, rows, cols, w_df)
-        if images.shape != (experts, need):
-            raise RuntimeError(f"moe_experts: the {experts} experts' images of a [{rows}, {cols}] matrix are a [{experts}, {need}] tensor, "
-                               f"got {list(images.shape)}")
-    return experts
-
-
-def _workspace(x, top, inter, more=0):
-    nbytes = _cabi.lib.buda_moe_workspace_bytes(x.shape[0], top, x.shape[1], inter)
-    if nbytes < 0:
-        raise _cabi.BudaError(_cabi.RUNTIME_ERROR, _cabi.last_error())
-    return torch.empty(nbytes + more, dtype=torch.uint8, device=x.device)
+    return _torch_ops.moe_route(x, w_router, top, renormalize)
 
 
 def moe_experts(x, weights, ids, gate, up, down, inter, w_df=DF.Bfp4_b, activation="silu", out=None):
@@ -325,36 +246,13 @@ def moe_experts(x, weights, ids, gate, up, down, inter, w_df=DF.Bfp4_b, activati
     gate, up, down: uint8 [E, bytes], each row the queue image of a [H,inter] (down: [inter,H]) tensor of format w_df --
     tilize_pack of a [1,E,H,inter] tensor, viewed as E rows; up None: experts without a gate, act(x @ gate) alone.
     activation "silu" or "gelu" (by erf).  Returns bfloat16 [T,H], or writes `out`, which may be x."""
-    experts = _experts_check(x, gate, up, down, inter, w_df, activation)
-    t, hidden = x.shape
-    if ids.dtype != torch.int32 or weights.dtype != torch.float32 or ids.dim() != 2 or ids.shape[0] != t or ids.shape != weights.shape or \
-            not ids.is_contiguous() or not weights.is_contiguous() or ids.device != x.device or weights.device != x.device:
-        raise RuntimeError(f"moe_experts: ids (int32) and weights (float32) are contiguous [{t}, top] tensors on {x.device}")
-    top = ids.shape[1]
-    out = _output("moe_experts", out, x, t, hidden, torch.bfloat16)
-    ws = _workspace(x, top, inter)
-    _launch(x.device, _cabi.lib.buda_moe_experts, x.data_ptr(), t, hidden, x.stride(0), weights.data_ptr(), ids.data_ptr(), top,
-            gate.data_ptr(), None if up is None else up.data_ptr(), down.data_ptr(), experts, inter, w_df, _ACTIVATIONS[activation],
-            out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel())
-    return out
+    return _torch_ops.moe_experts(x, weights, ids, gate, up, down, inter, w_df, activation, out)
 
 
 def moe_layer(x, w_router, top, gate, up, down, inter, w_df=DF.Bfp4_b, activation="silu", renormalize=True, out=None):
     """A whole mixture-of-experts layer for a few tokens: moe_route, then moe_experts with its choice, as one call whose
     launches overlap.  Arguments as there; returns bfloat16 [T,H], or writes `out`, which may be x."""
-    _router_check(x, w_router)
-    experts = _experts_check(x, gate, up, down, inter, w_df, activation)
-    if w_router.shape[0] != experts:
-        raise RuntimeError(f"moe_layer: the router has {w_router.shape[0]} rows for {experts} experts")
-    t, hidden = x.shape
-    out = _output("moe_layer", out, x, t, hidden, torch.bfloat16)
-    ws = _workspace(x, top, inter, 8 * t * top)      # the choice (weights, ids) behind the intermediate rows
-    choice = ws.data_ptr() + ws.numel() - 8 * t * top
-    _launch(x.device, _cabi.lib.buda_moe_layer, x.data_ptr(), t, hidden, x.stride(0), w_router.data_ptr(),
-            5 if w_router.dtype == torch.bfloat16 else 0, w_router.stride(0), top, renormalize, gate.data_ptr(),
-            None if up is None else up.data_ptr(), down.data_ptr(), experts, inter, w_df, _ACTIVATIONS[activation], choice,
-            choice + 4 * t * top, out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel())
-    return out
+    return _torch_ops.moe_layer(x, w_router, top, gate, up, down, inter, w_df, activation, renormalize, out)
 
 
 def i8_matmul(a, w_image, n, scale=None, zero_point=0.0, out="int32"):
