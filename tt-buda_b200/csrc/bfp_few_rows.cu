@@ -33,6 +33,7 @@
 // the rounded rest, together within 2^-16 of h), so nothing is lost against a binary32 h at twice the tensor work.
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <type_traits>
@@ -850,21 +851,20 @@ int groups_of_8(int rows) { return rows == 1 ? 0 : rows <= 8 ? 1 : rows <= 16 ? 
 struct Split {
     int units, cluster;       // units of 8 warps in a CTA; CTAs
 };
-// First CTAs, one to an SM, while each warp of 8 keeps a tile row; then more warps in a CTA, while each keeps 8 tile rows.
-// Measured (us; B200): 1x1024x1024 Bfp4_b, 8 column groups: 4 CTAs of 8 warps 2.75, 8 of 8 3.30, 1 of 24 3.75.  8x4096x1024
-// Bfp8_b: 8 of 8 4.79, 8 of 16 5.05, 1 of 16 11.5.  1x4096x16384 Bfp4_b, 128 groups: 1 of 8 12.75, 1 of 16 11.0, 1 of 24 11.5, 2 of 8
-// 14.6 (the join over a cluster costs about 2.5).
+// CTAs of a cluster first, one to an SM, while each warp of 8 keeps a tile row, and two to an SM while it keeps two; then more
+// warps in a CTA, while each keeps 4.
+// Measured, us, as CTAs x warps (B200): 1x1024x1024 Bfp4_b, 8 column groups: 4x8 2.46, 8x8 2.91, 1x16 3.19.  8x4096x1024 Bfp8_b, 8
+// groups: 8x8 4.81, 8x16 4.99, 1x16 10.3.  12x4096x4096 Bfp4_b, 32 groups: 8x8 6.70, 4x8 7.91, 4x16 7.06.  1x4096x16384 Bfp4_b,
+// 128 groups: 1x16 9.75, 2x8 10.5, 1x8 12.4.
 Split split_of(int64_t groups, int64_t tile_rows, int sm_count, int per_sm)
 {
-    const int64_t useful = (tile_rows + kUnitWarps - 1) / kUnitWarps;
-    int64_t c = sm_count / groups;
-    c = c < 1 ? 1 : c > 8 ? 8 : c;
-    if (c > useful) c = useful;
-    int64_t u = tile_rows / (c * kUnitWarps * 8);
-    const int64_t room = (int64_t)sm_count * per_sm / (groups * c);
-    if (u > room) u = room;
-    if (u > per_sm) u = per_sm;
-    return {(int)(u < 1 ? 1 : u), (int)c};
+    int64_t c = std::min<int64_t>(sm_count / groups, (tile_rows + kUnitWarps - 1) / kUnitWarps);
+    if (2 * groups <= sm_count) c = std::max(c, std::min<int64_t>(2 * sm_count / groups, tile_rows / (2 * kUnitWarps)));
+    c = std::max<int64_t>(1, std::min<int64_t>(c, 8));
+    int64_t u = tile_rows / (c * kUnitWarps * 4);
+    u = std::min<int64_t>(u, (int64_t)sm_count * per_sm / (groups * c));
+    u = std::max<int64_t>(1, std::min<int64_t>(u, per_sm));
+    return {(int)u, (int)c};
 }
 
 template <int MODE, int MB>
