@@ -16,8 +16,8 @@
 //   * A warp owns 128 output columns (4 tile columns) and walks tile rows.  Each lane loads its own pieces of the records
 //     straight into registers, one tile row ahead: four whole rows (4t .. 4t+3) of a face, the four exponents beside them and
 //     the four activations they meet, each consecutive bytes; the four lanes of a face read its 128 bytes (Bfp4) in one
-//     access.  With 16 warps an SM that is 37 KB under way.  (The same through bulk copies into a ring of shared memory took half as many instructions again:
-//     barrier, copy issue, second load; 11.0 us against 9.8 for 1x4096x16384 Bfp4_b.)
+//     access.  With 16 warps an SM that is 37 KB under way.  (The same through bulk copies into a ring of shared memory took
+//     half as many instructions again: barrier, copy issue, second load; 11.0 us against 9.8 for 1x4096x16384 Bfp4_b.)
 //   * Decode: a datum's sign and magnitude bits are moved to bit 15 and to the top of the 7 mantissa bits of a
 //     bfloat16, which makes the subnormal number (-1)^s q 2^(-126 - m); a packed multiply by 2^E finishes it, exactly.
 //     One byte permute puts the same byte of two weight rows into both halves of a register in both places, so a pair
@@ -49,6 +49,7 @@ constexpr int kPitch = 132;             // floats per token of a warp's sums: 8-
 constexpr int kDown = 24;               // single-token sums are held times 2^-24 (see single_step)
 
 enum { kMatvec = 0, kExpertsIn = 1, kExpertsOut = 2, kExpertsEach = 3 };
+enum { kUsual = 0, kPlain = 1, kWide = 2 };   // forms of a sweep (see products)
 __host__ __device__ constexpr bool from_h(int mode) { return mode == kExpertsOut || mode == kExpertsEach; }
 
 // How many units of 8 warps an SM holds, by registers: 128 a thread suffice for up to 8 tokens and, in the matvec of data below 8
@@ -354,8 +355,8 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     const int col = group * span + tile, fc = (g >> 1) & 1;
     matrix += (int64_t)(col < A.Nt ? col : group * span) * F::kRec;
 
-    const bool vec = from_h(MODE) || ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 7) == 0;
-    const bool pairs = ((reinterpret_cast<uintptr_t>(A.x) | (uintptr_t)(A.ldx * 2)) & 3) == 0;
+    const bool vec = from_h(MODE) || ((reinterpret_cast<uintptr_t>(A.x) | (A.rows > 1 ? (uintptr_t)(A.ldx * 2) : 0)) & 7) == 0;
+    const bool pairs = ((reinterpret_cast<uintptr_t>(A.x) | (A.rows > 1 ? (uintptr_t)(A.ldx * 2) : 0)) & 3) == 0;
     const int whole = from_h(MODE) ? A.Kt : vec ? A.K / 32 : 0;    // tile rows whose activations are loaded four at a time
 
     // What a lane loads ahead: its rows of one face or of the upper and the lower one, and token g's activations beside them.
@@ -369,9 +370,12 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     uint32_t seen = 0;                // all shared exponents met, ORed
 
     // One sweep over the share.  The first one takes every step as it usually is and looks afterwards whether one was not (an
-    // exponent of 128 or more, a column that is no finite number): then all is done again with the exact wide steps.
-    auto sweep = [&](auto wide_tag) {
-        constexpr bool WIDE = decltype(wide_tag)::value;
+    // exponent of 128 or more, a column that is no finite number): then all is done again with the exact wide steps.  The plain
+    // form is for activations that are not aligned.  The usual form's loop has no test in it, so that the compiler schedules
+    // two tile rows as one; the last rows, where activations may end inside a tile row, come behind it (1x4096x16384 Bfp4_b 9.8
+    // -> 8.7 us).
+    auto sweep = [&](auto kind_tag) {
+        constexpr bool WIDE = decltype(kind_tag)::value == kWide, PLAIN = decltype(kind_tag)::value == kPlain;
 #pragma unroll
         for (int j = 0; j < 8; j++)
 #pragma unroll
@@ -416,10 +420,10 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
                 xp[nt] += x_kt * 32 + 4 * t;
             }
         };
-        auto load_x = [&](uint2 (&x)[PIECES][NT], int f) {
+        auto load_x = [&](uint2 (&x)[PIECES][NT], int f, bool inside) {      // inside: the tile row is known to lie inside the rows
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                if (from_h(MODE) || x_kt < whole) {
+                if (inside || from_h(MODE) || x_kt < whole) {
 #pragma unroll
                     for (int q = 0; q < PIECES; q++) {
                         const uint2 *p = reinterpret_cast<const uint2 *>(xp[nt] + q * A.hpad + f * 16);
@@ -461,21 +465,22 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
                 single_step<MB, PIECES>(acc, raw, A, b);
             }
         };
-        Part P0;
-        if constexpr (WIDE) {             // rare: nothing ahead, which leaves the registers to the usual sweep
+        if constexpr (WIDE || (PLAIN && MODE != kMatvec)) {   // rare: nothing ahead, which leaves the registers to the usual form
+            Part P;
             if (n > 0) rows_of();
 #pragma unroll 1
             for (int i = 0; i < n; i++) {
 #pragma unroll
                 for (int f = 0; f < 2; f++) {
-                    load_w(P0.raw[0], f);
-                    load_x(P0.x[0], f);
-                    compute(P0.raw[0], P0.x[0]);
+                    load_w(P.raw[0], f);
+                    load_x(P.x[0], f, false);
+                    compute(P.raw[0], P.x[0]);
                 }
                 next_w();
                 next_x();
             }
         } else {
+            Part P0, P1;
             if (n > 0) {
 #pragma unroll
                 for (int f = 0; f < HALVES; f++) load_w(P0.raw[f], f);
@@ -490,45 +495,71 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
             if (n > 0) {
                 rows_of();
 #pragma unroll
-                for (int f = 0; f < HALVES; f++) load_x(P0.x[f], f);
+                for (int f = 0; f < HALVES; f++) load_x(P0.x[f], f, false);
                 if (HALVES == 2) next_x();
             }
-            Part P1;
+            int i = 0;
             if constexpr (HALVES == 2) {
-                auto both = [&](Part &P) {
+                auto both = [&](Part &P, bool inside) {
                     load_w(P.raw[0], 0);
                     load_w(P.raw[1], 1);
                     next_w();
-                    load_x(P.x[0], 0);
-                    load_x(P.x[1], 1);
+                    load_x(P.x[0], 0, inside);
+                    load_x(P.x[1], 1, inside);
                     next_x();
                 };
-                for (int i = 0; i < n; i += 2) {
-                    if (i + 1 < n) both(P1);
-                    compute(P0.raw[0], P0.x[0]);
-                    compute(P0.raw[1], P0.x[1]);
-                    if (i + 1 >= n) break;
-                    if (i + 2 < n) both(P0);
-                    compute(P1.raw[0], P1.x[0]);
-                    compute(P1.raw[1], P1.x[1]);
+                auto compute2 = [&](const Part &P) {
+                    compute(P.raw[0], P.x[0]);
+                    compute(P.raw[1], P.x[1]);
+                };
+#pragma unroll 1
+                for (; i + 3 < n; i += 2) {
+                    both(P1, !PLAIN);
+                    compute2(P0);
+                    both(P0, !PLAIN);
+                    compute2(P1);
+                }
+                const int left = n - i;      // up to 3, the first one in P0
+                if (left > 0) {
+                    if (left > 1) both(P1, false);
+                    compute2(P0);
+                    if (left > 1) {
+                        if (left > 2) both(P0, false);
+                        compute2(P1);
+                        if (left > 2) compute2(P0);
+                    }
                 }
             } else {
-                for (int i = 0; i < n; i++) {
+                auto lower = [&](bool inside) {
                     load_w(P1.raw[0], 1);
-                    load_x(P1.x[0], 1);
+                    load_x(P1.x[0], 1, inside);
                     next_w();
                     next_x();
+                };
+                auto upper = [&](bool inside) {
+                    load_w(P0.raw[0], 0);
+                    load_x(P0.x[0], 0, inside);
+                };
+#pragma unroll 1
+                for (; i + 2 < n; i++) {
+                    lower(!PLAIN);
                     compute(P0.raw[0], P0.x[0]);
-                    if (i + 1 < n) {
-                        load_w(P0.raw[0], 0);
-                        load_x(P0.x[0], 0);
-                    }
+                    upper(!PLAIN);
+                    compute(P1.raw[0], P1.x[0]);
+                }
+#pragma unroll 1
+                for (; i < n; i++) {
+                    lower(false);
+                    compute(P0.raw[0], P0.x[0]);
+                    if (i + 1 < n) upper(false);
                     compute(P1.raw[0], P1.x[0]);
                 }
             }
         }
     };
-    sweep(std::false_type());
+    using Usual = std::integral_constant<int, kUsual>;
+    if (from_h(MODE) || vec) sweep(Usual());
+    else if constexpr (!from_h(MODE)) sweep(std::integral_constant<int, kPlain>());
     bool again = (seen & 0x80808080u) != 0;
     if constexpr (SINGLE) {
         float z = 0.0f;                   // a sum of zeros, unless something is not finite
@@ -538,7 +569,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
             for (int v = 0; v < 4; v++) z = fmaf(acc[j][0][v], 0.0f, z);
         again |= z != 0.0f;
     }
-    if (__any_sync(0xffffffffu, again)) sweep(std::true_type());
+    if (__any_sync(0xffffffffu, again)) sweep(std::integral_constant<int, kWide>());
 
     float *sums = reinterpret_cast<float *>(smem);
     if constexpr (SINGLE) {
