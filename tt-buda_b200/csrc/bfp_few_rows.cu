@@ -488,9 +488,9 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
             }
             // The weights were asked for before what the launch in front of this one computes is waited for: it writes activations,
             // never weights, and what was in front of that one was complete before it let this launch begin.
-            if (W.begin) {
-                if (MODE != kExpertsIn) griddep_wait();
-                if (MODE == kMatvec) griddep_launch();
+            if (W.begin && MODE != kExpertsIn) {
+                griddep_wait();
+                griddep_launch();
             }
             if (n > 0) {
                 rows_of();
@@ -825,6 +825,7 @@ __global__ void __launch_bounds__(256) sum_slots_kernel(const float *partial, in
                                                         __nv_bfloat16 *y, int64_t ldy)
 {
     griddep_wait();
+    griddep_launch();
     const int t = blockIdx.y, lane = threadIdx.x & 31, col = blockIdx.x * 1024 + threadIdx.x * 4;
     const int e = lane < top ? __ldcg(ids + t * top + lane) : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, e);

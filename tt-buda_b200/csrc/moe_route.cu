@@ -6,7 +6,8 @@
 // Bound: for a few tokens the latency of one pass over w (E * H values that every cluster reads once, from L2 after the
 // first).  A cluster of 8 CTAs takes a block of tokens; its CTAs share the experts, the warps of a CTA share an expert's
 // row when there are fewer experts than warps, so that all of w is asked for at once.  The scores meet in distributed
-// shared memory; the warp of token i chooses in CTA i % 8.
+// shared memory; the warp of token i chooses in CTA i % 8.  Most of a call is waiting for w, so a warp asks for a row's piece in one
+// go (8 octets a lane), before it even waits for the activations, which are kept in shared memory for all its rows.
 // Scores decide which experts run: a lane adds its products 8 at a time, the 32 lanes and the pieces of a row are joined in
 // binary64, and the result is rounded to binary32 once.
 #include <cuda_bf16.h>
@@ -17,7 +18,7 @@ namespace buda {
 namespace route {
 
 constexpr int kCluster = 8;
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kPerCta = kMaxExperts / kCluster;
 
@@ -95,6 +96,8 @@ __device__ __forceinline__ uint32_t order_of(float l)
     return b >> 31 ? ~b : b | 0x80000000u;
 }
 
+constexpr int kStaged = 28 * 1024;       // activations of a block of tokens up to this size are kept in shared memory
+
 template <typename TW, int TB>
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2)
     route_kernel(const __nv_bfloat16 *x, int64_t ldx, int T, int H, const TW *w, int64_t ldw, int E, int top, int renorm, int split,
@@ -102,8 +105,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2)
 {
     __shared__ double part[kPerCta * TB * kWarps];      // [expert of this CTA][token][piece of the row]
     __shared__ float score[kPerCta * TB];
-    asm volatile("griddepcontrol.wait;" ::: "memory");                // x may come from the launch in front of this one
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    extern __shared__ __align__(16) __nv_bfloat16 xs[]; // [TB][8 * octets], zero past H
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t rank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -112,44 +114,69 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2)
     const bool xvec = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * 2)) & 15) == 0;
     const bool wvec = ((reinterpret_cast<uintptr_t>(w) | (uintptr_t)(ldw * sizeof(TW))) & 15) == 0;
     const int octets = (H + 7) / 8;
-    for (int task = warp; task < mine * split; task += kWarps) {
-        const int el = task / split, piece = task % split;
+    const bool staged = TB * octets * 16 <= kStaged;
+
+    // A warp's work: batches of kBatch octets (of every lane) of its tasks, a task being a piece of an expert's row.
+    constexpr int kBatch = (TB == 1 ? 8 : 4) * 2 / (int)sizeof(TW);
+    const int batches = (octets + split * 32 * kBatch - 1) / (split * 32 * kBatch);   // of a piece; the last ones may be empty
+    const int tasks = mine * split > warp ? (mine * split - warp + kWarps - 1) / kWarps : 0;
+    Octet<TW> a[kBatch];
+    int el, piece, o0, o1;
+    auto load = [&](int it) {
+        const int task = warp + it / batches * kWarps;
+        el = task / split;
+        piece = task % split;
+        o0 = (int)((int64_t)octets * piece / split) + it % batches * 32 * kBatch + lane;
+        o1 = (int)((int64_t)octets * (piece + 1) / split);
         const TW *row = w + (int64_t)(rank + el * kCluster) * ldw;
-        const int o1 = (int)((int64_t)octets * (piece + 1) / split);
-        float s[TB];
 #pragma unroll
-        for (int i = 0; i < TB; i++) s[i] = 0.0f;
-        constexpr int kBatch = TB > 1 ? 4 : 8;       // octets of a row on their way at once
-        for (int o = (int)((int64_t)octets * piece / split) + lane; o < o1; o += 32 * kBatch) {
-            Octet<TW> a[kBatch];
-            Octet<__nv_bfloat16> b[kBatch][TB];
+        for (int u = 0; u < kBatch; u++) a[u].load(row, o0 + 32 * u < o1 ? (o0 + 32 * u) * 8 : H, H, wvec);
+    };
+    if (tasks) load(0);          // the router's weights are not what the launch in front of this one writes
+    asm volatile("griddepcontrol.wait;" ::: "memory");                // x may be
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (staged) {
+        for (int i = tid; i < nt * octets; i += kThreads) {
+            Octet<__nv_bfloat16> b;
+            const int t = i / octets, o = i - t * octets;
+            b.load(x + (int64_t)(t0 + t) * ldx, o * 8, H, xvec);
+            *reinterpret_cast<uint4 *>(xs + (int64_t)i * 8) = b.r;
+        }
+        __syncthreads();
+    }
+    float s[TB];
+    for (int it = 0; it < tasks * batches; it++) {
+        if (it) load(it);
+        if (it % batches == 0)
 #pragma unroll
-            for (int u = 0; u < kBatch; u++) {
-                const int h = o + 32 * u < o1 ? (o + 32 * u) * 8 : H;
-                a[u].load(row, h, H, wvec);
+            for (int i = 0; i < TB; i++) s[i] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < TB; i++) b[u][i].load(x + (int64_t)(t0 + min(i, nt - 1)) * ldx, h, H, xvec);
-            }
+        for (int u = 0; u < kBatch; u++) {
+            if (o0 + 32 * u >= o1) break;
+            float av[8];
+            a[u].get(av);
 #pragma unroll
-            for (int u = 0; u < kBatch; u++) {
-                float av[8];
-                a[u].get(av);
+            for (int i = 0; i < TB; i++) {
+                const int t = min(i, nt - 1);
+                Octet<__nv_bfloat16> b;
+                if (staged) b.r = *reinterpret_cast<const uint4 *>(xs + (t * octets + o0 + 32 * u) * 8);
+                else b.load(x + (int64_t)(t0 + t) * ldx, (o0 + 32 * u) * 8, H, xvec);
+                float bv[8], p = 0.0f;
+                b.get(bv);
 #pragma unroll
-                for (int i = 0; i < TB; i++) {
-                    float bv[8], p = 0.0f;
-                    b[u][i].get(bv);
-#pragma unroll
-                    for (int v = 0; v < 8; v++) p = fmaf(av[v], bv[v], p);
-                    s[i] += p;
-                }
+                for (int v = 0; v < 8; v++) p = fmaf(av[v], bv[v], p);
+                s[i] += p;
             }
         }
+        if (it % batches == batches - 1) {
+            __syncwarp();
 #pragma unroll
-        for (int i = 0; i < TB; i++) {
-            double all = s[i];
+            for (int i = 0; i < TB; i++) {
+                double all = s[i];
 #pragma unroll
-            for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-            if (lane == 0) part[(el * TB + i) * split + piece] = all;
+                for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+                if (lane == 0) part[(el * TB + i) * split + piece] = all;
+            }
         }
     }
     __syncthreads();
@@ -235,6 +262,8 @@ cudaError_t launch_tw(const void *x, int64_t ldx, int T, int H, const void *w, i
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((T + tb - 1) / tb * kCluster));
     cfg.blockDim = dim3(kThreads);
+    const int64_t x_bytes = (int64_t)tb * ((H + 7) / 8) * 16;
+    cfg.dynamicSmemBytes = x_bytes <= kStaged ? x_bytes : 0;
     cfg.stream = stream;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;     // begins while the launch in front of it ends, if that one lets it
