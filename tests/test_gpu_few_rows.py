@@ -433,3 +433,135 @@ def test_image_past_4_gib(ops):
     last = ops.moe_experts(x, weights, torch.tensor([[255], [255]], dtype=torch.int32, device="cuda"), images, images, images, i, ops.DF.Bfp8_b)
     low = ops.moe_experts(x, weights, torch.tensor([[3], [3]], dtype=torch.int32, device="cuda"), images, images, images, i, ops.DF.Bfp8_b)
     assert torch.equal(last, low) and last.float().abs().max() > 0.01
+
+
+# ------------------------------------------------------------------------------------------------ what a caller may do, and may not
+def test_empty_batches(ops, oracle):
+    images, _ = _make_experts(oracle, 3, 64, 32, "Bfp4_b", 40)
+    x = torch.zeros(0, 64, dtype=torch.bfloat16, device="cuda")
+    wr = torch.ones(3, 64, device="cuda")
+    weights, ids = ops.moe_route(x, wr, 2)
+    assert weights.shape == ids.shape == (0, 2)
+    assert ops.moe_experts(x, weights, ids, *images, 32).shape == (0, 64)
+    assert ops.moe_layer(x, wr, 2, *images, 32).shape == (0, 64)
+
+
+def test_refusals(ops, oracle):
+    images, _ = _make_experts(oracle, 3, 64, 32, "Bfp4_b", 41)
+    x, wr = torch.zeros(2, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(3, 64, device="cuda")
+    weights, ids = torch.ones(2, 2, device="cuda"), torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    big = torch.zeros(4 * 576 + 32, dtype=torch.uint8, device="cuda")
+    bad = [
+        lambda: ops.bfp_matvec(x, big[16:], 64),                                          # image not 32-byte aligned
+        lambda: ops.bfp_matvec(x, big[:3 * 576], 64),                                     # too small
+        lambda: ops.bfp_matvec(x, big, 0),
+        lambda: ops.bfp_matvec(x, big.view(torch.int8), 64),
+        lambda: ops.bfp_matvec(x.expand(65, 2, 64)[:, 0], big, 64),                       # 65 rows
+        lambda: ops.bfp_matvec(x, big, 64, out_dtype=torch.float16),
+        lambda: ops.bfp_matvec(x, big, 64, out=torch.empty(2, 65, dtype=torch.bfloat16, device="cuda")),
+        lambda: ops.bfp_matvec(x, big, 64, out=torch.empty(64, 2, dtype=torch.bfloat16, device="cuda").t()),
+        lambda: ops.bfp_matvec(x, big, 64, out=torch.empty(1, 64, dtype=torch.bfloat16, device="cuda").expand(2, 64)),   # rows on one another
+        lambda: ops.moe_route(x, wr, 4),                                                  # more than there are
+        lambda: ops.moe_route(x, wr, 0),
+        lambda: ops.moe_route(x, wr[:, :63], 1),
+        lambda: ops.moe_route(x, wr.half(), 1),
+        lambda: ops.moe_route(x, wr.expand(90, 3, 64).reshape(270, 64), 1),               # 270 experts
+        lambda: ops.moe_experts(x, weights, ids.long(), *images, 32),
+        lambda: ops.moe_experts(x, weights[:, :1], ids, *images, 32),
+        lambda: ops.moe_experts(x, weights.t(), ids, *images, 32),
+        lambda: ops.moe_experts(x, weights, ids, images[0], images[1][:2], images[2], 32),
+        lambda: ops.moe_experts(x, weights, ids, *images, 33),
+        lambda: ops.moe_experts(x, weights, ids, *images, 32, activation="tanh"),
+        lambda: ops.moe_layer(x, wr[:2], 2, *images, 32),
+        lambda: ops.moe_layer(x.cpu(), wr, 2, *images, 32),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    prev = ops.get_bfp_policy()
+    try:
+        ops.set_bfp_policy(ops._cabi.BfpPolicy(face_order=(0, 2, 1, 3)))
+        with pytest.raises(ops._cabi.BudaError, match="byte layout"):
+            ops.bfp_matvec(x, big, 64)
+    finally:
+        ops.set_bfp_policy(prev)
+    ops.bfp_matvec(x, big, 64)
+
+
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("t,h,i,e", [(40, 1024, 40, 2), (64, 1056, 200, 3)])
+def test_experts_of_many_tokens_over_clusters(ops, oracle, df, t, h, i, e):
+    """Several passes over one expert's tokens, each joined over a cluster of CTAs."""
+    images, vals = _make_experts(oracle, e, h, i, df, 42)
+    x = _bf16(_rand((t, h), 43))
+    weights, ids = _routing(t, e, 2, 44)
+    got = ops.moe_experts(x.cuda(), weights.cuda(), ids.cuda(), *images, i, getattr(ops.DF, df))
+    _check_experts(got, x, weights, ids, vals, "silu")
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_weights_that_another_stream_has_just_packed(ops, oracle, captured):
+    """A launch may ask for its weights while the launch in front of it still runs; not before an event that the stream waits for."""
+    k = n = 512
+    a = _bf16(_rand((1, k), 45)).cuda()
+    other, _ = _store(oracle, _rand((k, n), 46, 0.1), "Bfp4_b")
+    w = [torch.from_numpy(_rand((1, 1, k, n), 47 + r, 0.1)).cuda() for r in range(4)]
+    want = [ops.bfp_matvec(a, ops.tilize_pack(x, ops.DF.Bfp4_b), n) for x in w]
+    src, img = w[0].clone(), torch.zeros_like(other)
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def step():
+        side.wait_stream(torch.cuda.current_stream())
+        ops.bfp_matvec(a, other, n)
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200000)
+            ops.tilize_pack(src, ops.DF.Bfp4_b, out=img)
+        torch.cuda.current_stream().wait_stream(side)
+        return ops.bfp_matvec(a, img, n)
+
+    torch.cuda.synchronize()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=main):
+            got = step()
+    for r in range(4):
+        img.zero_()
+        src.copy_(w[r])
+        torch.cuda.synchronize()
+        if captured:
+            graph.replay()
+        else:
+            with torch.cuda.stream(main):
+                got = step()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want[r]), r
+
+
+_FIRST_CALL_CAPTURED = """
+import sys
+sys.path[:0] = {path!r}
+import torch
+from pybuda import cuda_ops as ops
+x = torch.ones(3, 64, device="cuda").bfloat16()
+img = torch.zeros(2, 4 * 576, dtype=torch.uint8, device="cuda")
+img[:, :64] = 120
+img[:, 64:] = 0x21
+wr = torch.ones(2, 64, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = ops.moe_layer(ops.bfp_matvec(x, img[0], 64), wr, 1, img, img, img, 64)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, ops.moe_layer(ops.bfp_matvec(x, img[0], 64), wr, 1, img, img, img, 64)) and y.float().abs().max() > 0
+print("captured ok")
+"""
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    import subprocess
+    import sys
+
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALL_CAPTURED.format(path=[p for p in sys.path if p])], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured ok" in r.stdout, r.stderr[-2000:]
