@@ -311,6 +311,26 @@ def test_experts_dropped_repeated_and_foreign_slots(ops, oracle):
     assert torch.all(none == 0)
 
 
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("t", [1, 3, 12])
+def test_experts_infinite_weights_reach_their_own_tokens_only(ops, oracle, df, t):
+    """Images packed from matrices with infinities: their experts' tokens get numbers that are not finite, all others what they get
+    without that expert.  (Few tokens run through all experts as one sum, with zeros in the other experts' rows.)"""
+    e, h, i = 3, 96, 64
+    images, vals = _make_experts(oracle, e, h, i, df, 24)
+    broken = _rand((i, h), 25, 0.1)
+    broken[3, :] = np.inf
+    images[2][1] = _store(oracle, broken, df)[0]
+    x = _bf16(_rand((t, h), 26))
+    ids = torch.tensor([[k % 3, (k + 2) % 3] for k in range(t)], dtype=torch.int32)     # every third pair has no expert 1
+    weights = torch.rand(t, 2, generator=torch.Generator().manual_seed(27)) + 0.1
+    got = ops.moe_experts(x.cuda(), weights.cuda(), ids.cuda(), *images, i, getattr(ops.DF, df))
+    clean = [k for k in range(t) if 1 not in ids[k]]
+    dirty = [k for k in range(t) if 1 in ids[k]]
+    assert not dirty or not torch.isfinite(got[dirty]).any()
+    _check_experts(got[clean], x[clean], weights[clean], ids[clean], vals, "silu")
+
+
 def test_experts_many_experts_one_token_each(ops, oracle):
     e, h, i, t = 256, 32, 32, 64
     images, vals = _make_experts(oracle, e, h, i, "Bfp2_b", 13)
