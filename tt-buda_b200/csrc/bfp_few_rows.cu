@@ -54,9 +54,9 @@ enum { kMatvec = 0, kExpertsIn = 1, kExpertsOut = 2, kExpertsEach = 3 };
 enum { kUsual = 0, kPlain = 1, kWide = 2 };   // forms of a sweep (see products)
 __host__ __device__ constexpr bool from_h(int mode) { return mode == kExpertsOut || mode == kExpertsEach; }
 
-// How many units of 8 warps an SM holds, by registers: 128 a thread suffice for up to 8 tokens and, in the matvec of data below 8
-// bits, for up to 16
-__host__ __device__ constexpr int units_per_sm(int mb, int nt, int mode) { return nt <= 1 || (nt == 2 && mb != 7 && mode == kMatvec) ? 2 : 1; }
+// How many units of 8 warps an SM holds, by registers: 128 a thread suffice for up to 8 tokens and, in the matvec, for up to 16
+// (8-bit data spill a little: 12x4096x16384 19.2 us against 20.7 with half the warps)
+__host__ __device__ constexpr int units_per_sm(int nt, int mode) { return nt <= 1 || (nt == 2 && mode == kMatvec) ? 2 : 1; }
 
 template <int MB>
 struct Fmt {
@@ -612,7 +612,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
 
 // NT: groups of 8 tokens in one pass; 0: one token.
 template <int MB, int NT, int MODE>
-__global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(MB, NT, MODE), 1) few_rows_kernel(const __grid_constant__ Args A)
+__global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(NT, MODE), 1) few_rows_kernel(const __grid_constant__ Args A)
 {
     using F = Fmt<MB>;
     using L = Lay<MB, NT>;
@@ -867,7 +867,7 @@ __global__ void __launch_bounds__(256) sum_slots_kernel(const float *partial, in
 template <int MB, int NT, int MODE>
 cudaError_t launch_one(const Args &a, dim3 grid, int warps, cudaStream_t stream)
 {
-    constexpr int most = Lay<MB, NT>::bytes(MODE, kUnitWarps * units_per_sm(MB, NT, MODE));
+    constexpr int most = Lay<MB, NT>::bytes(MODE, kUnitWarps * units_per_sm(NT, MODE));
     static_assert(most <= 227 * 1024, "shared memory of the largest CTA");
     static std::atomic<uint64_t> ready{0};      // devices whose kernel may take this much shared memory
     int dev = 0;
@@ -900,7 +900,7 @@ int groups_of_8(int rows) { return rows == 1 ? 0 : rows <= 8 ? 1 : rows <= 16 ? 
 struct Split {
     int units, cluster;       // units of 8 warps in a CTA; CTAs
 };
-// CTAs of a cluster first, one to an SM, while each warp of 8 keeps a tile row, and two to an SM while it keeps two; then more
+// CTAs of a cluster first, one to an SM, while each warp of 8 keeps a tile row, and as many as fit while it keeps two; then more
 // warps in a CTA, while each keeps 4.
 // Measured, us, as CTAs x warps (B200): 1x1024x1024 Bfp4_b, 8 column groups: 4x8 2.46, 8x8 2.91, 1x16 3.19.  8x4096x1024 Bfp8_b, 8
 // groups: 8x8 4.81, 8x16 4.99, 1x16 10.3.  12x4096x4096 Bfp4_b, 32 groups: 8x8 6.70, 4x8 7.91, 4x16 7.06.  1x4096x16384 Bfp4_b,
@@ -908,7 +908,7 @@ struct Split {
 Split split_of(int64_t groups, int64_t tile_rows, int sm_count, int per_sm)
 {
     int64_t c = std::min<int64_t>(sm_count / groups, (tile_rows + kUnitWarps - 1) / kUnitWarps);
-    if (2 * groups <= sm_count) c = std::max(c, std::min<int64_t>(2 * sm_count / groups, tile_rows / (2 * kUnitWarps)));
+    if (2 * groups <= sm_count) c = std::max(c, std::min<int64_t>((int64_t)per_sm * sm_count / groups, tile_rows / (2 * kUnitWarps)));
     c = std::max<int64_t>(1, std::min<int64_t>(c, 8));
     int64_t u = tile_rows / (c * kUnitWarps * 4);
     u = std::min<int64_t>(u, (int64_t)sm_count * per_sm / (groups * c));
@@ -933,7 +933,7 @@ cudaError_t launch_nt(int nt, const Args &a, dim3 grid, int warps, cudaStream_t 
 template <int MODE>
 cudaError_t dispatch(int mant_bits, int nt, Args &a, int groups, double copies, int64_t tile_rows, int y, int sm_count, cudaStream_t stream)
 {
-    const Split s = split_of((int64_t)(groups * copies + 0.5), tile_rows, sm_count, units_per_sm(mant_bits, nt, MODE));
+    const Split s = split_of((int64_t)(groups * copies + 0.5), tile_rows, sm_count, units_per_sm(nt, MODE));
     const dim3 grid((unsigned)(groups * s.cluster), y);
     const int warps = s.units * kUnitWarps;
     a.cluster = s.cluster;
