@@ -307,8 +307,10 @@ def test_experts_dropped_repeated_and_foreign_slots(ops, oracle):
     got = ops.moe_experts(x.cuda(), weights.cuda(), ids.cuda(), *images, i)
     _check_experts(got, x, weights, ids, vals, "silu")
     assert torch.all(got[2] == 0)
-    none = ops.moe_experts(x.cuda(), weights.cuda(), torch.full_like(ids, -1).cuda(), *images, i)
-    assert torch.all(none == 0)
+    for rows in (1, 6, 12):
+        none = ops.moe_experts(x.repeat(2, 1)[:rows].cuda(), weights.repeat(2, 1)[:rows].cuda(), torch.full((rows, 4), -1, dtype=torch.int32, device="cuda"),
+                               *images, i)
+        assert torch.all(none == 0) and none.shape == (rows, h)
 
 
 @pytest.mark.parametrize("df", FORMATS)

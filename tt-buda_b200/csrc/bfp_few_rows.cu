@@ -363,7 +363,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
 
     // What a lane loads ahead: its rows of one face or of the upper and the lower one, and token g's activations beside them.
     // Lanes past the last token read the first one's row: their columns of the product are dropped.
-    constexpr int HALVES = MB == 7 || NT > 1 ? 1 : 2;      // by registers
+    constexpr int HALVES = MB == 7 || NT == 2 || (NT == 4 && MODE != kMatvec) ? 1 : 2;      // by registers
     struct Part {
         Raw<MB> raw[HALVES];
         uint2 x[HALVES][PIECES][NT];
@@ -710,7 +710,11 @@ __global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(NT, MODE), 1) f
                 __syncthreads();
                 W.units = count * A.Kt;
             } else {
-                if ((int)blockIdx.y >= count) return;                              // the whole cluster: it shares blockIdx.y
+                if ((int)blockIdx.y >= count) {                                    // the whole cluster: it shares blockIdx.y
+                    // where no slot counts at all, some block still has to stand behind the launch in front
+                    if (MODE == kExpertsEach && blockIdx.y == 0) griddep_wait();
+                    return;
+                }
                 int e = 0, left = blockIdx.y;
                 for (int w = 0; w < kMaxExperts / 32; w++) {
                     const int here = __popc(map[w]);

@@ -2,7 +2,8 @@
 sm_100a CUDA kernels (libbuda_cuda.so) behind the reference's backend_api entry points.
 
 Only the data-format path is here: tilize / untilize, Bfp8_b / Bfp4_b / Bfp2_b pack and unpack,
-the golden int8 quantise ops and the Bfp8_b-weight matmul.  There is no CPU fallback.
+the golden int8 quantise ops, the Bfp8_b-weight matmul, and the few-row products and mixture-of-experts
+layers of a decoding step on block-float weights.  There is no CPU fallback.
 """
 TILE_DIM = 32
 
