@@ -376,7 +376,7 @@ int buda_i8_gemm(const void *A, int64_t M, int64_t K, int64_t lda, const void *W
 
 /* ------------------------------------------------------------------ a few rows against block-float weights
  * Products of 1..64 rows (the tokens of a decoding step) with weights stored as block-float queue images, each weight read
- * once.  Images are those of buda_bfp8b_gemm, for Bfp8_b, Bfp4_b and Bfp2_b alike: geometry grid 1x1, ublock 1x1, order R,
+ * once for every 32 rows.  Images are those of buda_bfp8b_gemm, for Bfp8_b, Bfp4_b and Bfp2_b alike: geometry grid 1x1, ublock 1x1, order R,
  * no tile header, default byte layout, 32-byte aligned; sizes that fill no tile are padded to whole tiles (with zeros, as
  * the pack writes them).  Every stored weight counts at its exact value, sums are binary32.  Results do not depend on
  * what else runs: the same call gives the same bits.  K, N, H, I <= 2^24. */

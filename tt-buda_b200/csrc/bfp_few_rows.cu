@@ -54,9 +54,10 @@ enum { kMatvec = 0, kExpertsIn = 1, kExpertsOut = 2, kExpertsEach = 3 };
 enum { kUsual = 0, kPlain = 1, kWide = 2 };   // forms of a sweep (see products)
 __host__ __device__ constexpr bool from_h(int mode) { return mode == kExpertsOut || mode == kExpertsEach; }
 
-// How many units of 8 warps an SM holds, by registers: 128 a thread suffice for up to 8 tokens and, in the matvec, for up to 16
-// (8-bit data spill a little: 12x4096x16384 19.2 us against 20.7 with half the warps)
-__host__ __device__ constexpr int units_per_sm(int nt, int mode) { return nt <= 1 || (nt == 2 && mode == kMatvec) ? 2 : 1; }
+// How many units of 8 warps an SM holds, by registers: 128 a thread for up to 16 tokens in a pass.  9 to 16 tokens spill a little and
+// are the faster for twice the warps all the same (12x4096x16384 Bfp8_b 19.2 us against 20.7; 64 tokens, 4 of 32 experts of
+// 1024 x 2048 Bfp4_b 68-74 against 86-90).
+__host__ __device__ constexpr int units_per_sm(int nt) { return nt <= 2 ? 2 : 1; }
 
 template <int MB>
 struct Fmt {
@@ -66,7 +67,7 @@ struct Fmt {
 };
 
 struct Args {
-    const __nv_bfloat16 *x;      // [rows, K], row stride ldx; experts-out: h
+    const __nv_bfloat16 *x;      // [rows, K], row stride ldx (matvec, experts-in; the others read h)
     int64_t ldx;
     int rows, K, Kt, N, Nt;
     const uint8_t *w0, *w1;      // w1: the up matrix of gated experts
@@ -612,7 +613,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
 
 // NT: groups of 8 tokens in one pass; 0: one token.
 template <int MB, int NT, int MODE>
-__global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(NT, MODE), 1) few_rows_kernel(const __grid_constant__ Args A)
+__global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(NT), 1) few_rows_kernel(const __grid_constant__ Args A)
 {
     using F = Fmt<MB>;
     using L = Lay<MB, NT>;
@@ -871,7 +872,7 @@ __global__ void __launch_bounds__(256) sum_slots_kernel(const float *partial, in
 template <int MB, int NT, int MODE>
 cudaError_t launch_one(const Args &a, dim3 grid, int warps, cudaStream_t stream)
 {
-    constexpr int most = Lay<MB, NT>::bytes(MODE, kUnitWarps * units_per_sm(NT, MODE));
+    constexpr int most = Lay<MB, NT>::bytes(MODE, kUnitWarps * units_per_sm(NT));
     static_assert(most <= 227 * 1024, "shared memory of the largest CTA");
     static std::atomic<uint64_t> ready{0};      // devices whose kernel may take this much shared memory
     int dev = 0;
@@ -937,7 +938,7 @@ cudaError_t launch_nt(int nt, const Args &a, dim3 grid, int warps, cudaStream_t 
 template <int MODE>
 cudaError_t dispatch(int mant_bits, int nt, Args &a, int groups, double copies, int64_t tile_rows, int y, int sm_count, cudaStream_t stream)
 {
-    const Split s = split_of((int64_t)(groups * copies + 0.5), tile_rows, sm_count, units_per_sm(nt, MODE));
+    const Split s = split_of((int64_t)(groups * copies + 0.5), tile_rows, sm_count, units_per_sm(nt));
     const dim3 grid((unsigned)(groups * s.cluster), y);
     const int warps = s.units * kUnitWarps;
     a.cluster = s.cluster;
@@ -971,7 +972,9 @@ cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stre
 {
     const int Ht = (m.H + 31) / 32, It = (m.I + 31) / 32;
     const int slots = m.T * m.top, most = m.E < slots ? m.E : slots;
-    // the experts that independent choices reach on average, and the tokens of one: up to 4 fit a group of 8 nearly always
+    // The experts that independent choices reach on average, and the tokens of one.  Up to 4 fit a group of 8 nearly always, and
+    // where they do not a second pass costs less than wider passes for all (32 tokens, 2 of 16 experts of 2048 x 1024 Bfp4_b: 24 us,
+    // 27 with a second pass, against 31.5 in passes of 16).
     const double miss = m.top < m.E ? 1.0 - (double)m.top / m.E : 0.0, reached = m.E * (1.0 - pow(miss, m.T));
     const double share = (double)slots / m.E;
     const int nt = m.T == 1 ? 0 : m.T <= kOneSum || share <= 4.0 ? 1 : share <= 10.0 ? 2 : 4;
