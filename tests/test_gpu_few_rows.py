@@ -587,3 +587,62 @@ def test_first_call_of_a_process_inside_a_capture():
 
     r = subprocess.run([sys.executable, "-c", _FIRST_CALL_CAPTURED.format(path=[p for p in sys.path if p])], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "captured ok" in r.stdout, r.stderr[-2000:]
+
+
+# ------------------------------------------------------------------------------------------------ what the launch in front writes
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("e,k", [(8, 4096), (64, 2048)])
+def test_router_weights_that_a_few_row_product_has_just_written(ops, oracle, e, k, captured):
+    """Launches overlap: the router may begin while the product that writes its weights still runs, and must not read them yet."""
+    h, t = 512, 3
+    img, _ = _store(oracle, _rand((k, h), 50, k ** -0.5), "Bfp8_b")
+    images, _ = _make_experts(oracle, e, h, 32, "Bfp4_b", 51)
+    rows = [_bf16(_rand((e, k), 52 + r)).cuda() for r in range(3)]
+    x = _bf16(_rand((t, h), 56)).cuda()
+    want = []
+    for r in rows:
+        w = ops.bfp_matvec(r, img, h, ops.DF.Bfp8_b, out_dtype=torch.float32)
+        torch.cuda.synchronize()
+        want.append((*ops.moe_route(x, w, 2), ops.moe_layer(x, w, 2, *images, 32)))
+        torch.cuda.synchronize()
+    assert not torch.equal(want[0][1], want[1][1])
+    buf, src = torch.zeros(e, h, device="cuda"), rows[0].clone()
+
+    def step():
+        ops.bfp_matvec(src, img, h, ops.DF.Bfp8_b, out=buf)
+        chosen = ops.moe_route(x, buf, 2)
+        ops.bfp_matvec(src, img, h, ops.DF.Bfp8_b, out=buf)
+        return (*chosen, ops.moe_layer(x, buf, 2, *images, 32))
+
+    torch.cuda.synchronize()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+    for r in range(60):
+        src.copy_(rows[r % 3])
+        if captured:
+            graph.replay()
+        else:
+            got = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[r % 3])), r
+
+
+def test_router_weights_that_the_experts_have_just_written(ops, oracle):
+    """The same behind the launch that adds up the slots of more than 8 tokens."""
+    e, h, i, t = 4, 256, 64, 12
+    images, _ = _make_experts(oracle, e, h, i, "Bfp4_b", 57)
+    xs = [_bf16(_rand((t, h), 58 + r)).cuda() for r in range(3)]
+    weights, ids = (v.cuda() for v in _routing(t, e, 2, 61))
+    q = _bf16(_rand((5, h), 62)).cuda()
+    want = []
+    for x in xs:
+        w = ops.moe_experts(x, weights, ids, *images, i)
+        torch.cuda.synchronize()
+        want.append(ops.moe_route(q, w, 3))
+        torch.cuda.synchronize()
+    buf = torch.zeros(t, h, dtype=torch.bfloat16, device="cuda")
+    for r in range(60):
+        ops.moe_experts(xs[r % 3], weights, ids, *images, i, out=buf)
+        got = ops.moe_route(q, buf, 3)
+        assert all(torch.equal(a, b) for a, b in zip(got, want[r % 3])), r

@@ -7,10 +7,11 @@
 // first).  A cluster of 8 CTAs takes a block of tokens; its CTAs share the experts, the warps of a CTA share an expert's
 // row when there are fewer experts than warps, so that all of w is asked for at once.  The scores meet in distributed
 // shared memory; the warp of token i chooses in CTA i % 8.  Most of a call is waiting for w, so a warp asks for a row's piece in one
-// go (8 octets a lane), before it even waits for the activations, which are kept in shared memory for all its rows.
+// go (8 octets a lane).  w may be what the launch in front has written, as x may: before that one is complete its addresses are
+// only named to L2, which brings no value into the kernel.
 // Scores decide which experts run: a lane adds its products 8 at a time, the 32 lanes and the pieces of a row are joined in
 // binary64, and the result is rounded to binary32 once.
-// Measured (B200): one token, 8 experts of 1024 binary32 weights 2.8 us; 16 tokens, 128 experts of 4096 bfloat16 weights 9.6 us
+// Measured (B200): one token, 8 experts of 1024 binary32 weights 3.6 us; 16 tokens, 128 experts of 4096 bfloat16 weights 10.8 us
 // (16 clusters read and widen the same 1 MB; the choice of 8 takes 0.8 of it).
 #include <cuda_bf16.h>
 
@@ -124,19 +125,29 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2)
     const int tasks = mine * split > warp ? (mine * split - warp + kWarps - 1) / kWarps : 0;
     Octet<TW> a[kBatch];
     int el, piece, o0, o1;
-    auto load = [&](int it) {
+    const TW *row;
+    auto place = [&](int it) {
         const int task = warp + it / batches * kWarps;
         el = task / split;
         piece = task % split;
         o0 = (int)((int64_t)octets * piece / split) + it % batches * 32 * kBatch + lane;
         o1 = (int)((int64_t)octets * (piece + 1) / split);
-        const TW *row = w + (int64_t)(rank + el * kCluster) * ldw;
+        row = w + (int64_t)(rank + el * kCluster) * ldw;
+    };
+    auto load = [&](int it) {
+        place(it);
 #pragma unroll
         for (int u = 0; u < kBatch; u++) a[u].load(row, o0 + 32 * u < o1 ? (o0 + 32 * u) * 8 : H, H, wvec);
     };
-    if (tasks) load(0);          // the router's weights are not what the launch in front of this one writes
-    asm volatile("griddepcontrol.wait;" ::: "memory");                // x may be
+    if (tasks) {
+        place(0);
+#pragma unroll
+        for (int u = 0; u < kBatch; u++)
+            if (o0 + 32 * u < o1) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + (o0 + 32 * u) * 8));
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");                // the launch in front may write x and w
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (tasks) load(0);
     if (staged) {
         for (int i = tid; i < nt * octets; i += kThreads) {
             Octet<__nv_bfloat16> b;
