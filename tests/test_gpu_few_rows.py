@@ -646,3 +646,48 @@ def test_router_weights_that_the_experts_have_just_written(ops, oracle):
         ops.moe_experts(xs[r % 3], weights, ids, *images, i, out=buf)
         got = ops.moe_route(q, buf, 3)
         assert all(torch.equal(a, b) for a, b in zip(got, want[r % 3])), r
+
+
+@pytest.mark.parametrize("m", [1, 5, 40])
+def test_images_that_the_launch_in_front_has_just_written(ops, oracle, m):
+    """An image whose bytes are the result of a product: bfloat16 numbers of [2, 4) are exponents and data of finite weights.  One-hot
+    rows pick which, over blocks with exponents of 128, so that the product in front takes its time."""
+    k, n, rows, side = 2048, 2304, 8, 256
+    assert 2 * rows * n == (side // 32) ** 2 * 576
+    img, _ = _store(oracle, 2 + 1.9 * np.random.default_rng(63).random((k, n), np.float32), "Bfp8_b")
+    picks = [torch.zeros(rows, k).index_put_((torch.arange(rows), torch.arange(rows) + 100 * r), torch.ones(())).bfloat16().cuda() for r in range(3)]
+    x = _bf16(_rand((m, side), 64)).cuda()
+    weights, ids = torch.ones(m, 1, device="cuda"), torch.zeros(m, 1, dtype=torch.int32, device="cuda")
+    buf = torch.zeros(rows, n, dtype=torch.bfloat16, device="cuda")
+    image = buf.view(torch.uint8).view(1, -1)
+
+    def use(which):
+        if which == 0:
+            return ops.bfp_matvec(x, image.view(-1), side, out_dtype=torch.float32)
+        images = [image.clone() if i != which else image for i in range(1, 4)]      # the copies are made of an older image
+        return images, lambda: ops.moe_experts(x, weights, ids, *images, side)
+
+    def fill(r):
+        ops.bfp_matvec(picks[r], img, n, ops.DF.Bfp8_b, out=buf)
+
+    want = []
+    for r in range(3):
+        fill(r)
+        torch.cuda.synchronize()
+        want.append(use(0))
+        torch.cuda.synchronize()
+    assert torch.isfinite(want[0]).all() and not torch.equal(want[0], want[1])
+    for r in range(30):
+        fill(r % 3)
+        assert torch.equal(use(0), want[r % 3]), r
+    fill(0)
+    for which in (1, 2, 3):
+        images, call = use(which)
+        for r in range(3):
+            fill(r)
+            torch.cuda.synchronize()
+            want[r] = call()
+            torch.cuda.synchronize()
+        for r in range(30):
+            fill(r % 3)
+            assert torch.equal(call().view(torch.int16), want[r % 3].view(torch.int16)), (which, r)

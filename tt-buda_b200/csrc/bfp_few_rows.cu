@@ -394,6 +394,15 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
             load_rows<MB>(raw, at + 64 + face * F::kFace + 4 * t * F::kRow);
             raw.e = __ldg(reinterpret_cast<const uint32_t *>(at + face * 16 + 4 * t));
         };
+        auto ask_l2 = [&]() {             // a tile row's pieces, by address alone
+#pragma unroll
+            for (int f = 0; f < 2; f++) {
+                const int face = 2 * f + fc;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(at + 64 + face * F::kFace + 4 * t * F::kRow));
+                if (MB == 7) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + 64 + face * F::kFace + 4 * t * F::kRow + 32));
+                if (t == 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + face * 16));
+            }
+        };
         auto next_w = [&]() {
             at += row_bytes;
             if (MODE == kExpertsOut && ++w_kt == A.Kt) {
@@ -499,16 +508,28 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
             }
         } else {
             Part P0, P1;
-            if (n > 0) {
+            // What the launch in front of this one computes is waited for before anything it may have written is read.  Of the
+            // experts' second launch that is the first one, which writes h and no image and waited itself for all that came before: the
+            // images may be read at once.  The product's launch stands behind any other launch, which may have written the image:
+            // it only names its first rows to L2 before the wait.
+            auto first_w = [&]() {
+                if (n > 0) {
 #pragma unroll
-                for (int f = 0; f < HALVES; f++) load_w(P0.raw[f], f);
-                if (HALVES == 2) next_w();
-            }
-            // The weights were asked for before what the launch in front of this one computes is waited for: it writes activations,
-            // never weights, and what was in front of that one was complete before it let this launch begin.
+                    for (int f = 0; f < HALVES; f++) load_w(P0.raw[f], f);
+                    if (HALVES == 2) next_w();
+                }
+            };
             if (W.begin && MODE != kExpertsIn) {
+                if (MODE == kMatvec) {
+                    if (n > 0) ask_l2();
+                } else {
+                    first_w();
+                }
                 griddep_wait();
                 griddep_launch();
+                if (MODE == kMatvec) first_w();
+            } else {
+                first_w();
             }
             if (n > 0) {
                 rows_of();
@@ -867,8 +888,9 @@ __global__ void __launch_bounds__(256) sum_slots_kernel(const float *partial, in
         if (col + b < H) y[(int64_t)t * ldy + col + b] = __float2bfloat16_rn(f[b]);
 }
 
-// Every launch may begin before the one in front of it is done (it waits for that one before it reads activations or ids, and
-// before it writes).  Only launches that say so let it: those of this file and of the router.
+// Every launch may begin before the one in front of it is done.  It waits for that one before it reads or writes anything that any
+// launch in front may have written or may read; the exception (images, in the experts' second launch) is explained in `products`.
+// Only launches that say so let it: those of this file and of the router, each after its own wait.
 template <int MB, int NT, int MODE>
 cudaError_t launch_one(const Args &a, dim3 grid, int warps, cudaStream_t stream)
 {
