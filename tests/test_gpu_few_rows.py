@@ -691,3 +691,31 @@ def test_images_that_the_launch_in_front_has_just_written(ops, oracle, m):
         for r in range(30):
             fill(r % 3)
             assert torch.equal(call().view(torch.int16), want[r % 3].view(torch.int16)), (which, r)
+
+
+# ------------------------------------------------------------------------------------------------ the ends of the number range
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("exponent", [0, 128, 200, 254, 255])
+@pytest.mark.parametrize("rows", [1, 3, 12, 20])
+def test_matvec_outermost_shared_exponents(ops, oracle, df, exponent, rows):
+    """One weight row of the exponent among ordinary ones, met by activations of all sizes that leave the product in binary32, the
+    smallest subnormal ones among them.  Weights that unpack to infinities give infinities."""
+    code = getattr(ops.DF, df)
+    rec = {"Bfp8_b": 1088, "Bfp4_b": 576, "Bfp2_b": 320}[df]
+    powers = [p for p in (-133, -126, -115, -103, -60, -1, 0, 20, 60, 126) if -110 <= exponent - 127 + p <= 126 or (exponent == 255 and p <= -1)]
+    for k in (0, 14, 31):
+        raw = np.random.default_rng(exponent + k).integers(0, 256, rec, dtype=np.uint8)
+        raw[:64] = 127
+        for face in (2 * (k // 16), 2 * (k // 16) + 1):
+            raw[16 * face + k % 16] = exponent
+        w = oracle.unpack_untilize(raw, getattr(oracle, df), (1, 1, 32, 32))[0, 0].astype(np.float64)
+        img = torch.from_numpy(raw).cuda()
+        for first in range(len(powers)):
+            a = torch.zeros(rows, 32)
+            a[:, k] = torch.tensor([(-1.0) ** (r + first) * 2.0 ** powers[(r + first) % len(powers)] for r in range(rows)])
+            a = a.bfloat16()
+            got = ops.bfp_matvec(a.cuda(), img, 32, code, out_dtype=torch.float32).cpu().numpy()
+            want = (a[:, k].double().numpy()[:, None] * w[k]).astype(np.float32)
+            assert np.array_equal(got, want), (k, first)
+    if exponent == 255 and df != "Bfp2_b":
+        assert np.isinf(w).any() and np.isfinite(w[k]).any()

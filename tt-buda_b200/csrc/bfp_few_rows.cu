@@ -252,26 +252,30 @@ __device__ __forceinline__ void single_step(float (&acc)[8][1][4], const Raw<MB>
     }
 }
 
-// One token where some x 2^(E - 24) is no finite bfloat16: what is too much for the column goes to the weights.
+// One token where some x 2^(E - 24) is no finite bfloat16: what is too much for the column goes to the weights.  Of E = 255 all of it
+// does: such a weight is taken to its own size first, where 2^128 and above becomes an infinity, and the 2^-24 comes behind that
+// (the activations would lose their last bits to it below 2^-102, and such a product may still be as large as 2^26).
 template <int MB, int PIECES>
 __device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Raw<MB> &raw, const Args &A, const uint2 (&x)[PIECES][1])
 {
 #pragma unroll
     for (int q = 0; q < PIECES; q++) {
-        uint32_t b[2], s1[2], s2[2], s3[2];
+        uint32_t b[2], s1[2], s2[2], s3[2], s4[2];
 #pragma unroll
         for (int p = 0; p < 2; p++) {
-            int d[2], v[2];
+            int d[2], v[2], last[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int E = (raw.e >> (16 * p + 8 * h)) & 0xff, ex = ((p ? x[q][0].y : x[q][0].x) >> (7 + 16 * h)) & 0xff;
-                d[h] = E == 255 ? 255 : max(ex + E - kDown - 254, 0);   // a weight of 2^128 and above stays an infinity
-                v[h] = E - kDown - d[h];
+                d[h] = E == 255 ? 255 : max(ex + E - kDown - 254, 0);
+                v[h] = E == 255 ? 0 : E - kDown - d[h];
+                last[h] = E == 255 ? -kDown : 0;
             }
             b[p] = mul_bf16x2(mul_bf16x2(p ? x[q][0].y : x[q][0].x, pow2_pair(min(v[0], 127), min(v[1], 127))), pow2_pair(max(v[0] - 127, 0), max(v[1] - 127, 0)));
             s1[p] = pow2_pair(min(d[0], 127), min(d[1], 127));
             s2[p] = pow2_pair(min(max(d[0] - 127, 0), 127), min(max(d[1] - 127, 0), 127));
             s3[p] = pow2_pair(max(d[0] - 254, 0), max(d[1] - 254, 0));
+            s4[p] = pow2_pair(last[0], last[1]);
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -279,7 +283,8 @@ __device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Ra
             pair_of<MB>(raw, 0, j, A, a[0], a[1]);
             pair_of<MB>(raw, 1, j, A, a[2], a[3]);
 #pragma unroll
-            for (int c = 0; c < 4; c++) a[c] = mul_bf16x2(mul_bf16x2(mul_bf16x2(a[c], s1[c >> 1]), s2[c >> 1]), s3[c >> 1]);
+            for (int c = 0; c < 4; c++)
+                a[c] = mul_bf16x2(mul_bf16x2(mul_bf16x2(mul_bf16x2(a[c], s1[c >> 1]), s2[c >> 1]), s3[c >> 1]), s4[c >> 1]);
             mma16816(acc[j][0], a, b[0], b[1]);
         }
     }
