@@ -719,3 +719,25 @@ def test_matvec_outermost_shared_exponents(ops, oracle, df, exponent, rows):
             assert np.array_equal(got, want), (k, first)
     if exponent == 255 and df != "Bfp2_b":
         assert np.isinf(w).any() and np.isfinite(w[k]).any()
+
+
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("t", [1, 3, 12])
+def test_experts_infinite_weights_keep_their_sign(ops, oracle, df, t):
+    """A row of infinities of both signs in one expert's second matrix: h times them is an infinity of the product's sign, whatever
+    pieces h is carried in."""
+    e, h, i = 3, 96, 64
+    images, vals = _make_experts(oracle, e, h, i, df, 65)
+    broken = _rand((i, h), 66, 0.1)
+    broken[3, :] = np.where(np.arange(h) % 3 == 0, -np.inf, np.inf)
+    images[2][1], stored = _store(oracle, broken, df)
+    assert np.isinf(stored[3]).all() and np.isfinite(np.delete(stored, 3, 0)).all()
+    x = _bf16(_rand((t, h), 67))
+    for other in (0, 2):
+        ids = torch.tensor([[other, 1]] * t, dtype=torch.int32)
+        weights = torch.rand(t, 2, generator=torch.Generator().manual_seed(68)) + 0.1
+        got = ops.moe_experts(x.cuda(), weights.cuda(), ids.cuda(), *images, i, getattr(ops.DF, df))
+        a, u = x.double().numpy() @ vals[0][1][:, 3], x.double().numpy() @ vals[1][1][:, 3]
+        h3 = a / (1 + np.exp(-a)) * u
+        assert np.abs(h3).min() > 1e-4
+        assert np.array_equal(got.double().cpu().numpy(), np.sign(h3)[:, None] * stored[3])

@@ -198,6 +198,13 @@ __device__ __forceinline__ uint32_t scale_pair(uint32_t e, int p, int by)
     return (__byte_perm(e, 0u, p ? 0x4342u : 0x4140u) + (uint32_t)(by + 127) * 0x00010001u) << 7;
 }
 
+// A pair of weights for the second piece of h: 0 in the place of an infinity.  The first piece alone meets it, for the sum of the
+// pieces times an infinity is what the first one gives, and a second one of zero or of the other sign would make it a NaN.
+__device__ __forceinline__ uint32_t finite_pair(uint32_t v)
+{
+    return v & ~__vcmpeq2(v & 0x7fff7fffu, 0x7f807f80u);
+}
+
 // One 16-row step for up to 8 * NT tokens: the weights are scaled.  BIG where a shared exponent is above 127 (2^E is no
 // bfloat16 then: up to three factors).
 template <int MB, int NT, int PIECES, bool BIG>
@@ -229,9 +236,13 @@ __device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw,
             }
         }
 #pragma unroll
-        for (int q = 0; q < PIECES; q++)
+        for (int q = 0; q < PIECES; q++) {
+            if (BIG && q == 1)
+#pragma unroll
+                for (int c = 0; c < 4; c++) a[c] = finite_pair(a[c]);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) mma16816(acc[j][nt], a, x[q][nt].x, x[q][nt].y);
+        }
     }
 }
 
@@ -283,8 +294,10 @@ __device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Ra
             pair_of<MB>(raw, 0, j, A, a[0], a[1]);
             pair_of<MB>(raw, 1, j, A, a[2], a[3]);
 #pragma unroll
-            for (int c = 0; c < 4; c++)
+            for (int c = 0; c < 4; c++) {
                 a[c] = mul_bf16x2(mul_bf16x2(mul_bf16x2(mul_bf16x2(a[c], s1[c >> 1]), s2[c >> 1]), s3[c >> 1]), s4[c >> 1]);
+                if (q > 0) a[c] = finite_pair(a[c]);
+            }
             mma16816(acc[j][0], a, b[0], b[1]);
         }
     }
