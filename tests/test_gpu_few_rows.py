@@ -741,3 +741,77 @@ def test_experts_infinite_weights_keep_their_sign(ops, oracle, df, t):
         h3 = a / (1 + np.exp(-a)) * u
         assert np.abs(h3).min() > 1e-4
         assert np.array_equal(got.double().cpu().numpy(), np.sign(h3)[:, None] * stored[3])
+
+
+@pytest.mark.parametrize("t", [1, 3, 12])
+def test_experts_intermediate_keeps_binary32(ops, oracle, t):
+    """Results that are the difference of two intermediate values within 2^-12 to 2^-14 of one another.  One-hot tokens make
+    h = silu(g) u of single stored values.  The exponential is good to 2 units of the last place and carries 0.27 of the value, the
+    addition, the division and the product round once each, 2^-22 h in all; three additions of pieces lose up to 2^-23 of the larger
+    value each; the result is rounded to bfloat16."""
+    h, i = 32, 64
+    grid = np.arange(64, 128) / 64                    # what Bfp8_b stores of [1, 2)
+    hs = (grid / (1 + np.exp(-grid)))[:, None] * grid[None, :]
+    order = np.argsort(hs, axis=None)
+    flat = hs.reshape(-1)[order]
+    gap = (flat[1:] - flat[:-1]) / flat[1:]
+    at = np.flatnonzero((gap > 2.0 ** -14) & (gap < 2.0 ** -12))
+    assert len(at) > 32 * 32
+    rng = np.random.default_rng(69)
+    gate, up, down = np.zeros((h, i), np.float32), np.zeros((h, i), np.float32), np.zeros((i, h), np.float32)
+    for k in range(h):
+        for n in range(h):
+            p = rng.choice(at)
+            for c, which in enumerate((order[p], order[p + 1])):
+                gate[k, 2 * n + c], up[k, 2 * n + c] = grid[which // 64], grid[which % 64]
+    down[np.arange(0, i, 2), np.arange(h)], down[np.arange(1, i, 2), np.arange(h)] = 1, -1
+    images = [_store(oracle, m, "Bfp8_b") for m in (gate, up, down)]
+    assert all(np.array_equal(v, m) for (_, v), m in zip(images, (gate, up, down)))
+    want = gate.astype(np.float64)
+    want = want / (1 + np.exp(-want)) * up
+    tol = 2 * 2.0 ** -22 * want[:, ::2] + 3 * 2.0 ** -23 * want[:, ::2]
+    want = want[:, ::2] - want[:, 1::2]
+    tol = tol + 2.0 ** -8 * (np.abs(want) + tol)
+    images = [m[0].view(1, -1) for m in images]
+    for first in range(0, h, t):
+        x = torch.eye(h)[first:first + t].bfloat16().cuda()
+        rows = x.shape[0]
+        got = ops.moe_experts(x, torch.ones(rows, 1, device="cuda"), torch.zeros(rows, 1, dtype=torch.int32, device="cuda"), *images, i, ops.DF.Bfp8_b)
+        err = np.abs(got.double().cpu().numpy() - want[first:first + t])
+        assert (err <= tol[first:first + t]).all(), np.max(err / tol[first:first + t])
+
+
+@pytest.mark.parametrize("df", ["Bfp8_b", "Bfp4_b"])
+@pytest.mark.parametrize("t", [1, 3, 12, 40])
+def test_experts_not_finite_activations_stay_in_their_token(ops, oracle, df, t):
+    """Tokens with a NaN, an infinity, or values that overflow on the way, among ordinary ones of the same experts."""
+    e, h, i = 2, 64, 96
+    images, vals = _make_experts(oracle, e, h, i, df, 70)
+    x = _bf16(_rand((t, h), 71))
+    weights, ids = torch.rand(t, 2, generator=torch.Generator().manual_seed(72)) + 0.1, torch.tensor([[0, 1]] * t, dtype=torch.int32)
+    bad = {0: float("nan"), t // 2: float("inf"), t - 1: 3e38}
+    for row, v in bad.items():
+        y = x.clone()
+        y[row, 5] = v
+        got = ops.moe_experts(y.cuda(), weights.cuda(), ids.cuda(), *images, i, getattr(ops.DF, df), "gelu").cpu()
+        assert not torch.isfinite(got[row]).any(), (row, v)
+        if v != v:
+            assert torch.isnan(got[row]).all()
+        rest = [r for r in range(t) if r != row]
+        if rest:
+            _check_experts(got[rest], y[rest], weights[rest], ids[rest], vals, "gelu")
+
+
+@pytest.mark.parametrize("t", [1, 3, 12])
+def test_experts_infinite_intermediate_gives_infinities(ops, oracle, t):
+    """An intermediate value beyond binary32 is an infinity, and its products with weights of one sign are."""
+    h, i = 32, 32
+    gate, up, down = np.zeros((h, i), np.float32), np.zeros((h, i), np.float32), np.full((i, h), 0.5, np.float32)
+    gate[0, :] = up[0, :] = 1.5
+    down[:, ::3] = -1.0
+    images = [_store(oracle, m, "Bfp8_b")[0].view(1, -1) for m in (gate, up, down)]
+    x = torch.zeros(t, h)
+    x[:, 0] = 2.0 ** 100
+    got = ops.moe_experts(x.bfloat16().cuda(), torch.ones(t, 1, device="cuda"), torch.zeros(t, 1, dtype=torch.int32, device="cuda"), *images, i,
+                          ops.DF.Bfp8_b).double().cpu().numpy()
+    assert np.array_equal(got, np.broadcast_to(np.sign(down[0]) * np.inf, got.shape))

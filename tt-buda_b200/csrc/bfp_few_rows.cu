@@ -31,8 +31,8 @@
 //     every time.
 // Measured (B200): 1x4096x16384 Bfp4_b 8.5 us, 4.4 TB/s of its 37.8 MB, integer pipe 51 % active; 32x4096x16384 Bfp8_b 24.7 us;
 // the products of 16 tokens' 4 of 32 experts, 4096 x 2048 gated Bfp4_b, 114 us, 3.5 TB/s.
-// Sums are held in binary32 throughout.  h is carried between the two launches as two bfloat16 pieces (the rounded value and
-// the rounded rest, together within 2^-16 of h), so nothing is lost against a binary32 h at twice the tensor work.
+// Sums are held in binary32 throughout, and so is h between the two launches: a lane cuts the values it loads into three bfloat16
+// pieces (8 bits of the significand each, exactly all 24), for three times the tensor work and a fifth more instructions.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -77,7 +77,7 @@ struct Args {
     const int *ids;
     const float *wts;
     int top, E, act;
-    __nv_bfloat16 *h;            // [rows * top][2][32 * tile rows of the down matrix]
+    float *h;                    // [rows * top][32 * tile rows of the down matrix]
     int hpad;
     float *partial;              // experts-each: [rows * top][32 * tile columns of the down matrix]
     uint32_t m4, m16, m64;       // 4, 16, 64: multiplying by a parameter keeps a shift off the integer pipe (see pair_of)
@@ -198,8 +198,8 @@ __device__ __forceinline__ uint32_t scale_pair(uint32_t e, int p, int by)
     return (__byte_perm(e, 0u, p ? 0x4342u : 0x4140u) + (uint32_t)(by + 127) * 0x00010001u) << 7;
 }
 
-// A pair of weights for the second piece of h: 0 in the place of an infinity.  The first piece alone meets it, for the sum of the
-// pieces times an infinity is what the first one gives, and a second one of zero or of the other sign would make it a NaN.
+// A pair of weights for the pieces of h behind the first: 0 in the place of an infinity.  The first piece alone meets it, for the
+// sum of the pieces times an infinity is what the first one gives, and another one of zero would make it a NaN.
 __device__ __forceinline__ uint32_t finite_pair(uint32_t v)
 {
     return v & ~__vcmpeq2(v & 0x7fff7fffu, 0x7f807f80u);
@@ -237,7 +237,7 @@ __device__ __forceinline__ void step(float (&acc)[8][NT][4], const Raw<MB> &raw,
         }
 #pragma unroll
         for (int q = 0; q < PIECES; q++) {
-            if (BIG && q == 1)
+            if (BIG && q == 1)         // and for those behind
 #pragma unroll
                 for (int c = 0; c < 4; c++) a[c] = finite_pair(a[c]);
 #pragma unroll
@@ -303,6 +303,32 @@ __device__ __forceinline__ void single_step_wide(float (&acc)[8][1][4], const Ra
     }
 }
 
+// Activations as the tensor operand takes them: pairs of bfloat16, of a binary32 value (h) in three pieces that add up to it.  Each
+// piece is the upper half of what is left, so the sign stays and nothing overflows.  What is not finite leaves a rest that is no
+// number, which shows in the sums; the wide form (EXACT) then takes the rest as zero.
+template <bool EXACT, int PIECES, int NT, int WORDS>
+__device__ __forceinline__ void pieces_of(uint2 (&b)[PIECES][NT], const uint32_t (&x)[NT][WORDS])
+{
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        if constexpr (WORDS == 2) {
+            b[0][nt] = make_uint2(x[nt][0], x[nt][1]);
+        } else {
+            uint32_t v[4] = {x[nt][0], x[nt][1], x[nt][2], x[nt][3]};
+#pragma unroll
+            for (int q = 0; q < PIECES; q++) {
+                b[q][nt] = make_uint2(__byte_perm(v[0], v[1], 0x7632u), __byte_perm(v[2], v[3], 0x7632u));
+                if (q + 1 < PIECES)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float rest = __uint_as_float(v[i]) - __uint_as_float(v[i] & 0xffff0000u);
+                        v[i] = EXACT && !isfinite(rest) ? 0u : __float_as_uint(rest);
+                    }
+            }
+        }
+    }
+}
+
 // Elements k .. k+3 of a row (k a multiple of 4), zero past K; `pairs`: 4-byte loads are allowed.
 __device__ __forceinline__ uint2 load_four(const __nv_bfloat16 *row, int k, int K, bool pairs)
 {
@@ -356,7 +382,8 @@ template <int MB, int NT, int MODE, bool SINGLE>
 __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *smem, int group, int me, int workers, int tok_pitch)
 {
     using F = Fmt<MB>;
-    constexpr int PIECES = from_h(MODE) ? 2 : 1;
+    constexpr int PIECES = from_h(MODE) ? 3 : 1, WORDS = from_h(MODE) ? 4 : 2;      // of four activations: in products, as loaded
+    using X = std::conditional_t<from_h(MODE), float, __nv_bfloat16>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t image = (int64_t)A.Kt * A.Nt * F::kRec, row_bytes = (int64_t)A.Nt * F::kRec;
     const uint32_t each = (uint32_t)W.units / (uint32_t)workers, extra = (uint32_t)W.units - each * workers;
@@ -385,13 +412,13 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     constexpr int HALVES = MB == 7 || NT == 2 || (NT == 4 && MODE != kMatvec) ? 1 : 2;      // by registers
     struct Part {
         Raw<MB> raw[HALVES];
-        uint2 x[HALVES][PIECES][NT];
+        uint32_t x[HALVES][NT][WORDS];
     };
     float acc[8][NT][4];
     uint32_t seen = 0;                // all shared exponents met, ORed
 
     // One sweep over the share.  The first one takes every step as it usually is and looks afterwards whether one was not (an
-    // exponent of 128 or more, a column that is no finite number): then all is done again with the exact wide steps.  The plain
+    // exponent of 128 or more, a sum that is no finite number): then all is done again with the exact wide steps.  The plain
     // form is for activations that are not aligned.  The usual form's loop has no test in it, so that the compiler schedules
     // two tile rows as one; the last rows, where activations may end inside a tile row, come behind it (1x4096x16384 Bfp4_b 9.8
     // -> 8.7 us).
@@ -428,7 +455,7 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
                 if (++w_s * A.Kt < W.units) at = matrix + W.list[w_s] * image;
             }
         };
-        const __nv_bfloat16 *xp[NT];
+        const X *xp[NT];
         uint32_t present[NT];             // experts-out: all ones where the token has this expert
         auto rows_of = [&]() {
 #pragma unroll
@@ -436,38 +463,34 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
                 int tk = SINGLE ? 0 : nt * 8 + g;
                 if (tk >= W.n_tok) tk = 0;
                 present[nt] = ~0u;
-                if (MODE == kMatvec) {
+                if constexpr (MODE == kMatvec) {
                     xp[nt] = A.x + (int64_t)(W.tok0 + tk) * A.ldx;
-                } else if (MODE == kExpertsIn) {
+                } else if constexpr (MODE == kExpertsIn) {
                     xp[nt] = A.x + (int64_t)(W.list[2 * (W.tok0 + tk)] / A.top) * A.ldx;
-                } else if (MODE == kExpertsEach) {
-                    xp[nt] = A.h + (int64_t)W.list[2 * (W.tok0 + tk)] * 2 * A.hpad;
+                } else if constexpr (MODE == kExpertsEach) {
+                    xp[nt] = A.h + (int64_t)W.list[2 * (W.tok0 + tk)] * A.hpad;
                 } else {
                     const int r = W.rows[x_s * tok_pitch + tk];
                     if (r < 0) present[nt] = 0u;
-                    xp[nt] = A.h + (int64_t)max(r, 0) * 2 * A.hpad;
+                    xp[nt] = A.h + (int64_t)max(r, 0) * A.hpad;
                 }
                 xp[nt] += x_kt * 32 + 4 * t;
             }
         };
-        auto load_x = [&](uint2 (&x)[PIECES][NT], int f, bool inside) {      // inside: the tile row is known to lie inside the rows
+        auto load_x = [&](uint32_t (&x)[NT][WORDS], int f, bool inside) {    // inside: the tile row is known to lie inside the rows
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                if (inside || from_h(MODE) || x_kt < whole) {
+                if constexpr (from_h(MODE)) {
+                    const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(xp[nt] + f * 16));
+                    x[nt][0] = v.x; x[nt][1] = v.y; x[nt][2] = v.z; x[nt][3] = v.w;
+                    if (MODE == kExpertsOut && !SINGLE)
 #pragma unroll
-                    for (int q = 0; q < PIECES; q++) {
-                        const uint2 *p = reinterpret_cast<const uint2 *>(xp[nt] + q * A.hpad + f * 16);
-                        x[q][nt] = from_h(MODE) ? __ldcg(p) : *p;
-                    }
+                        for (int i = 0; i < 4; i++) x[nt][i] &= present[nt];
                 } else {
-                    x[0][nt] = load_four(xp[nt] - x_kt * 32 - 4 * t, x_kt * 32 + f * 16 + 4 * t, A.K, pairs);
+                    const uint2 v = inside || x_kt < whole ? *reinterpret_cast<const uint2 *>(xp[nt] + f * 16)
+                                                           : load_four(xp[nt] - x_kt * 32 - 4 * t, x_kt * 32 + f * 16 + 4 * t, A.K, pairs);
+                    x[nt][0] = v.x; x[nt][1] = v.y;
                 }
-                if (MODE == kExpertsOut && !SINGLE)
-#pragma unroll
-                    for (int q = 0; q < PIECES; q++) {
-                        x[q][nt].x &= present[nt];
-                        x[q][nt].y &= present[nt];
-                    }
             }
         };
         auto next_x = [&]() {
@@ -479,8 +502,10 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
                 if (++x_s * A.Kt < W.units) rows_of();
             }
         };
-        auto compute = [&](const Raw<MB> &raw, const uint2 (&x)[PIECES][NT]) {
+        auto compute = [&](const Raw<MB> &raw, const uint32_t (&loaded)[NT][WORDS]) {
             if (!WIDE) seen |= raw.e;
+            uint2 x[PIECES][NT];
+            pieces_of<WIDE>(x, loaded);
             if constexpr (WIDE && MODE == kExpertsOut && !SINGLE) {
                 // a stored infinity times the zero that stands for "not this token's expert" is no zero: such columns are left out
                 float part[8][NT][4] = {};
@@ -618,12 +643,14 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     if (from_h(MODE) || vec) sweep(Usual());
     else if constexpr (!from_h(MODE)) sweep(std::integral_constant<int, kPlain>());
     bool again = (seen & 0x80808080u) != 0;
-    if constexpr (SINGLE) {
+    if constexpr (SINGLE || from_h(MODE)) {
         float z = 0.0f;                   // a sum of zeros, unless something is not finite
 #pragma unroll
         for (int j = 0; j < 8; j++)
 #pragma unroll
-            for (int v = 0; v < 4; v++) z = fmaf(acc[j][0][v], 0.0f, z);
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) z = fmaf(acc[j][nt][v], 0.0f, z);
         again |= z != 0.0f;
     }
     if (__any_sync(0xffffffffu, again)) sweep(std::integral_constant<int, kWide>());
@@ -843,22 +870,9 @@ __global__ void __launch_bounds__(32 * kUnitWarps * units_per_sm(NT), 1) few_row
                 if (gated) up = total(tk, q + 4);
                 const float w = __int_as_float(list[2 * (W.tok0 + tk) + 1]);
                 float r2[2] = {activate(v.x, A.act) * up.x * w, activate(v.y, A.act) * up.y * w};
-                __nv_bfloat16 *h = A.h + (int64_t)list[2 * (W.tok0 + tk)] * 2 * A.hpad;
-                if (col < A.hpad) {
-                    uint32_t hi = 0, lo = 0;
-#pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        if (col + b >= A.N) continue;  // tile padding stays zero
-                        const __nv_bfloat16 a = __float2bfloat16_rn(r2[b]);
-                        // infinities and NaN are carried by the first piece alone
-                        const float rest = r2[b] - __bfloat162float(a);
-                        const __nv_bfloat16 d = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);
-                        hi |= (uint32_t)__bfloat16_as_ushort(a) << (16 * b);
-                        lo |= (uint32_t)__bfloat16_as_ushort(d) << (16 * b);
-                    }
-                    *reinterpret_cast<uint32_t *>(h + col) = hi;
-                    *reinterpret_cast<uint32_t *>(h + A.hpad + col) = lo;
-                }
+                if (col < A.hpad)                  // tile padding is zero: its weights are
+                    *reinterpret_cast<float2 *>(A.h + (int64_t)list[2 * (W.tok0 + tk)] * A.hpad + col) =
+                        make_float2(col < A.N ? r2[0] : 0.0f, col + 1 < A.N ? r2[1] : 0.0f);
             } else if (MODE == kExpertsEach) {
                 if (col < 32 * A.Nt)
                     *reinterpret_cast<float2 *>(A.partial + (int64_t)list[2 * (W.tok0 + tk)] * 32 * A.Nt + col) = v;
@@ -1023,7 +1037,7 @@ cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stre
     a.rows = m.T; a.K = m.H; a.Kt = Ht; a.N = m.I; a.Nt = It;
     a.w0 = (const uint8_t *)m.gate; a.w1 = (const uint8_t *)m.up;
     a.ids = m.ids; a.wts = m.weights; a.top = m.top; a.E = m.E; a.act = m.act;
-    a.h = (__nv_bfloat16 *)m.h; a.hpad = 32 * It;
+    a.h = (float *)m.h; a.hpad = 32 * It;
     const int span = m.up ? kGroupTiles / 2 : kGroupTiles;
     cudaError_t e = dispatch<kExpertsIn>(m.mant_bits, nt, a, (It + span - 1) / span, reached, Ht, most, sm_count, stream);
     if (e != cudaSuccess) return e;

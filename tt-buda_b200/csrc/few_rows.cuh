@@ -22,10 +22,10 @@ struct MoeArgs {
     void *h;                  // workspace
 };
 
-// Workspace between the expert launches: two bfloat16 pieces of every slot's intermediate row, and above kOneSum tokens a binary32
-// row of the result for every slot.
+// Workspace between the expert launches, binary32: every slot's intermediate row, and above kOneSum tokens a row of the result for
+// every slot.
 constexpr int kOneSum = 8;
-inline int64_t moe_h_bytes(int64_t T, int64_t top, int64_t I) { return T * top * 2 * (32 * ((I + 31) / 32)) * 2; }
+inline int64_t moe_h_bytes(int64_t T, int64_t top, int64_t I) { return T * top * (32 * ((I + 31) / 32)) * 4; }
 inline int64_t moe_workspace(int64_t T, int64_t top, int64_t H, int64_t I)
 {
     return moe_h_bytes(T, top, I) + (T > kOneSum ? T * top * (32 * ((H + 31) / 32)) * 4 : 0);
