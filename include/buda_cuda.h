@@ -391,7 +391,8 @@ int buda_bfp_matvec(const void *A, int64_t M, int64_t K, int64_t lda, const void
 
 /* The router of a mixture of experts: scores X[T,H] (bfloat16) @ W_router[E,H]^T (bfloat16 or binary32, one row for each
  * expert), their softmax over the experts, and for each token the `top` experts of the largest scores in descending order,
- * the lowest index first among equal ones; a NaN score ranks below every number.  weights[T,top] (binary32) are the softmax
+ * the lowest index first among equal ones; a NaN score ranks below every number.  Scores are sums of 64 bits over groups of 8 products
+ * that are added in binary32, and are compared in 64 bits.  weights[T,top] (binary32) are the softmax
  * values, divided by their sum over the chosen experts when `renormalize` is not 0; ids[T,top] (int32) the experts.
  * T <= 64, E <= 256, top <= 16 and <= E. */
 #define BUDA_MAX_EXPERTS 256

@@ -815,3 +815,28 @@ def test_experts_infinite_intermediate_gives_infinities(ops, oracle, t):
     got = ops.moe_experts(x.bfloat16().cuda(), torch.ones(t, 1, device="cuda"), torch.zeros(t, 1, dtype=torch.int32, device="cuda"), *images, i,
                           ops.DF.Bfp8_b).double().cpu().numpy()
     assert np.array_equal(got, np.broadcast_to(np.sign(down[0]) * np.inf, got.shape))
+
+
+@pytest.mark.parametrize("router", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("e", [7, 64, 256])
+def test_route_orders_scores_that_binary32_cannot_tell_apart(ops, router, e):
+    """Scores of thousands that differ by 2^-9 to 2^-15.  At most one product of each 8 is not zero, so that every sum is exact in
+    64 bits."""
+    h, top = 512, min(e, 16)
+    rng = np.random.default_rng(73 + e)
+    w = np.zeros((e, h), np.float32)
+    w[:, 0:128:8] = (rng.integers(128, 256, 16) * 4).astype(np.float32)      # the same for all experts
+    place = rng.permutation(e)
+    for b in range(8):
+        w[:, 128 + 8 * b] = (place >> b & 1) * 2.0 ** (b - 15)
+    x = torch.ones(3, h)
+    x[1] *= -1
+    x[2] *= 2
+    weights, ids = ops.moe_route(x.bfloat16().cuda(), torch.from_numpy(w).to(router).cuda(), top, True)
+    descending = np.argsort(-place)
+    for row, order in ((0, descending), (1, descending[::-1]), (2, descending)):
+        assert ids[row].cpu().tolist() == order[:top].tolist()
+    score = place[descending] * 2.0 ** -15
+    p = np.exp(score[:top] - score[0])
+    # the exponential and the sum of up to 16 of them: 2 and 16 units of 2^-23, the quotient one rounding
+    assert np.abs(weights[0].double().cpu().numpy() * p.sum() / p - 1).max() <= 19 * 2.0 ** -23

@@ -9,10 +9,12 @@
 // shared memory; the warp of token i chooses in CTA i % 8.  Most of a call is waiting for w, so a warp asks for a row's piece in one
 // go (8 octets a lane).  w may be what the launch in front has written, as x may: before that one is complete its addresses are
 // only named to L2, which brings no value into the kernel.
-// Scores decide which experts run: a lane adds its products 8 at a time, the 32 lanes and the pieces of a row are joined in
-// binary64, and the result is rounded to binary32 once.
-// Measured (B200): one token, 8 experts of 1024 binary32 weights 3.6 us; 16 tokens, 128 experts of 4096 bfloat16 weights 10.8 us
-// (16 clusters read and widen the same 1 MB; the choice of 8 takes 0.8 of it).
+// Scores decide which experts run: a lane adds 8 products in binary32 (off by at most 7 * 2^-24 of their magnitudes), everything
+// behind that is binary64 up to the choice, and the softmax takes binary64 differences.  Sums and choice in binary32 take 0.8 us less
+// for the 16 tokens below, but experts closer than 2^-24 of their scores come in the wrong order and the weights are off by
+// 1.4e-7 instead of 6e-8.  Keeping what every addition rounds off leaves 5.9e-8 and takes 4 us more.
+// Measured (B200): one token, 8 experts of 1024 binary32 weights 3.5 us; 16 tokens, 128 experts of 4096 bfloat16 weights 11.6 us
+// (16 clusters read and widen the same 1 MB).
 #include <cuda_bf16.h>
 
 #include "few_rows.cuh"
@@ -30,12 +32,12 @@ __device__ __forceinline__ void cluster_sync()
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(const float *p, uint32_t rank)
+__device__ __forceinline__ double ld_cluster_f64(const double *p, uint32_t rank)
 {
     uint32_t a;
-    float v;
+    double v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(a) : "memory");
     return v;
 }
 
@@ -91,12 +93,12 @@ struct Octet<float> {
     }
 };
 
-// Binary32 in an order that unsigned integers have: NaN below every number, 0 for "already chosen".
-__device__ __forceinline__ uint32_t order_of(float l)
+// Binary64 in an order that unsigned integers have: NaN below every number, 0 for "already chosen".
+__device__ __forceinline__ uint64_t order_of(double l)
 {
     if (isnan(l)) return 1u;
-    const uint32_t b = __float_as_uint(l + 0.0f);
-    return b >> 31 ? ~b : b | 0x80000000u;
+    const uint64_t b = (uint64_t)__double_as_longlong(l + 0.0);
+    return b >> 63 ? ~b : b | (1ull << 63);
 }
 
 constexpr int kStaged = 28 * 1024;       // activations of a block of tokens up to this size are kept in shared memory
@@ -107,7 +109,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2)
                  float *weights, int *ids)
 {
     __shared__ double part[kPerCta * TB * kWarps];      // [expert of this CTA][token][piece of the row]
-    __shared__ float score[kPerCta * TB];
+    __shared__ double score[kPerCta * TB];
     extern __shared__ __align__(16) __nv_bfloat16 xs[]; // [TB][8 * octets], zero past H
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t rank;
@@ -157,12 +159,12 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2)
         }
         __syncthreads();
     }
-    float s[TB];
+    double s[TB];
     for (int it = 0; it < tasks * batches; it++) {
         if (it) load(it);
         if (it % batches == 0)
 #pragma unroll
-            for (int i = 0; i < TB; i++) s[i] = 0.0f;
+            for (int i = 0; i < TB; i++) s[i] = 0.0;
 #pragma unroll
         for (int u = 0; u < kBatch; u++) {
             if (o0 + 32 * u >= o1) break;
@@ -196,7 +198,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2)
     for (int i = tid; i < mine * TB; i += kThreads) {
         double v = 0.0;
         for (int p = 0; p < split; p++) v += part[i * split + p];
-        score[i] = (float)v;
+        score[i] = v;
     }
     cluster_sync();
     // warp `warp` of CTA `rank` chooses for token 8 * warp + rank of the block
@@ -204,26 +206,26 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2)
     if (i < nt) {
         constexpr int kPer = kMaxExperts / 32;
         const int per = (E + 31) / 32;
-        float l[kPer];
-        uint32_t key[kPer];
+        double l[kPer];
+        uint64_t key[kPer];
 #pragma unroll
         for (int q = 0; q < kPer; q++) {
-            l[q] = 0.0f;
+            l[q] = 0.0;
             key[q] = 0u;
             if (q < per) {
                 const int e = q * 32 + lane;
                 if (e < E) {
-                    l[q] = ld_cluster_f32(&score[(e / kCluster) * TB + i], e % kCluster);
+                    l[q] = ld_cluster_f64(&score[(e / kCluster) * TB + i], e % kCluster);
                     key[q] = order_of(l[q]);
                 }
             }
         }
         int my_id = 0;              // lane s keeps the s-th choice
-        float my_l = 0.0f, most = 0.0f;
+        double my_l = 0.0, most = 0.0;
         for (int s = 0; s < top; s++) {
-            uint32_t best = 0;
+            uint64_t best = 0;
             int at = 0;
-            float bl = 0.0f;
+            double bl = 0.0;
 #pragma unroll
             for (int q = 0; q < kPer; q++)
                 if (q < per && key[q] > best) {
@@ -231,32 +233,39 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2)
                     at = q * 32 + lane;
                     bl = l[q];
                 }
-            const uint32_t top_key = __reduce_max_sync(0xffffffffu, best);
-            const uint32_t id = __reduce_min_sync(0xffffffffu, best == top_key ? (uint32_t)at : 0xffffffffu);
-            const float v = __shfl_sync(0xffffffffu, bl, id & 31);
+            const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+            const uint32_t among = __ballot_sync(0xffffffffu, (uint32_t)(best >> 32) == high);
+            int id;
+            if (__popc(among) == 1) {
+                id = __shfl_sync(0xffffffffu, at, __ffs(among) - 1);
+            } else {            // the same in the upper 32 bits
+                const uint32_t low = __reduce_max_sync(0xffffffffu, among >> lane & 1 ? (uint32_t)best : 0u);
+                id = (int)__reduce_min_sync(0xffffffffu, (among >> lane & 1) && (uint32_t)best == low ? (uint32_t)at : 0xffffffffu);
+            }
+            const double v = __shfl_sync(0xffffffffu, bl, id & 31);
 #pragma unroll
             for (int q = 0; q < kPer; q++)
-                if (q * 32 + lane == (int)id) key[q] = 0;
+                if (q * 32 + lane == id) key[q] = 0;
             if (s == 0) most = v;
             if (lane == s) {
-                my_id = (int)id;
+                my_id = id;
                 my_l = v;
             }
         }
         float sum = 0.0f;
         if (renorm) {
-            sum = lane < top ? expf(my_l - most) : 0.0f;
+            sum = lane < top ? expf((float)(my_l - most)) : 0.0f;
         } else {
 #pragma unroll
             for (int q = 0; q < kPer; q++)
-                if (q * 32 + lane < E) sum += expf(l[q] - most);
+                if (q * 32 + lane < E) sum += expf((float)(l[q] - most));
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (lane < top) {
             const int64_t o = (int64_t)(t0 + i) * top + lane;
             ids[o] = my_id;
-            weights[o] = expf(my_l - most) / sum;
+            weights[o] = expf((float)(my_l - most)) / sum;
         }
     }
     cluster_sync();      // no CTA leaves while another reads its scores
