@@ -840,3 +840,24 @@ def test_route_orders_scores_that_binary32_cannot_tell_apart(ops, router, e):
     p = np.exp(score[:top] - score[0])
     # the exponential and the sum of up to 16 of them: 2 and 16 units of 2^-23, the quotient one rounding
     assert np.abs(weights[0].double().cpu().numpy() * p.sum() / p - 1).max() <= 19 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("t", [1, 4, 16])
+def test_experts_gelu_of_negative_values_keeps_its_digits(ops, oracle, t):
+    """gelu(v) for v from -2 to -8, where 1 + erf is a small difference: results, not sums, for the second matrix is the unit matrix.
+    z = v / sqrt 2 is off by 2 * 2^-24 of itself, which erfc turns into 2 z^2 times that; erfc is good to 4 units of 2^-23; two
+    products and the rounding to bfloat16."""
+    h = i = 32
+    gate = -(64 + np.random.default_rng(74).integers(0, 64, (h, i))).astype(np.float32) / 64
+    images = [_store(oracle, m, "Bfp8_b") for m in (gate, np.eye(i, h, dtype=np.float32))]
+    assert np.array_equal(images[0][1], gate) and np.array_equal(images[1][1], np.eye(i, h))
+    gate_i, down_i = (m[0].view(1, -1) for m in images)
+    for first in range(0, h, t):
+        x = torch.eye(h)[first:first + t] * torch.linspace(2, 4, t).view(t, 1)
+        x = x.bfloat16()
+        got = ops.moe_experts(x.cuda(), torch.ones(t, 1, device="cuda"), torch.zeros(t, 1, dtype=torch.int32, device="cuda"), gate_i, None, down_i, i,
+                              ops.DF.Bfp8_b, "gelu")
+        v = x.double() @ torch.from_numpy(gate).double()
+        want = (0.5 * v * torch.erfc(-v / 2 ** 0.5)).numpy()
+        rel = 2 * (v.numpy() ** 2 / 2) * 2 * 2.0 ** -24 + 4 * 2.0 ** -23 + 2 * 2.0 ** -24
+        assert (np.abs(got.double().cpu().numpy() - want) <= (2.0 ** -8 + 1.01 * rel) * np.abs(want)).all()

@@ -346,7 +346,7 @@ __device__ __forceinline__ uint2 load_four(const __nv_bfloat16 *row, int k, int 
 __device__ __forceinline__ float activate(float v, int act)
 {
     if (act == BUDA_ACT_SILU) return v / (1.0f + expf(-v));
-    return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+    return 0.5f * v * erfcf(v * -0.70710678118654752f);      // 1 + erf(z) = erfc(-z), which keeps its digits where erf is near -1
 }
 
 // Shared memory: [the warps' sums][the CTA's sums][tables]
