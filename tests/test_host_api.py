@@ -363,3 +363,33 @@ def test_few_row_operators_refuse_bad_arguments():
     assert _cabi.lib.buda_moe_workspace_bytes(9, 2, 100, 33) == 9 * 2 * (2 * 64 * 2 + 128 * 4)
     for bad in ((65, 2, 32, 32), (-1, 2, 32, 32), (1, 0, 32, 32), (1, 17, 32, 32), (1, 1, 32, 0), (1, 1, 0, 32), (1, 1, 32, 1 << 25)):
         assert _cabi.lib.buda_moe_workspace_bytes(*bad) == -1, bad
+
+
+_WITHOUT_TORCH_OPS = """
+import sys
+sys.path[:0] = {path!r}
+sys.modules["pybuda._torch_ops"] = None
+import torch
+from pybuda import cuda_ops as ops
+for call in (lambda: ops.bfp_matvec(None, None, 1), lambda: ops.moe_route(None, None, 1),
+             lambda: ops.moe_experts(None, None, None, None, None, None, 1), lambda: ops.moe_layer(None, None, 1, None, None, None, 1)):
+    try:
+        call()
+        raise SystemExit("not refused")
+    except ImportError as e:
+        assert "build.py" in str(e), e
+try:
+    ops.tilize_pack(torch.zeros(1, 1, 32, 32), ops.DF.Bfp8_b)
+    raise SystemExit("no device asked for")
+except (RuntimeError, ValueError) as e:
+    assert "CUDA" in str(e), e
+print("the others work")
+"""
+
+
+def test_only_the_few_row_operators_need_the_torch_extension():
+    import subprocess
+    import sys
+
+    r = subprocess.run([sys.executable, "-c", _WITHOUT_TORCH_OPS.format(path=[p for p in sys.path if p])], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "the others work" in r.stdout, r.stdout + r.stderr[-2000:]

@@ -14,10 +14,20 @@ from ._cabi import QueueGeom, check
 
 try:
     from . import _torch_ops
-except ImportError as e:
-    raise ImportError("pybuda._torch_ops is missing or does not load: build it with `python tt-buda_b200/build.py`") from e
 
-_torch_ops.set_error(_cabi.BudaError)
+    _torch_ops.set_error(_cabi.BudaError)
+except ImportError as _e:
+    class _NotLoaded:
+        """Stands for pybuda._torch_ops where it does not load: the few-row operators need it, nothing else here does."""
+
+        def __init__(self, why):
+            self._why = why
+
+        def __getattr__(self, name):
+            raise ImportError(f"{name}: pybuda._torch_ops is missing or does not load; build it with "
+                              "`python tt-buda_b200/build.py`") from self._why
+
+    _torch_ops = _NotLoaded(_e)
 
 
 class DF(enum.IntEnum):
