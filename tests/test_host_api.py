@@ -393,3 +393,47 @@ def test_only_the_few_row_operators_need_the_torch_extension():
 
     r = subprocess.run([sys.executable, "-c", _WITHOUT_TORCH_OPS.format(path=[p for p in sys.path if p])], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "the others work" in r.stdout, r.stdout + r.stderr[-2000:]
+
+
+def _build_module():
+    import importlib.util
+    import os
+
+    spec = importlib.util.spec_from_file_location("buda_build", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tt-buda_b200", "build.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+def test_torch_extension_is_rebuilt_for_another_torch(tmp_path, monkeypatch):
+    import os
+
+    import torch
+
+    build = _build_module()
+    src, target, stamp = (tmp_path / n for n in ("few_rows.cpp", "ops.so", "torch_ops.txt"))
+    src.write_text("")
+    target.write_text("")
+    newest = os.path.getmtime(os.path.join(build.INCLUDE, "buda_cuda.h")) + 10
+    os.utime(src, (newest - 5, newest - 5))
+    os.utime(target, (newest, newest))
+    key = build.torch_ops_key()
+    assert torch.__version__ in key
+    assert build.torch_ops_stale(target, src, stamp, key)             # built before what it is good for was written down
+    stamp.write_text(key)
+    assert not build.torch_ops_stale(target, src, stamp, key)
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    assert build.torch_ops_stale(target, src, stamp, build.torch_ops_key())
+    monkeypatch.undo()
+    os.utime(src, (newest + 1, newest + 1))
+    assert build.torch_ops_stale(target, src, stamp, key)
+
+
+def test_build_goes_on_where_torch_has_no_cuda_libraries(monkeypatch, capsys):
+    import torch
+
+    build = _build_module()
+    monkeypatch.setattr(torch.version, "cuda", None)
+    monkeypatch.setattr(build, "_run", lambda cmd: pytest.fail("nothing is compiled"))
+    assert build.build_torch_ops(force=True) is None
+    assert "not built" in capsys.readouterr().out

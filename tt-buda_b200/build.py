@@ -117,11 +117,35 @@ def torch_ops_target():
     return os.path.join(HERE, "pybuda", "_torch_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
+def torch_ops_key():
+    """What a binary of pybuda._torch_ops is good for; None where it cannot be built: no torch, or one without CUDA libraries."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    if torch.version.cuda is None:
+        return None
+    return f"torch {torch.__version__}, CUDA {torch.version.cuda}, C++11 ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}\n"
+
+
+def torch_ops_stale(target, src, stamp, key):
+    """Whether pybuda._torch_ops has to be built: its source or the C ABI is newer, or it was built for another torch."""
+    if _newer(target, [src, os.path.join(INCLUDE, "buda_cuda.h")]) or not os.path.exists(stamp):
+        return True
+    with open(stamp) as f:
+        return f.read() != key
+
+
 def build_torch_ops(force=False):
     """pybuda._torch_ops: the operators whose calls are too short for ctypes, on torch tensors (torch's headers and libraries)."""
     target = torch_ops_target()
     src = os.path.join(HOST_DIR, "torch_ops", "few_rows.cpp")
-    if not (force or _newer(target, [src, os.path.join(INCLUDE, "buda_cuda.h")])):
+    stamp = os.path.join(HOST_DIR, "build", "torch_ops.txt")
+    key = torch_ops_key()
+    if key is None:
+        print("pybuda._torch_ops is not built: it needs a torch with CUDA libraries; the few-row operators will say that it is missing")
+        return None
+    if not (force or torch_ops_stale(target, src, stamp, key)):
         return target
     import torch
     from torch.utils import cpp_extension
@@ -131,6 +155,9 @@ def build_torch_ops(force=False):
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] +
          [a for i in inc for a in ("-isystem", i)] + [src, "-o", target, "-L", LIB_DIR, "-lbuda_cuda", "-Wl,-rpath,$ORIGIN/../lib"] +
          [a for d in cpp_extension.library_paths() for a in ("-L", d)] + ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"])
+    os.makedirs(os.path.dirname(stamp), exist_ok=True)
+    with open(stamp, "w") as f:
+        f.write(key)
     return target
 
 
