@@ -861,3 +861,128 @@ def test_experts_gelu_of_negative_values_keeps_its_digits(ops, oracle, t):
         want = (0.5 * v * torch.erfc(-v / 2 ** 0.5)).numpy()
         rel = 2 * (v.numpy() ** 2 / 2) * 2 * 2.0 ** -24 + 4 * 2.0 ** -23 + 2 * 2.0 ** -24
         assert (np.abs(got.double().cpu().numpy() - want) <= (2.0 ** -8 + 1.01 * rel) * np.abs(want)).all()
+
+
+# ------------------------------------------------------------------------------------------------ forms that a caller meets
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_one_unaligned_row(ops, oracle, df, offset):
+    """A single row whose values begin at any element: the product, and the experts."""
+    k, n = 333, 150
+    img, w = _store(oracle, _rand((k, n), 75, 0.1), df)
+    buf = _bf16(_rand((k + 8,), 76)).cuda()
+    a = buf[offset:offset + k].view(1, k)
+    for dtype in (torch.bfloat16, torch.float32):
+        _check_sum(ops.bfp_matvec(a, img, n, getattr(ops.DF, df), out_dtype=dtype), a.double().cpu().numpy(), w, dtype)
+    e, i = 3, 70
+    images, vals = _make_experts(oracle, e, k, i, df, 77)
+    weights, ids = torch.tensor([[0.4, 0.7]]), torch.tensor([[2, 0]], dtype=torch.int32)
+    got = ops.moe_experts(a, weights.cuda(), ids.cuda(), *images, i, getattr(ops.DF, df))
+    _check_experts(got, a.cpu(), weights, ids, vals, "silu")
+
+
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("t", [7, 12, 40])
+def test_experts_of_unaligned_rows(ops, oracle, df, t):
+    e, h, i = 3, 101, 70
+    images, vals = _make_experts(oracle, e, h, i, df, 78)
+    x = _bf16(_rand((t * h + 1,), 79)).cuda()[1:].view(t, h)
+    weights, ids = _routing(t, e, 2, 80)
+    got = ops.moe_experts(x, weights.cuda(), ids.cuda(), *images, i, getattr(ops.DF, df))
+    _check_experts(got, x.cpu(), weights, ids, vals, "silu")
+
+
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("t", [1, 3, 12, 40])
+@pytest.mark.parametrize("scale", [2.0, 0.6])
+def test_experts_with_large_weights(ops, oracle, df, t, scale):
+    """All three matrices with shared exponents of 128 and more: nearly all of them, or some."""
+    e, h, i = 2, 160, 96
+    parts = [[_store(oracle, _rand(s, 81 + 10 * which + k, scale), df) for k in range(e)] for which, s in enumerate(((h, i), (h, i), (i, h)))]
+    images, vals = [torch.stack([p[0] for p in m]) for m in parts], [np.stack([p[1] for p in m]) for m in parts]
+    assert all(int(m[:, :64].max()) >= 128 and (scale > 1 or int(m[:, :64].min()) < 128) for m in images)
+    x = _bf16(_rand((t, h), 84, 0.05))
+    weights, ids = torch.rand(t, 2, generator=torch.Generator().manual_seed(85)), torch.tensor([[0, 1]] * t, dtype=torch.int32)
+    got = ops.moe_experts(x.cuda(), weights.cuda(), ids.cuda(), *images, i, getattr(ops.DF, df), "gelu")
+    _check_experts(got, x, weights, ids, vals, "gelu")
+
+
+@pytest.mark.parametrize("df", FORMATS)
+@pytest.mark.parametrize("rows", [9, 16, 17, 32, 64])
+def test_matvec_rows_of_mixed_magnitudes(ops, oracle, df, rows):
+    """Blocks of very unlike shared exponents against activations that undo them, in wider passes."""
+    k, n = 160, 200
+    rng = np.random.default_rng(86)
+    power = rng.integers(-60, 61, (k, 1))
+    w0 = rng.standard_normal((k, n)) * 2.0 ** power * np.repeat(2.0 ** rng.integers(-8, 9, (k, -(-n // 16))), 16, 1)[:, :n]
+    img, w = _store(oracle, w0.astype(np.float32), df)
+    a = torch.from_numpy(rng.standard_normal((rows, k)) * 2.0 ** (-power[:, 0] + 20)).bfloat16()
+    got = ops.bfp_matvec(a.cuda(), img, n, getattr(ops.DF, df), out_dtype=torch.float32)
+    _check_sum(got, a.double().numpy(), w, torch.float32)
+
+
+@pytest.mark.parametrize("t", [1, 6, 12, 40])
+def test_weights_of_dropped_slots_are_not_looked_at(ops, oracle, t):
+    """A padded batch: slots without an expert hold whatever was there."""
+    e, h, i = 4, 96, 64
+    images, vals = _make_experts(oracle, e, h, i, "Bfp4_b", 87)
+    x = _bf16(_rand((t, h), 88))
+    weights, ids = _routing(t, e, 3, 89)
+    ids[:, 1] = torch.tensor([-1, 4, -2 ** 31, 2 ** 31 - 1], dtype=torch.int32).repeat(t)[:t]
+    weights[:, 1] = torch.tensor([float("nan"), float("inf")]).repeat(t)[:t]
+    got = ops.moe_experts(x.cuda(), weights.cuda(), ids.cuda(), *images, i)
+    _check_experts(got, x, weights, ids, vals, "silu")
+
+
+@pytest.mark.parametrize("t", [1, 8, 12, 64])
+def test_layer_in_place(ops, oracle, t):
+    e, h, i = 6, 128, 64
+    images, _ = _make_experts(oracle, e, h, i, "Bfp8_b", 90)
+    wr = torch.randn(e, h, generator=torch.Generator().manual_seed(91)).cuda()
+    x = _bf16(_rand((t, h), 92)).cuda()
+    want = ops.moe_layer(x, wr, 2, *images, i, ops.DF.Bfp8_b)
+    for _ in range(10):
+        y = x.clone()
+        assert ops.moe_layer(y, wr, 2, *images, i, ops.DF.Bfp8_b, out=y) is y
+        assert torch.equal(y, want)
+
+
+def test_calls_from_two_threads_at_once(ops, oracle):
+    import threading
+
+    e, h, i = 6, 128, 96
+    images, _ = _make_experts(oracle, e, h, i, "Bfp4_b", 93)
+    proj, _ = _store(oracle, _rand((h, h), 94, h ** -0.5), "Bfp4_b")
+    wr = torch.randn(e, h, generator=torch.Generator().manual_seed(95)).cuda()
+    xs = [_bf16(_rand((t, h), 96 + t)).cuda() for t in (1, 3, 12, 40)]
+    want = [_block(ops, x, proj, wr, images, i) for x in xs]
+    torch.cuda.synchronize()
+    wrong, errors = [], []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for r in range(40):
+                    got = _block(ops, xs[k], proj, wr, images, i)
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                        wrong.append((k, r))
+        except Exception as ex:           # noqa: BLE001 -- shown below
+            errors.append(ex)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    assert not errors and not wrong, (errors, wrong)
+
+
+@pytest.mark.parametrize("router", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t,h,e,top", [(1, 16384, 8, 2), (2, 20001, 3, 1), (30, 7168, 16, 4), (64, 4104, 16, 4), (37, 4001, 9, 3)])
+def test_route_rows_too_long_to_be_staged(ops, router, t, h, e, top):
+    g = torch.Generator().manual_seed(t + h + e)
+    x, w = torch.randn(t, h, generator=g).bfloat16(), (torch.randn(e, h, generator=g) * 2 * h ** -0.5).to(router)
+    weights, ids = ops.moe_route(x.cuda(), w.cuda(), top, True)
+    ref, rid = _route_ref(x, w, top, True)
+    assert np.array_equal(ids.cpu().numpy(), rid)
+    # a score is off by 7 * 2^-24 of its products' magnitudes at most, a weight by twice that and a few units of 2^-24
+    mag = (x.double().abs() @ w.double().abs().T).max().item()
+    assert (np.abs(weights.double().cpu().numpy() - ref) <= (14 * mag + 8) * 2.0 ** -24 * ref).all()
