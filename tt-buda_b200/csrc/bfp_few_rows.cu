@@ -3,7 +3,7 @@
 //   matvec      Y[m, n]  = sum_k A[m, k] W[k, n]
 //   experts     h[s, i]  = w_s act((x_t G_e)[i]) (x_t U_e)[i]            ("in")
 //               y[t, n]  = sum over the slots s of token t of sum_i h[s, i] D_e[i, n]
-// The second product of the experts has two forms.  Up to 8 tokens ("out"): a column group runs through all reached experts
+// The second product of the experts has two forms.  Up to 3 tokens ("out"): a column group runs through all reached experts
 // as if their rows were one long sum, with zeros where a token has not chosen an expert; nothing is left to add up.  More
 // tokens ("each"): every expert's products on their own with only its own tokens, into binary32 rows of the workspace that a third
 // launch adds up -- otherwise most columns of the tensor product would be zeros (16 experts, 32 tokens, two each: 4 of 32).
@@ -978,7 +978,7 @@ Split split_of(int64_t groups, int64_t tile_rows, int sm_count, int per_sm)
 template <int MODE, int MB>
 cudaError_t launch_nt(int nt, const Args &a, dim3 grid, int warps, cudaStream_t stream)
 {
-    // one sum over all experts serves up to 8 tokens, sums of their own more than that
+    // one sum over all experts serves up to kOneSum tokens, sums of their own more than that
     if constexpr (MODE != kExpertsEach)
         if (nt == 0) return launch_one<MB, 0, MODE>(a, grid, warps, stream);
     if constexpr (MODE != kExpertsOut) {
@@ -1026,12 +1026,22 @@ cudaError_t launch_moe_experts(const MoeArgs &m, int sm_count, cudaStream_t stre
 {
     const int Ht = (m.H + 31) / 32, It = (m.I + 31) / 32;
     const int slots = m.T * m.top, most = m.E < slots ? m.E : slots;
-    // The experts that independent choices reach on average, and the tokens of one.  Up to 4 fit a group of 8 nearly always, and
-    // where they do not a second pass costs less than wider passes for all (32 tokens, 2 of 16 experts of 2048 x 1024 Bfp4_b: 24 us,
-    // 27 with a second pass, against 31.5 in passes of 16).
+    // The experts that independent choices reach on average, and the tokens of one.  A pass over an expert's weights takes 8, 16 or
+    // 32 tokens.  Measured, us, passes of 8 / 16 / 32, gated, 4 of 16 experts (B200):
+    //   tokens an expert       5                   6                   8                   10                  12                  16
+    //   1024 x 1024 Bfp4_b     22.5 / 27.5 / 31.9  28.5 / 28.2 / 32.4  31.6 / 28.4 / 32.7  32.8 / 29.6 / 34.5  39.5 / 38.0 / 35.1  45.2 / 46.8 / 36.2
+    //   2048 x 1024 Bfp2_b     25.7 / 32.5 / 51.2  32.8 / 33.1 / 52.0  36.7 / 33.5 / 52.6  37.8 / 34.6 / 54.6  44.4 / 45.3 / 55.8  53.1 / 56.7 / 57.1
+    //   1024 x 2048 Bfp8_b     35.4 / 45.6 / 66.4  42.8 / 46.3 / 67.2  47.1 / 47.1 / 68.1  50.8 / 49.2 / 71.1  58.6 / 63.3 / 72.3  67.4 / 74.5 / 74.3
+    // and 2 of 4 experts, 16 tokens an expert: 29.7 / 26.0 / 19.5, 33.0 / 32.2 / 23.2, 34.8 / 38.4 / 23.7.
+    // One sum over all experts (up to kOneSum tokens) against sums of their own for 2, 3, 4 and 8 tokens:
+    //   4 of 32 of 1024 x 1024 Bfp4_b  14.3, 16.8, 22.6, 30.0 against 14.4, 17.4, 18.6, 27.2
+    //   2 of 16 of 2048 x 1024 Bfp2_b  13.6, 15.3, 17.2, 22.9 against 14.7, 16.8, 17.8, 20.2
+    //   2 of 16 of 4096 x 1024 Bfp8_b  20.7, 30.0, 34.3, 43.8 against 22.8, 26.7, 28.3, 41.9
+    //   8 of 64 of 2048 x 1024 Bfp4_b  31.0, 51.4, 57.7, 79.4 against 26.5, 42.2, 44.3, 58.6
+    //   2 of 8 of 4096 x 2048 Bfp4_b   30.4, 38.9, 38.6, 41.2 against 26.1, 44.5, 37.6, 39.1
     const double miss = m.top < m.E ? 1.0 - (double)m.top / m.E : 0.0, reached = m.E * (1.0 - pow(miss, m.T));
     const double share = (double)slots / m.E;
-    const int nt = m.T == 1 ? 0 : m.T <= kOneSum || share <= 4.0 ? 1 : share <= 10.0 ? 2 : 4;
+    const int nt = m.T == 1 ? 0 : m.T <= 8 || share <= 6.0 ? 1 : share <= 10.0 ? 2 : 4;
     Args a = {};
     a.x = (const __nv_bfloat16 *)m.x; a.ldx = m.ldx;
     a.rows = m.T; a.K = m.H; a.Kt = Ht; a.N = m.I; a.Nt = It;
