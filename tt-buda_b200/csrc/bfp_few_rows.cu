@@ -29,10 +29,12 @@
 //   * The tile rows are split over the warps of a CTA and, where there are few columns, over a cluster of up to 8 CTAs;
 //     sums are joined through shared and distributed shared memory in a fixed order: no workspace, no atomics, the same bits
 //     every time.
-// Measured (B200): 1x4096x16384 Bfp4_b 8.5 us, 4.4 TB/s of its 37.8 MB, integer pipe 51 % active; 32x4096x16384 Bfp8_b 24.7 us;
-// the products of 16 tokens' 4 of 32 experts, 4096 x 2048 gated Bfp4_b, 114 us, 3.5 TB/s.
+// Measured (B200, images in turn that exceed L2 four times): 1x4096x16384 Bfp4_b 9.0 us, 4.2 TB/s of its 37.8 MB, integer pipe 50 %
+// active; 32x4096x16384 Bfp8_b 24.7 us, 2.9 TB/s; the products of 16 tokens' 4 of 32 experts, 4096 x 2048 gated Bfp4_b, 123 us,
+// 3.3 TB/s.
 // Sums are held in binary32 throughout, and so is h between the two launches: a lane cuts the values it loads into three bfloat16
-// pieces (8 bits of the significand each, exactly all 24), for three times the tensor work and a fifth more instructions.
+// pieces (8 bits of the significand each, exactly all 24), for three times the tensor work of the second product and a fifth more
+// instructions (the layer of those 32 experts takes 128 us; with two pieces, within 2^-16 of h, it took 119).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -54,8 +56,8 @@ enum { kMatvec = 0, kExpertsIn = 1, kExpertsOut = 2, kExpertsEach = 3 };
 enum { kUsual = 0, kPlain = 1, kWide = 2 };   // forms of a sweep (see products)
 __host__ __device__ constexpr bool from_h(int mode) { return mode == kExpertsOut || mode == kExpertsEach; }
 
-// How many units of 8 warps an SM holds, by registers: 128 a thread for up to 16 tokens in a pass.  9 to 16 tokens spill a little and
-// are the faster for twice the warps all the same (12x4096x16384 Bfp8_b 19.2 us against 20.7; 64 tokens, 4 of 32 experts of
+// How many units of 8 warps an SM holds, by registers: 128 a thread for up to 16 tokens in a pass.  Of 9 to 16 tokens that is too few
+// (Bfp8_b spills 256 bytes a thread in the product, 372 and 672 in the experts' launches), and twice the warps are the faster all the same (12x4096x16384 Bfp8_b 19.2 us against 20.7; 64 tokens, 4 of 32 experts of
 // 1024 x 2048 Bfp4_b 68-74 against 86-90).
 __host__ __device__ constexpr int units_per_sm(int nt) { return nt <= 2 ? 2 : 1; }
 
@@ -418,7 +420,9 @@ __device__ __forceinline__ void products(const Args &A, const Work &W, uint8_t *
     uint32_t seen = 0;                // all shared exponents met, ORed
 
     // One sweep over the share.  The first one takes every step as it usually is and looks afterwards whether one was not (an
-    // exponent of 128 or more, a sum that is no finite number): then all is done again with the exact wide steps.  The plain
+    // exponent of 128 or more, a sum that is no finite number): then all of the warp's share is done again with the exact wide steps,
+    // which load nothing ahead.  One such block makes 1x4096x16384 Bfp4_b take 14.9 us instead of 8.9, 32x4096x16384 Bfp8_b 40 instead
+    // of 25; blocks in every share 24 and 50, and 16 tokens' 4 of 32 experts 292 instead of 122.  The plain
     // form is for activations that are not aligned.  The usual form's loop has no test in it, so that the compiler schedules
     // two tile rows as one; the last rows, where activations may end inside a tile row, come behind it (1x4096x16384 Bfp4_b 9.8
     // -> 8.7 us).

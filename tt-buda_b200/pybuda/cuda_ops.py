@@ -234,8 +234,8 @@ def bfp8b_matmul(a, w_image, n, out=None):
 def bfp_matvec(a, w_image, n, w_df=DF.Bfp4_b, out=None, out_dtype=torch.bfloat16):
     """A @ W for a few rows: A bfloat16 [M,K] with M <= 64, W the Bfp8_b / Bfp4_b / Bfp2_b queue image of a [K,n] tensor
     (default geometry, no header; K and n that fill no tile: the image of the zero-padded tensor).  Returns [M,n] in
-    out_dtype (bfloat16 or float32), or writes `out` (dense rows, must not overlap a).  The image is read once for every 32 rows;
-    bfp8b_matmul is the one for many rows."""
+    out_dtype (bfloat16 or float32), or writes `out` (dense rows, must not overlap a).  The image is read once for every 32 rows
+    (again where weights of magnitude 2 and above are met, at up to three times the time); bfp8b_matmul is the one for many rows."""
     return _torch_ops.bfp_matvec(a, w_image, n, w_df, out, out_dtype)
 
 
