@@ -376,13 +376,15 @@ int buda_i8_gemm(const void *A, int64_t M, int64_t K, int64_t lda, const void *W
 
 /* ------------------------------------------------------------------ a few rows against block-float weights
  * Products of 1..64 rows (the tokens of a decoding step) with weights stored as block-float queue images, each weight read
- * once for every 32 rows, and once more by a part of the kernel that meets a shared exponent of 128 or more (a weight of magnitude 2
- * and above; such images are served exactly, at up to three times the time).  Images are those of buda_bfp8b_gemm, for Bfp8_b, Bfp4_b and Bfp2_b alike: geometry grid 1x1, ublock 1x1, order R,
- * no tile header, default byte layout, 32-byte aligned; sizes that fill no tile are padded to whole tiles (with zeros, as
- * the pack writes them).  Every stored weight counts at its exact value (from 2^128 on that is an infinity, as in the unpack), sums
- * are binary32, and so is what the experts carry from one product to the next.  Results do not depend on
- * what else runs: the same call gives the same bits.  Launches begin early and wait for what stands in front of them in
- * the stream before they read anything that it may write: any argument may be the result of the launch before.  K, N, H, I <= 2^24. */
+ * once for every 32 rows, and once more by a part of the kernel that meets a shared exponent of 128 or more (a weight of
+ * magnitude 2 and above; such images are served exactly, at up to three times the time).
+ * Images are those of buda_bfp8b_gemm, for Bfp8_b, Bfp4_b and Bfp2_b alike: geometry grid 1x1, ublock 1x1, order R, no tile
+ * header, default byte layout, 32-byte aligned; sizes that fill no tile are padded to whole tiles (with zeros, as the pack
+ * writes them).  Every stored weight counts at its exact value (from 2^128 on that is an infinity, as in the unpack); sums are
+ * binary32 (of a single row, a product below 2^-102 counts in steps of 2^-125), and so is what the experts carry from one product
+ * to the next.  Results do not depend on what else runs: the same call gives the same bits.  Launches begin early and wait for
+ * what stands in front of them in the stream before they read anything that it may write: any argument may be the result of
+ * the launch before.  K, N, H, I <= 2^24. */
 #define BUDA_MAX_FEW_ROWS 64
 
 /* Y[M,N] (BUDA_DF_Float16_b or BUDA_DF_Float32, row stride ldy elements) = A[M,K] (bfloat16, row stride lda elements) @ W,

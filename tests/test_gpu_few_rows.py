@@ -986,3 +986,28 @@ def test_route_rows_too_long_to_be_staged(ops, router, t, h, e, top):
     # a score is off by 7 * 2^-24 of its products' magnitudes at most, a weight by twice that and a few units of 2^-24
     mag = (x.double().abs() @ w.double().abs().T).max().item()
     assert (np.abs(weights.double().cpu().numpy() - ref) <= (14 * mag + 8) * 2.0 ** -24 * ref).all()
+
+
+_OUT_OF_MEMORY = """
+import sys
+sys.path[:0] = {path!r}
+import torch
+from pybuda import cuda_ops as ops
+a, img = torch.ones(64, 32, device="cuda").bfloat16(), torch.zeros(1 << 15, 320, dtype=torch.uint8, device="cuda").view(-1)
+torch.cuda.set_per_process_memory_fraction(2 ** 26 / torch.cuda.get_device_properties(0).total_memory)
+try:
+    ops.bfp_matvec(a, img, 1 << 20, ops.DF.Bfp2_b, out_dtype=torch.float32)
+except torch.OutOfMemoryError:
+    y = ops.bfp_matvec(a, img, 1 << 10, ops.DF.Bfp2_b)
+    assert torch.all(y == 0)
+    print("out of memory said so")
+"""
+
+
+def test_results_that_do_not_fit_raise_torchs_out_of_memory_error():
+    """The allocator's limit for this process stands in for a full device."""
+    import subprocess
+    import sys
+
+    r = subprocess.run([sys.executable, "-c", _OUT_OF_MEMORY.format(path=[p for p in sys.path if p])], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "out of memory said so" in r.stdout, r.stderr[-2000:]

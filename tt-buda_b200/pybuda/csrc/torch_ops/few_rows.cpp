@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdarg>
@@ -145,8 +146,8 @@ PyObject *guarded(Py_ssize_t got, Py_ssize_t want, F body)
         if (got != want) refuse("takes %zd arguments", want);
         return body();
     } catch (const Refused &) {
-    } catch (const std::exception &e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {                        // torch's own: memory that ran out is torch.OutOfMemoryError
+        torch::translate_exception_to_python(std::current_exception());
     }
     return nullptr;
 }
